@@ -63,7 +63,7 @@ namespace vkllama {
 namespace absl = ::absl_shim;
 
 // src/core/common.h:15-22
-typedef enum : int { FP32 = 0, FP16, UINT32, INT8, Q8_0 } DType;
+typedef enum : int { FP32 = 0, FP16, UINT32, INT8, Q8_0, BF16 } DType;
 
 #define VKLLAMA_STATUS_OK(__expr)              \
   if (auto __s = (__expr); !__s.ok()) {        \
@@ -412,6 +412,58 @@ class ReadKVCache : public Op {
   absl::StatusOr<Tensor> operator()(Tensor cache, uint32_t offset, uint32_t len) noexcept {
     vkl_tensor *o = nullptr;
     const int st = vkl_read_kvcache_run(op_, cache.handle(), offset, len, &o);
+    return out(st, o);
+  }
+};
+
+// A key-value cache in pages that many sequences share (vkllama_b200.h); no counterpart in the reference.
+class PagedTables : public Op {
+ public:
+  struct Rows {
+    Tensor map, starts;
+  };
+  PagedTables(GPUDevice *dev, Command *command, const int page_size) : Op(dev, command) {
+    vkl_paged_tables_create(dev->handle(), command->handle(), page_size, &op_);
+  }
+  absl::StatusOr<Rows> operator()(Tensor lengths, Tensor target, Tensor table, Tensor pool, size_t rows) noexcept {
+    vkl_tensor *m = nullptr, *s = nullptr;
+    const int st = vkl_paged_tables_run(op_, lengths.handle(), target.handle(), table.handle(), pool.handle(), rows, &m, &s);
+    if (st != VKL_OK) return ToStatus(st);
+    return Rows{Tensor::Borrow(m, dev_), Tensor::Borrow(s, dev_)};
+  }
+};
+
+class UpdatePagedKVCache : public Op {
+ public:
+  UpdatePagedKVCache(GPUDevice *dev, Command *command, const int dim, const int page_size, const float theta = 10000.0f, Tensor::DType dtype = FP16)
+      : Op(dev, command) {
+    vkl_update_paged_kvcache_create(dev->handle(), command->handle(), dim, page_size, theta, dtype, &op_);
+  }
+  absl::Status operator()(Tensor kcache, Tensor vcache, Tensor k, Tensor v, Tensor map) noexcept {
+    return ToStatus(vkl_update_paged_kvcache_run(op_, kcache.handle(), vcache.handle(), k.handle(), v.handle(), map.handle(), nullptr, nullptr));
+  }
+  absl::StatusOr<Tensor> operator()(Tensor kcache, Tensor vcache, Tensor k, Tensor v, Tensor map, Tensor q) noexcept {  // the queries, rotated
+    vkl_tensor *o = nullptr;
+    const int st = vkl_update_paged_kvcache_run(op_, kcache.handle(), vcache.handle(), k.handle(), v.handle(), map.handle(), q.handle(), &o);
+    return out(st, o);
+  }
+};
+
+class PagedAttention : public Op {
+ public:
+  PagedAttention(GPUDevice *dev, Command *command, const int heads, const int kv_heads, const int dim, const int page_size, const float scale = 0.0f,
+                 const int window = 0, Tensor::DType dtype = FP16)
+      : Op(dev, command) {
+    vkl_paged_attention_create(dev->handle(), command->handle(), heads, kv_heads, dim, page_size, scale, window, dtype, &op_);
+  }
+  absl::StatusOr<Tensor> operator()(Tensor q, Tensor kcache, Tensor vcache, Tensor table, Tensor lengths) noexcept {  // one new token each
+    vkl_tensor *o = nullptr;
+    const int st = vkl_paged_attention_run(op_, q.handle(), kcache.handle(), vcache.handle(), table.handle(), lengths.handle(), nullptr, &o);
+    return out(st, o);
+  }
+  absl::StatusOr<Tensor> operator()(Tensor q, Tensor kcache, Tensor vcache, Tensor table, Tensor lengths, Tensor starts) noexcept {
+    vkl_tensor *o = nullptr;
+    const int st = vkl_paged_attention_run(op_, q.handle(), kcache.handle(), vcache.handle(), table.handle(), lengths.handle(), starts.handle(), &o);
     return out(st, o);
   }
 };

@@ -31,7 +31,7 @@ typedef struct vkl_gguf vkl_gguf;
 typedef struct vkl_sampler vkl_sampler;
 
 /* src/core/common.h:15-22 (enum DType), same numeric values; BF16 is this library's own
- * (weights and activations of the layer-list decoder designs, not an operand of the ops). */
+ * (weights and activations of the layer-list decoder designs, and of the operators of a paged cache). */
 enum vkl_dtype { VKL_FP32 = 0, VKL_FP16 = 1, VKL_UINT32 = 2, VKL_INT8 = 3, VKL_Q8_0 = 4, VKL_BF16 = 5 };
 
 /* absl::StatusCode values used by the reference's ops. */
@@ -199,6 +199,55 @@ int vkl_slice_run(vkl_op *op, vkl_tensor *in, const uint32_t starts[3],
 /* Cast, src/ops/cast.h:15-20 (FP16 -> FP32 and FP32 -> FP16). */
 int vkl_cast_create(vkl_device *dev, vkl_command *cmd, int from, int to, vkl_op **out);
 int vkl_cast_run(vkl_op *op, vkl_tensor *in, vkl_tensor **out);
+
+/* ---- a key-value cache in pages, shared by many sequences. No counterpart in the reference, whose caches
+ * (UpdateKVCache, ReadKVCache, MultiHeadAttentionV2) hold one sequence each. dtype is VKL_FP16 or VKL_BF16 throughout.
+ *
+ *   cache   [pages, kv_heads * page_size, dim], dense, keys and values apart: a page holds page_size tokens, row
+ *           g * page_size + r is key head g of its token r. At most 2^32 - 2 rows.
+ *   table   UINT32 [1, n, width]: row i holds the pages of sequence i in order, its token j lies in page
+ *           table[i][j / page_size], row j % page_size. Entries behind a sequence's last page are not read. Sequences may share
+ *           pages for reading.
+ *   lengths UINT32 [1, 1, n]: tokens of every sequence.
+ *   map     UINT32 [1, 2, rows]: row 0 the slots (page * page_size + r) of the pass's new tokens, 0xffffffff for none; row 1 their positions.
+ *   starts  UINT32 [1, 1, n + 1]: sequence i's new tokens are the rows starts[i] .. starts[i + 1] of the pass.
+ *
+ * What only the device can see (a page number beyond the cache, lengths beyond the table, an empty pool) is checked there; nothing outside
+ * the tensors is touched, and the next vkl_command_wait returns the error. The calls of ONE op share its outputs and workspace: they must not
+ * overlap on the GPU, also not as replays of captured graphs. After a first call of the same shape a call allocates nothing and
+ * can be captured (vkl_command_stream); the error word is then read by the wait of the next directly recorded call.
+ *
+ * PagedTables: gives and takes pages so that every sequence has pages for target[i] tokens, and names the slots of its new ones. Sequences may
+ * grow, shrink (to 0: finished; by some: tokens taken back) or stay in one call; lengths becomes target.
+ * pool UINT32 [1, 1, 1 + capacity]: pool[0] free pages, which are pool[1 .. pool[0]]; the last one is taken first, in order of
+ * sequences, and what comes back goes on top in the reverse order, so taking pages and giving them back restores the pool.
+ * `rows` (a host number) is how many rows the pass has; rows behind the last new token get no slot. A call that cannot be carried out
+ * whole (RESOURCE_EXHAUSTED: not enough pages; OUT_OF_RANGE: a target beyond the table, more new tokens than rows) changes nothing and
+ * gives no row a slot. At most 8192 sequences. Pages are owned by one sequence here: a shared one would be given back twice. */
+int vkl_paged_tables_create(vkl_device *dev, vkl_command *cmd, int page_size, vkl_op **out);
+int vkl_paged_tables_run(vkl_op *op, vkl_tensor *lengths, vkl_tensor *target, vkl_tensor *table, vkl_tensor *pool, size_t rows,
+                         vkl_tensor **map, vkl_tensor **starts);
+/* UpdatePagedKVCache: writes the rows k, v [1, rows, kv_heads * dim] to their slots, the keys rotated by their positions as Rope rotates
+ * (neighbouring pairs, angle position * theta^(-2k/dim), angles in 64 bits); theta 0: not rotated. Rows without a slot are not written.
+ * q [1, rows, heads * dim], or NULL: rotated into the op's output (rows without a slot by their map's position as well). k, v and q may be views of wider
+ * rows whose rows start at multiples of 16 bytes. Slots of one call must differ: of two rows with one slot either may be
+ * stored, piece by piece. dim: a multiple of 8 up to 256. */
+int vkl_update_paged_kvcache_create(vkl_device *dev, vkl_command *cmd, int dim, int page_size, float theta, int dtype, vkl_op **out);
+int vkl_update_paged_kvcache_run(vkl_op *op, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *k, vkl_tensor *v, vkl_tensor *map,
+                                 vkl_tensor *q, vkl_tensor **out);
+/* PagedAttention: softmax(scale q k^T) v over each sequence's cached tokens, the new ones' keys and values among them. heads: a multiple of
+ * kv_heads, query head h reads key head h / (heads / kv_heads). scale 0: 1 / sqrt(dim). window > 0: a token sees the last `window`
+ * positions up to its own. fp32 sums and softmax, one rounding of the output (with `starts` also of the probabilities, to dtype).
+ *   starts NULL: one new token per sequence, q [1, n, heads * dim], row i the last token of sequence i (position lengths[i] - 1); a sequence
+ *   of no tokens gives zeros.
+ *   else q [1, rows, heads * dim]: sequence i's new tokens are the last starts[i + 1] - starts[i] of its lengths[i]; each sees the
+ *   positions up to its own. Sequences without new rows are skipped; output rows that belong to no sequence are left as they were.
+ * q may be a view of wider rows (16-byte row starts). Values at positions that a row does not see never reach it, whatever they
+ * are. In the one-token form an infinite value that weighs less than 2^-25 may come out as NaN. */
+int vkl_paged_attention_create(vkl_device *dev, vkl_command *cmd, int heads, int kv_heads, int dim, int page_size, float scale, int window,
+                               int dtype, vkl_op **out);
+int vkl_paged_attention_run(vkl_op *op, vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths,
+                            vkl_tensor *starts, vkl_tensor **out);
 
 /* Row arg-max that allocates nothing. No counterpart in the reference.
  * For callers that cannot allocate device memory where they need the greedy pick

@@ -11,6 +11,7 @@ from .api import (  # noqa: F401
     VklError, Device, Tensor, Command,
     MatMul, FeedForward, MultiHeadAttentionV2, UpdateKVCache, RMSNorm, Rope, Softmax,
     ArgOp, ArgMax, ArgMin, Embedding, ElementWise, Transpose, Slice, Cast, Concat, Reduce, ReadKVCache,
+    PagedTables, UpdatePagedKVCache, PagedAttention,
     Model, ModelConfig, q8_0_quantize, q8_0_quantize36, q8_0_dequantize, blocks36_to_34,
     kernel_launches, library_path, load_library, matmul_run_many,
     load_model, architectures, distance_bucket, Gguf, Sampler, TopkSampler, TopPSampler,

@@ -76,6 +76,11 @@ def load_library():
         "vkl_argop_create": [vp, vp, i32, i32, pvp], "vkl_argop_run": [vp, vp, pvp],
         "vkl_embedding_create": [vp, vp, vp, u32, i32, pvp], "vkl_embedding_run": [vp, vp, pvp],
         "vkl_elementwise_create": [vp, vp, i32, i32, pvp], "vkl_elementwise_run": [vp, vp, vp, pvp],
+        "vkl_paged_tables_create": [vp, vp, i32, pvp], "vkl_paged_tables_run": [vp, vp, vp, vp, vp, sz, pvp, pvp],
+        "vkl_update_paged_kvcache_create": [vp, vp, i32, i32, f32, i32, pvp],
+        "vkl_update_paged_kvcache_run": [vp, vp, vp, vp, vp, vp, vp, pvp],
+        "vkl_paged_attention_create": [vp, vp, i32, i32, i32, i32, f32, i32, i32, pvp],
+        "vkl_paged_attention_run": [vp, vp, vp, vp, vp, vp, vp, pvp],
         "vkl_transpose_create": [vp, vp, i32, i32, pvp], "vkl_transpose_run": [vp, vp, pvp],
         "vkl_slice_create": [vp, vp, i32, pvp],
         "vkl_slice_run": [vp, vp, C.POINTER(u32), C.POINTER(u32), pvp],
@@ -575,6 +580,48 @@ class ReadKVCache(Op):
     def __call__(self, cache, offset, length):
         out = vp()
         _ck(self.L.vkl_read_kvcache_run(self.h, cache.h, offset, length, C.byref(out)))
+        return self._out(out)
+
+
+class PagedTables(Op):
+    """Page tables and slots of sequences that grow or shrink, over a pool of free pages (include/vkllama_b200.h)."""
+
+    def __init__(self, dev, command, page_size):
+        super().__init__(dev, command)
+        _ck(self.L.vkl_paged_tables_create(dev.h, command.h, page_size, C.byref(self.h)))
+
+    def __call__(self, lengths, target, table, pool, rows):
+        """lengths becomes target, table and pool follow. Returns the map [1, 2, rows] (slots, positions) and starts [1, 1, n + 1]
+        of the new tokens."""
+        m, s = vp(), vp()
+        _ck(self.L.vkl_paged_tables_run(self.h, _h(lengths), _h(target), _h(table), _h(pool), rows, C.byref(m), C.byref(s)))
+        return self._out(m), self._out(s)
+
+
+class UpdatePagedKVCache(Op):
+    """New keys and values into the pages of their sequences, keys (and queries) rotated by their positions on the way."""
+
+    def __init__(self, dev, command, dim, page_size, theta=10000.0, dtype=FP16):
+        super().__init__(dev, command)
+        _ck(self.L.vkl_update_paged_kvcache_create(dev.h, command.h, dim, page_size, theta, dtype, C.byref(self.h)))
+
+    def __call__(self, kcache, vcache, k, v, map, q=None):
+        """Returns the rotated queries, or None where there are none."""
+        out = vp()
+        _ck(self.L.vkl_update_paged_kvcache_run(self.h, _h(kcache), _h(vcache), _h(k), _h(v), _h(map), _h(q), C.byref(out)))
+        return self._out(out) if q is not None else None
+
+
+class PagedAttention(Op):
+    """Attention over a paged cache: of one new token per sequence, or of the rows that `starts` gives every sequence."""
+
+    def __init__(self, dev, command, heads, kv_heads, dim, page_size, scale=0.0, window=0, dtype=FP16):
+        super().__init__(dev, command)
+        _ck(self.L.vkl_paged_attention_create(dev.h, command.h, heads, kv_heads, dim, page_size, scale, window, dtype, C.byref(self.h)))
+
+    def __call__(self, q, kcache, vcache, table, lengths, starts=None):
+        out = vp()
+        _ck(self.L.vkl_paged_attention_run(self.h, _h(q), _h(kcache), _h(vcache), _h(table), _h(lengths), _h(starts), C.byref(out)))
         return self._out(out)
 
 

@@ -8,49 +8,11 @@
 #include <algorithm>
 #include <cmath>
 
-#include "runtime.h"
+#include "op.h"
 
 using namespace vkl;
 
-struct vkl_op {
-  vkl_device *dev;
-  vkl_command *cmd;
-  bool inited = false;
-  cudaEvent_t e0 = nullptr, e1 = nullptr;
-  bool timed = false;
-  vkl_op(vkl_device *d, vkl_command *c) : dev(d), cmd(c) {}
-  virtual int init() = 0;
-  virtual ~vkl_op() {
-    if (e0) cudaEventDestroy(e0);
-    if (e1) cudaEventDestroy(e1);
-  }
-  int base_init() {
-    if (!dev || !cmd) return fail(VKL_INVALID_ARGUMENT, "op: null device or command");
-    VKL_CUDA(cudaEventCreate(&e0));
-    VKL_CUDA(cudaEventCreate(&e1));
-    inited = true;
-    return VKL_OK;
-  }
-  int enter(const char *who) {
-    if (!inited) return fail(VKL_FAILED_PRECONDITION, "%s: init() was not called", who);
-    VKL_OKAY(recording(cmd, who));
-    VKL_CUDA(cudaEventRecord(e0, cmd->stream));
-    return VKL_OK;
-  }
-  int leave() {
-    VKL_CUDA(cudaEventRecord(e1, cmd->stream));
-    timed = true;
-    return VKL_OK;
-  }
-};
-
 namespace {
-
-int need_dense(const vkl_tensor *t, const char *who) {
-  if (!t) return fail(VKL_INVALID_ARGUMENT, "%s: null tensor", who);
-  if (!t->dense()) return fail(VKL_UNIMPLEMENTED, "%s: strided views are not supported by this op", who);
-  return VKL_OK;
-}
 
 // -------------------------------------------------------------------- MatMul
 struct MatMulOp : vkl_op {
@@ -754,15 +716,6 @@ struct CastOp : vkl_op {
     return leave();
   }
 };
-
-template <class T>
-int as(vkl_op *op, T **out, const char *who) {
-  if (!op) return fail(VKL_INVALID_ARGUMENT, "%s: null op", who);
-  T *t = dynamic_cast<T *>(op);
-  if (!t) return fail(VKL_INVALID_ARGUMENT, "%s: handle is another kind of op", who);
-  *out = t;
-  return VKL_OK;
-}
 
 }  // namespace
 

@@ -1,0 +1,93 @@
+// A key-value cache in pages that many sequences share: what its operators' launchers take.
+//
+// cache   [pages][kv_heads][page][dim], keys and values apart, fp16 or bf16
+// table   [sequences][width]: a sequence's pages in order; position j is row j % page of page table[j / page]
+// slot    page * page_size + row of a token, or kNoSlot
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace vkl {
+
+constexpr uint32_t kNoSlot = 0xffffffffu;
+
+// What a kernel found on the device that the host could not see, in the command's error word (wait() reports it). Waits inside
+// kernels that ran out have codes below 0x100.
+enum PagedError : uint32_t {
+  PAGED_POOL_EMPTY = 0x101,  // tables: more pages are needed than the pool holds
+  PAGED_TABLE_FULL,          // a sequence is longer than a row of its table
+  PAGED_ROWS,                // tables: more new rows than the call has room for
+  PAGED_POOL_BAD,            // tables: the pool's count and what comes back do not fit it
+  PAGED_BAD_PAGE,            // a page that the cache does not have
+  PAGED_BAD_ROWS,            // attention: starts and lengths do not belong together
+};
+
+// n / d for n < 2^31 by a multiplication.
+struct Divisor {
+  uint32_t d, mul, shift;
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s};
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor &v) { return (__umulhi(n, v.mul) + n) >> v.shift; }
+__device__ __forceinline__ void raise(uint32_t *error, uint32_t code) { atomicCAS(error, 0u, code); }
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+#endif
+
+struct PagedTables {
+  uint32_t *lengths;       // [n], becomes target
+  const uint32_t *target;  // [n]
+  uint32_t *table;         // [n][width]
+  uint32_t *pool;          // [0] count, then the free pages, the next one to be taken last
+  uint32_t *map;           // [2][rows]: slots, positions of the new rows
+  uint32_t *starts;        // [n + 1] first new row of every sequence
+  uint32_t *arrived;       // CTAs that are through; 0 between launches
+  uint32_t *error;
+  uint32_t n, width, capacity, rows;
+  Divisor page;
+};
+constexpr uint32_t kTablesMaxSequences = 8192;
+cudaError_t launch_paged_tables(const PagedTables &p, uint32_t sms, cudaStream_t s);
+cudaError_t setup_paged_tables();  // once per device
+
+struct PagedUpdate {
+  const void *q, *k, *v;        // [rows] of heads * dim, kv_heads * dim values, apart by q_ld, ... values; q may be null
+  void *q_out;                  // [rows][heads * dim]
+  void *kcache, *vcache;
+  const uint32_t *map;          // [2][rows]
+  uint32_t *error;
+  uint64_t q_ld, k_ld, v_ld;
+  uint32_t rows, heads, kv_heads, dim, pages;
+  Divisor page;
+  const double *turns;          // [dim / 2] turns of a pair per position, or null: no rotation
+  bool bf;
+};
+cudaError_t launch_paged_update(const PagedUpdate &p, cudaStream_t s);
+
+struct PagedAttention {
+  const void *q;                // [rows] of heads * dim values, q_ld apart
+  const void *kcache, *vcache;
+  void *out;                    // [rows][heads * dim]
+  const uint32_t *table, *lengths;
+  const uint32_t *starts;       // [n + 1], or null: row i is the last token of sequence i
+  float *scratch;               // partial results, paged_token_scratch() bytes
+  uint32_t *counters;           // [SMs + 1], 0 between launches
+  uint32_t *error;
+  uint64_t q_ld;
+  uint32_t rows, n, heads, kv_heads, dim, width, pages, window;
+  Divisor page;
+  float scale;                  // on the scores
+  bool bf;
+};
+// One new token per sequence.
+cudaError_t launch_paged_token(const PagedAttention &p, uint32_t sms, cudaStream_t s);
+size_t paged_token_scratch(uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t sms);
+cudaError_t setup_paged_token();   // once per device
+// Any number of rows per sequence.
+cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStream_t s);
+cudaError_t setup_paged_prompt();
+
+}  // namespace vkl

@@ -1,0 +1,304 @@
+// The operators of a key-value cache in pages (paged.h): argument checks, outputs, launches.
+#include <math.h>
+
+#include <cmath>
+#include <new>
+
+#include "op.h"
+#include "paged.h"
+
+using namespace vkl;
+
+namespace {
+
+constexpr uint64_t kMaxTokens = 0x7fffffffu;  // of a sequence, so that positions and their quotients stay in 32 bits
+
+// The op's device is current while it launches, whatever the caller's thread has current.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(int ordinal) {
+    if (cudaGetDevice(&before) != cudaSuccess || before == ordinal || cudaSetDevice(ordinal) != cudaSuccess) before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+struct PagedOp : vkl_op {
+  using vkl_op::vkl_op;
+  int check(const vkl_tensor *t, const char *who, const char *name, int dtype, bool dense = true) {
+    if (!t) return fail(VKL_INVALID_ARGUMENT, "%s: null %s", who, name);
+    if (t->dev->ordinal != dev->ordinal) return fail(VKL_INVALID_ARGUMENT, "%s: %s is on device %d, the op on device %d", who, name, t->dev->ordinal, dev->ordinal);
+    if (t->dtype != dtype) return fail(VKL_INVALID_ARGUMENT, "%s: %s has dtype %d, expected %d", who, name, t->dtype, dtype);
+    if (dense && !t->dense()) return fail(VKL_UNIMPLEMENTED, "%s: %s must be dense", who, name);
+    return VKL_OK;
+  }
+  int check_list(const vkl_tensor *t, const char *who, const char *name, size_t n) {
+    VKL_OKAY(check(t, who, name, VKL_UINT32));
+    if (t->c != 1 || t->h != 1 || t->w != n)
+      return fail(VKL_INVALID_ARGUMENT, "%s: %s has shape (%zu, %zu, %zu), expected (1, 1, %zu)", who, name, t->c, t->h, t->w, n);
+    return VKL_OK;
+  }
+  // Rows of `w` values, possibly apart (a view of wider rows).
+  int check_rows(const vkl_tensor *t, const char *who, const char *name, int dtype) {
+    VKL_OKAY(check(t, who, name, dtype, false));
+    if (t->c != 1) return fail(VKL_INVALID_ARGUMENT, "%s: %s has %zu channels, expected 1", who, name, t->c);
+    if (t->h > kMaxTokens) return fail(VKL_OUT_OF_RANGE, "%s: %zu rows", who, t->h);
+    return VKL_OK;
+  }
+  int check_apart(const vkl_tensor *t, const char *who, const char *name) {
+    if (t->h > 1 && t->hs % 16) return fail(VKL_UNIMPLEMENTED, "%s: rows of %s are %zu bytes apart, which is no multiple of 16", who, name, t->hs);
+    return VKL_OK;
+  }
+  int check_cache(const vkl_tensor *k, const vkl_tensor *v, const char *who, int dtype, size_t kv_heads, size_t page, size_t dim) {
+    VKL_OKAY(check(k, who, "key cache", dtype));
+    VKL_OKAY(check(v, who, "value cache", dtype));
+    if (k->c != v->c || k->h != v->h || k->w != v->w || k->h != kv_heads * page || k->w != dim)
+      return fail(VKL_INVALID_ARGUMENT, "%s: caches have shapes (%zu, %zu, %zu) and (%zu, %zu, %zu), expected (pages, %zu, %zu)", who, k->c, k->h, k->w, v->c, v->h,
+                  v->w, kv_heads * page, dim);
+    if (k->c * k->h >= 0xffffffffu) return fail(VKL_OUT_OF_RANGE, "%s: a cache of %zu rows; at most 2^32 - 2 can be named", who, k->c * k->h);
+    return VKL_OK;
+  }
+  int check_table(const vkl_tensor *t, const char *who, size_t page) {
+    VKL_OKAY(check(t, who, "table", VKL_UINT32));
+    if (t->c != 1) return fail(VKL_INVALID_ARGUMENT, "%s: the table has %zu channels, expected 1", who, t->c);
+    if (t->w * page > kMaxTokens) return fail(VKL_OUT_OF_RANGE, "%s: a table of %zu pages of %zu tokens; a sequence has at most 2^31 - 1", who, t->w, page);
+    return VKL_OK;
+  }
+};
+
+bool good_page(int page) { return page >= 1 && page <= 1 << 20; }
+bool good_dim(int dim) { return dim >= 8 && dim <= 256 && dim % 8 == 0; }
+bool good_dtype(int dtype) { return dtype == VKL_FP16 || dtype == VKL_BF16; }
+
+// -------------------------------------------------------------- PagedTables
+struct PagedTablesOp : PagedOp {
+  int page;
+  vkl_tensor *map = nullptr, *starts = nullptr, *arrived = nullptr;
+  PagedTablesOp(vkl_device *d, vkl_command *c, int pg) : PagedOp(d, c), page(pg) {}
+  ~PagedTablesOp() override {
+    for (vkl_tensor *t : {map, starts, arrived}) vkl_tensor_release(t);
+  }
+  int init() override {
+    if (inited) return VKL_OK;
+    if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "PagedTables op: a page of %d tokens", page);
+    VKL_CUDA(setup_paged_tables());
+    VKL_OKAY(tensor_new(dev, 1, 1, 1, VKL_UINT32, &arrived));
+    VKL_CUDA(cudaMemsetAsync(arrived->data(), 0, 4, cmd->stream));
+    uint32_t *word;
+    VKL_OKAY(command_error_word(cmd, &word));  // allocated here, so that run() does not have to
+    return base_init();
+  }
+  int run(vkl_tensor *lengths, vkl_tensor *target, vkl_tensor *table, vkl_tensor *pool, size_t rows, vkl_tensor **o_map, vkl_tensor **o_starts) {
+    const char *who = "paged_tables";
+    OnDevice here(dev->ordinal);
+    VKL_OKAY(check_table(table, who, page));
+    const size_t n = table->h;
+    VKL_OKAY(check_list(lengths, who, "lengths", n));
+    VKL_OKAY(check_list(target, who, "target", n));
+    VKL_OKAY(check(pool, who, "pool", VKL_UINT32));
+    if (pool->c != 1 || pool->h != 1 || pool->w < 1) return fail(VKL_INVALID_ARGUMENT, "%s: the pool has shape (%zu, %zu, %zu), expected (1, 1, 1 + pages)", who, pool->c, pool->h, pool->w);
+    if (n > kTablesMaxSequences) return fail(VKL_OUT_OF_RANGE, "%s: %zu sequences, at most %u", who, n, kTablesMaxSequences);
+    if (rows > kMaxTokens || pool->w > kMaxTokens) return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, a pool of %zu pages", who, rows, pool->w - 1);
+    VKL_OKAY(enter(who));
+    VKL_OKAY(ensure_tensor(dev, &map, 1, 2, rows, VKL_UINT32));
+    VKL_OKAY(ensure_tensor(dev, &starts, 1, 1, n + 1, VKL_UINT32));
+    PagedTables p = {};
+    p.lengths = (uint32_t *)lengths->data();
+    p.target = (const uint32_t *)target->data();
+    p.table = (uint32_t *)table->data();
+    p.pool = (uint32_t *)pool->data();
+    p.map = (uint32_t *)map->data();
+    p.starts = (uint32_t *)starts->data();
+    p.arrived = (uint32_t *)arrived->data();
+    VKL_OKAY(command_error_word(cmd, &p.error));
+    p.n = (uint32_t)n, p.width = (uint32_t)table->w, p.capacity = (uint32_t)pool->w - 1, p.rows = (uint32_t)rows;
+    p.page = divisor(page);
+    VKL_LAUNCH(1, launch_paged_tables(p, dev->prop.multiProcessorCount, cmd->stream));
+    if (o_map) *o_map = map;
+    if (o_starts) *o_starts = starts;
+    return leave();
+  }
+};
+
+// ------------------------------------------------------- UpdatePagedKVCache
+struct UpdatePagedOp : PagedOp {
+  int dim, page, dtype;
+  float theta;
+  vkl_tensor *turns = nullptr, *out = nullptr;
+  UpdatePagedOp(vkl_device *d, vkl_command *c, int dm, int pg, float th, int dt) : PagedOp(d, c), dim(dm), page(pg), dtype(dt), theta(th) {}
+  ~UpdatePagedOp() override {
+    vkl_tensor_release(turns);
+    vkl_tensor_release(out);
+  }
+  int init() override {
+    if (inited) return VKL_OK;
+    if (!good_dtype(dtype)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: only fp16 and bf16 dtypes are supported.");
+    if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: a page of %d tokens", page);
+    if (!good_dim(dim)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: head dim %d is no multiple of 8 up to 256", dim);
+    if (theta != 0.f && !(theta >= 1.f && theta <= 1e30f)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: theta is %g", theta);
+    if (theta != 0.f) {
+      std::vector<double> per(dim / 2);
+      for (int k = 0; k < dim / 2; ++k) per[k] = std::pow((double)theta, -2.0 * k / dim) / (2.0 * std::acos(-1.0));
+      VKL_OKAY(tensor_new(dev, 1, 1, dim, VKL_FP32, &turns));
+      VKL_CUDA(cudaMemcpyAsync(turns->data(), per.data(), per.size() * 8, cudaMemcpyHostToDevice, cmd->stream));
+      VKL_CUDA(cudaStreamSynchronize(cmd->stream));
+    }
+    uint32_t *word;
+    VKL_OKAY(command_error_word(cmd, &word));
+    return base_init();
+  }
+  int run(vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *k, vkl_tensor *v, vkl_tensor *map, vkl_tensor *q, vkl_tensor **o) {
+    const char *who = "update_paged_kvcache";
+    OnDevice here(dev->ordinal);
+    VKL_OKAY(check_rows(k, who, "keys", dtype));
+    VKL_OKAY(check_rows(v, who, "values", dtype));
+    if (k->h != v->h || k->w != v->w || k->w == 0 || k->w % dim)
+      return fail(VKL_INVALID_ARGUMENT, "%s: keys have shape (%zu, %zu, %zu), values (%zu, %zu, %zu), heads are %d wide", who, k->c, k->h, k->w, v->c, v->h, v->w, dim);
+    const size_t rows = k->h, kv_heads = k->w / dim;
+    if (q) {
+      VKL_OKAY(check_rows(q, who, "queries", dtype));
+      if (q->h != rows || q->w == 0 || q->w % dim)
+        return fail(VKL_INVALID_ARGUMENT, "%s: queries have shape (%zu, %zu, %zu) beside %zu keys, heads are %d wide", who, q->c, q->h, q->w, rows, dim);
+    }
+    VKL_OKAY(check_cache(kcache, vcache, who, dtype, kv_heads, page, dim));
+    VKL_OKAY(check(map, who, "map", VKL_UINT32));
+    if (map->c != 1 || map->h != 2 || map->w != rows)
+      return fail(VKL_INVALID_ARGUMENT, "%s: the map has shape (%zu, %zu, %zu), expected (1, 2, %zu)", who, map->c, map->h, map->w, rows);
+    VKL_OKAY(check_apart(k, who, "keys"));
+    VKL_OKAY(check_apart(v, who, "values"));
+    if (q) VKL_OKAY(check_apart(q, who, "queries"));
+    if ((q ? q->w : 0) + 2 * k->w > 1u << 24) return fail(VKL_OUT_OF_RANGE, "%s: rows of %zu values", who, (q ? q->w : 0) + 2 * k->w);
+    VKL_OKAY(enter(who));
+    if (q) VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
+    if (rows) {
+      PagedUpdate p = {};
+      p.k = k->data(), p.v = v->data();
+      p.k_ld = k->hs / 2, p.v_ld = v->hs / 2;
+      if (q) {
+        p.q = q->data(), p.q_out = out->data();
+        p.q_ld = q->hs / 2;
+        p.heads = (uint32_t)(q->w / dim);
+      }
+      p.kcache = kcache->data(), p.vcache = vcache->data();
+      p.map = (const uint32_t *)map->data();
+      VKL_OKAY(command_error_word(cmd, &p.error));
+      p.rows = (uint32_t)rows, p.kv_heads = (uint32_t)kv_heads, p.dim = (uint32_t)dim, p.pages = (uint32_t)kcache->c;
+      p.page = divisor(page);
+      p.turns = turns ? (const double *)turns->data() : nullptr;
+      p.bf = dtype == VKL_BF16;
+      VKL_LAUNCH(1, launch_paged_update(p, cmd->stream));
+    }
+    if (o) *o = q ? out : nullptr;
+    return leave();
+  }
+};
+
+// ------------------------------------------------------------ PagedAttention
+struct PagedAttentionOp : PagedOp {
+  int heads, kv_heads, dim, page, window, dtype;
+  float scale;
+  vkl_tensor *out = nullptr, *scratch = nullptr, *counters = nullptr;
+  PagedAttentionOp(vkl_device *d, vkl_command *c, int h, int kv, int dm, int pg, float s, int w, int dt)
+      : PagedOp(d, c), heads(h), kv_heads(kv), dim(dm), page(pg), window(w), dtype(dt), scale(s) {}
+  ~PagedAttentionOp() override {
+    for (vkl_tensor *t : {out, scratch, counters}) vkl_tensor_release(t);
+  }
+  int init() override {
+    if (inited) return VKL_OK;
+    if (!good_dtype(dtype)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: only fp16 and bf16 dtypes are supported.");
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65535)
+      return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: %d heads over %d key heads", heads, kv_heads);
+    if (!good_dim(dim)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: head dim %d is no multiple of 8 up to 256", dim);
+    if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: a page of %d tokens", page);
+    if (window < 0) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: a window of %d positions", window);
+    if (!std::isfinite(scale)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: scale is %g", scale);
+    const uint32_t sms = dev->prop.multiProcessorCount;
+    VKL_CUDA(setup_paged_token());
+    VKL_CUDA(setup_paged_prompt());
+    VKL_OKAY(tensor_new(dev, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32, &scratch));
+    VKL_OKAY(tensor_new(dev, 1, 1, sms + 1, VKL_UINT32, &counters));
+    VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
+    uint32_t *word;
+    VKL_OKAY(command_error_word(cmd, &word));
+    return base_init();
+  }
+  int run(vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths, vkl_tensor *starts, vkl_tensor **o) {
+    const char *who = "paged_attention";
+    OnDevice here(dev->ordinal);
+    VKL_OKAY(check_rows(q, who, "queries", dtype));
+    if (q->w != (size_t)heads * dim) return fail(VKL_INVALID_ARGUMENT, "%s: queries are %zu wide, expected %d heads of %d", who, q->w, heads, dim);
+    VKL_OKAY(check_cache(kcache, vcache, who, dtype, kv_heads, page, dim));
+    VKL_OKAY(check_table(table, who, page));
+    const size_t n = table->h, rows = q->h, per = heads / kv_heads;
+    VKL_OKAY(check_list(lengths, who, "lengths", n));
+    if (starts) VKL_OKAY(check_list(starts, who, "starts", n + 1));
+    if (!starts && rows != n) return fail(VKL_INVALID_ARGUMENT, "%s: %zu queries for %zu sequences of one new token each", who, rows, n);
+    VKL_OKAY(check_apart(q, who, "queries"));
+    if (rows * per > kMaxTokens || n * (table->w * page / 16 + 1) > 0xffffffffu || n > kMaxTokens)
+      return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, %zu sequences of up to %zu tokens", who, rows, n, table->w * page);
+    VKL_OKAY(enter(who));
+    VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
+    if (rows && n) {
+      PagedAttention p = {};
+      p.q = q->data(), p.q_ld = q->hs / 2;
+      p.kcache = kcache->data(), p.vcache = vcache->data();
+      p.out = out->data();
+      p.table = (const uint32_t *)table->data();
+      p.lengths = (const uint32_t *)lengths->data();
+      p.starts = starts ? (const uint32_t *)starts->data() : nullptr;
+      p.scratch = (float *)scratch->data();
+      p.counters = (uint32_t *)counters->data();
+      VKL_OKAY(command_error_word(cmd, &p.error));
+      p.rows = (uint32_t)rows, p.n = (uint32_t)n, p.heads = heads, p.kv_heads = kv_heads, p.dim = dim;
+      p.width = (uint32_t)table->w, p.pages = (uint32_t)kcache->c, p.window = window;
+      p.page = divisor(page);
+      p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
+      p.bf = dtype == VKL_BF16;
+      const uint32_t sms = dev->prop.multiProcessorCount;
+      VKL_LAUNCH(1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
+    }
+    *o = out;
+    return leave();
+  }
+};
+
+template <class T, class... A> int make(vkl_op **out, vkl_device *dev, vkl_command *cmd, A... a) {
+  if (!out) return fail(VKL_INVALID_ARGUMENT, "op create: null output");
+  if (!dev || !cmd) return fail(VKL_INVALID_ARGUMENT, "op create: null device or command");
+  if (cmd->dev->ordinal != dev->ordinal) return fail(VKL_INVALID_ARGUMENT, "op create: the command is on device %d, not %d", cmd->dev->ordinal, dev->ordinal);
+  *out = new (std::nothrow) T(dev, cmd, a...);
+  return *out ? VKL_OK : fail(VKL_RESOURCE_EXHAUSTED, "op create: out of host memory");
+}
+
+}  // namespace
+
+extern "C" {
+
+int vkl_paged_tables_create(vkl_device *dev, vkl_command *cmd, int page_size, vkl_op **out) { return make<PagedTablesOp>(out, dev, cmd, page_size); }
+int vkl_paged_tables_run(vkl_op *op, vkl_tensor *lengths, vkl_tensor *target, vkl_tensor *table, vkl_tensor *pool, size_t rows, vkl_tensor **map, vkl_tensor **starts) {
+  PagedTablesOp *m;
+  VKL_OKAY(as(op, &m, "paged_tables_run"));
+  if (!map || !starts) return fail(VKL_INVALID_ARGUMENT, "paged_tables_run: null output");
+  return m->run(lengths, target, table, pool, rows, map, starts);
+}
+int vkl_update_paged_kvcache_create(vkl_device *dev, vkl_command *cmd, int dim, int page_size, float theta, int dtype, vkl_op **out) {
+  return make<UpdatePagedOp>(out, dev, cmd, dim, page_size, theta, dtype);
+}
+int vkl_update_paged_kvcache_run(vkl_op *op, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *k, vkl_tensor *v, vkl_tensor *map, vkl_tensor *q, vkl_tensor **out) {
+  UpdatePagedOp *m;
+  VKL_OKAY(as(op, &m, "update_paged_kvcache_run"));
+  if (q && !out) return fail(VKL_INVALID_ARGUMENT, "update_paged_kvcache_run: null output");
+  return m->run(kcache, vcache, k, v, map, q, out);
+}
+int vkl_paged_attention_create(vkl_device *dev, vkl_command *cmd, int heads, int kv_heads, int dim, int page_size, float scale, int window, int dtype, vkl_op **out) {
+  return make<PagedAttentionOp>(out, dev, cmd, heads, kv_heads, dim, page_size, scale, window, dtype);
+}
+int vkl_paged_attention_run(vkl_op *op, vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths, vkl_tensor *starts, vkl_tensor **out) {
+  PagedAttentionOp *m;
+  VKL_OKAY(as(op, &m, "paged_attention_run"));
+  if (!out) return fail(VKL_INVALID_ARGUMENT, "paged_attention_run: null output");
+  return m->run(q, kcache, vcache, table, lengths, starts, out);
+}
+
+}  // extern "C"

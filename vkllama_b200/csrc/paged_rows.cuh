@@ -1,0 +1,130 @@
+// What the kernels for several new rows per sequence share: which rows a tile has, and a row computed by itself.
+#pragma once
+#include "common.cuh"
+#include "paged.h"
+#include "paged_value.cuh"
+
+namespace vkl {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A tile of packed rows: which sequence, and its rows.
+struct Place {
+  uint32_t seq, row0, fresh, len;  // first row of the sequence in q, its new rows, its length
+  uint32_t first;                  // first packed row of the tile
+};
+
+// Rows of sequence i, 0 where starts, lengths and table do not belong together.
+__device__ __forceinline__ uint32_t fresh_rows(const PagedAttention &p, uint32_t i, bool &bad) {
+  const uint32_t a = p.starts[i], b = p.starts[i + 1], len = p.lengths[i];
+  if (a <= b && b <= p.rows && b - a <= len && len <= p.width * p.page.d) return b - a;
+  bad = true;
+  return 0;
+}
+
+// The place of tile `tile` when every sequence has ceil(new * per / rows) of them; false beyond the last.
+template <uint32_t THREADS> __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint64_t back, Place &at) {
+  __shared__ uint64_t before_s[THREADS + 1], sums_s[THREADS / 32];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t each = (p.n + THREADS - 1) / THREADS, i0 = min(tid * each, p.n), i1 = min(i0 + each, p.n);
+  bool bad = false;
+  uint64_t mine = 0;
+  auto tiles = [&](uint32_t i) { return ((uint64_t)fresh_rows(p, i, bad) * per + rows - 1) / rows; };
+  for (uint32_t i = i0; i < i1; ++i) mine += tiles(i);
+  if (bad && blockIdx.x == 0 && blockIdx.y == 0) raise(p.error, PAGED_BAD_ROWS);
+  uint64_t up = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t a = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += a;
+  }
+  if (lane == 31) sums_s[warp] = up;
+  __syncthreads();
+  uint64_t base = 0;
+  for (uint32_t w = 0; w < warp; ++w) base += sums_s[w];
+  before_s[tid] = base + up - mine;
+  if (tid == THREADS - 1) before_s[THREADS] = base + up;
+  __syncthreads();
+  if (back >= before_s[THREADS]) return false;
+  const uint64_t tile = before_s[THREADS] - 1 - back;  // the last tiles of a sequence see most: they start first
+  uint32_t lo = 0, hi = THREADS;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (before_s[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  uint64_t left = tile - before_s[lo];
+  at.seq = lo * each;
+  for (uint64_t n = tiles(at.seq); left >= n; n = tiles(at.seq)) {
+    left -= n;
+    ++at.seq;
+  }
+  at.fresh = fresh_rows(p, at.seq, bad);
+  at.row0 = p.starts[at.seq];
+  at.len = p.lengths[at.seq];
+  at.first = (uint32_t)left * rows;
+  return true;
+}
+
+// One packed row by a warp, from the definition in fp32. In the tiles' second product a position that a row does not see has the
+// probability 0, and 0 times an infinity or a NaN in that position's value is NaN: rows that come out of it not finite are computed
+// again here, from the positions that they see. (So a value that is not finite costs time, and reaches only the rows that see it.)
+template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &p, const Place &at, uint32_t kvh, uint32_t packed) {
+  const uint32_t lane = threadIdx.x & 31, per = p.heads / p.kv_heads, t = packed / per, h = kvh * per + packed - t * per;
+  const uint32_t pos = at.len - at.fresh + t, first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
+  const uint16_t *q = static_cast<const uint16_t *>(p.q) + (at.row0 + t) * p.q_ld + h * p.dim;
+  const uint16_t *k = static_cast<const uint16_t *>(p.kcache), *v = static_cast<const uint16_t *>(p.vcache);
+  float m = -INFINITY, l = 0.f;
+  float2 o[4] = {};  // dimensions lane * 2 + 64 i
+  for (uint32_t j0 = first; j0 <= pos; j0 += 32) {
+    const uint32_t j = j0 + lane;
+    bool there = j <= pos;
+    size_t row = 0;
+    float s = -INFINITY;
+    if (there) {
+      const uint32_t n = quotient(j, p.page), page = p.table[(size_t)at.seq * p.width + n];
+      there = page < p.pages;
+      if (there) {
+        row = ((size_t)page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
+        s = 0.f;
+        for (uint32_t d = 0; d < p.dim; d += 2) {
+          const float2 a = unpack2<BF>(*reinterpret_cast<const uint32_t *>(q + d)), b = unpack2<BF>(*reinterpret_cast<const uint32_t *>(k + row * p.dim + d));
+          s = fmaf(a.x, b.x, s);
+          s = fmaf(a.y, b.y, s);
+        }
+        s *= p.scale * kLog2e;
+      }
+    }
+    const float now = fmaxf(m, warp_max(s)), ref = now == -INFINITY ? 0.f : now, c = exp2f(m - ref);
+    const float w = there ? exp2f(s - ref) : 0.f;
+    m = now;
+    l = l * c + warp_sum(w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i].x *= c, o[i].y *= c;
+    const uint32_t all = __ballot_sync(0xffffffffu, there);
+    for (uint32_t x = 0; x < 32; ++x) {
+      if (!(all >> x & 1)) continue;
+      const float wx = __shfl_sync(0xffffffffu, w, x);
+      const size_t rx = __shfl_sync(0xffffffffu, (unsigned long long)row, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t d = lane * 2 + 64 * i;
+        if (d < p.dim) {
+          const float2 b = unpack2<BF>(*reinterpret_cast<const uint32_t *>(v + rx * p.dim + d));
+          o[i].x = fmaf(wx, b.x, o[i].x);
+          o[i].y = fmaf(wx, b.y, o[i].y);
+        }
+      }
+    }
+  }
+  const float r = 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t d = lane * 2 + 64 * i;
+    if (d < p.dim) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + ((size_t)(at.row0 + t) * p.heads + h) * p.dim + d) = pack2<BF>(o[i].x * r, o[i].y * r);
+  }
+}
+
+}  // namespace
+}  // namespace vkl

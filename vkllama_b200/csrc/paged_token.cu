@@ -1,0 +1,525 @@
+// Attention of one new token per sequence over a paged cache:
+//   out = sum_j softmax_j(scale q.k_j) v_j over the positions max(0, length - window) <= j < length.
+//
+// Every visible key and value is read once for all query heads of its group, so HBM bounds it: 4 dim bytes a position and key head.
+// The products run on mma.sync (m16n8k16, fp32 sums) because a group's queries share the fragments: 8 (or 16) query heads are the
+// rows of A, cached rows the columns. A tile's upper eight rows would be empty; in P.V they carry what rounding the probabilities to
+// 16 bits leaves over (p = hi + lo, both exact products, added at the end), so the result has the probabilities' 32 bits at no cost.
+//
+// Work is cut into equal shares, not by sequence: the tiles of 16 positions of all (sequence, head group) pairs stand in one row, every
+// CTA takes a range of it and every warp of the CTA a range of that, however the lengths are spread. Ranges cut pairs: a warp keeps
+// running maximum, sum and output of its part; parts meet in shared memory, and those of several CTAs in scratch, where the CTA that
+// arrives last adds them up in their order (the result does not depend on who that is). Cuts that would leave a small piece of a pair are
+// moved to its border.
+//
+// A warp streams its range through a ring of its own (cp.async, tiles of keys and of values alternating, swizzled for ldmatrix):
+// no barrier inside the stream, the next pages are looked up a tile ahead. Rows that are not visible are not read and count as zeros.
+#include <algorithm>
+
+#include "common.cuh"
+#include "paged.h"
+#include "paged_value.cuh"
+
+namespace vkl {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kTile = 16;                // positions
+constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
+constexpr uint32_t kShareTiles = 16;          // a CTA's share is at least this many tiles
+constexpr uint32_t kSnapTiles = 16;           // a cut this near to a pair's border moves there
+
+// DP: padded head width, MG: groups of eight query heads.
+template <int DP, int MG> struct Cfg {
+  static constexpr uint32_t kHalf = kTile * DP * 2;  // bytes of a tile's keys, or values
+  static constexpr uint32_t kRing = DP == 64 ? 8 : DP == 128 ? (MG == 1 ? 6 : 4) : 2;
+  static constexpr uint32_t kHeads = 8 * MG;
+  static constexpr uint32_t kStash = kHeads * DP * 4;  // a warp's first part, where its range goes on behind it
+  static constexpr uint32_t kSmem = kWarps * (kRing * kHalf + kStash + 2 * kHeads * 2 * 4);
+  static_assert(kSmem + 1536 <= 227 * 1024, "shared memory of an SM");
+  static_assert(kRing * kHalf >= kStash, "a warp's last part lies in its ring");
+};
+
+struct Pair {        // tiles t .. t1 of a sequence and head group
+  uint32_t seq, grp;
+  uint32_t t, t0, t1;
+  uint32_t len, first;  // visible positions
+};
+
+// One record per part of a pair that ends inside a CTA.
+struct Part {
+  uint32_t seq, grp;
+  uint8_t there, begins, ends;  // the pair begins, ends in this part
+};
+
+template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1) paged_token_kernel(const PagedAttention p) {
+  using C = Cfg<DP, MG>;
+  constexpr uint32_t CH = DP / 8;            // 16-byte pieces of a row
+  constexpr uint32_t NC = kTile * CH / 32;   // of a half and lane
+  constexpr int KS = DP / 16, NT = DP / 8;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint32_t before_s[kThreads + 1];  // tiles of one head group's sequences; the host has checked that they fit 32 bits
+  __shared__ uint32_t warp_sum_s[kWarps];
+  __shared__ uint64_t border_s[2];
+  __shared__ Part part_s[kWarps][2];
+  __shared__ uint32_t last_s[2];
+  unsigned char *ring = smem + threadIdx.x / 32 * C::kRing * C::kHalf;
+  float *stash = reinterpret_cast<float *>(smem + kWarps * C::kRing * C::kHalf);       // [warp][head][DP]
+  float *ml = reinterpret_cast<float *>(smem + kWarps * (C::kRing * C::kHalf + C::kStash));  // [warp][2][head][2]
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const uint32_t per = p.heads / p.kv_heads, groups = (per + C::kHeads - 1) / C::kHeads, pairs = p.kv_heads * groups;
+  const uint32_t room = p.width * p.page.d;  // positions that a table holds (checked by the host to fit 31 bits)
+
+  // ---- where this CTA's and this warp's range is ----
+  auto length = [&](uint32_t i) { return min(p.lengths[i], room); };
+  auto first_of = [&](uint32_t len) { return p.window && len > p.window ? len - p.window : 0u; };
+  auto tiles = [&](uint32_t len) { return max((len + kTile - 1) / kTile, 1u) - first_of(len) / kTile; };
+  const uint32_t each = (p.n + kThreads - 1) / kThreads;
+  {
+    const uint32_t i0 = min(tid * each, p.n), i1 = min(i0 + each, p.n);
+    uint32_t mine = 0;
+    for (uint32_t i = i0; i < i1; ++i) {
+      if (p.lengths[i] > room && blockIdx.x == 0) raise(p.error, PAGED_TABLE_FULL);
+      mine += tiles(length(i));
+    }
+    uint32_t up = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t a = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += a;
+    }
+    if (lane == 31) warp_sum_s[warp] = up;
+    if (tid < kWarps * 2) part_s[tid >> 1][tid & 1].there = 0;
+    __syncthreads();
+    uint32_t base = 0;
+    for (uint32_t w = 0; w < warp; ++w) base += warp_sum_s[w];
+    before_s[tid] = base + up - mine;
+    if (tid == kThreads - 1) before_s[kThreads] = base + up;
+    __syncthreads();
+  }
+  const uint64_t total = (uint64_t)before_s[kThreads] * pairs;
+  const uint64_t share = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)kShareTiles);
+  auto find = [&](uint64_t pos) {  // the pair and tile at pos < total
+    uint32_t lo = 0, hi = kThreads;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if ((uint64_t)before_s[mid] * pairs <= pos) lo = mid;
+      else hi = mid;
+    }
+    Pair r;
+    r.seq = lo * each;
+    uint64_t left = pos - (uint64_t)before_s[lo] * pairs;
+    uint32_t len = length(r.seq), n = tiles(len);
+    while (left >= (uint64_t)n * pairs) {
+      left -= (uint64_t)n * pairs;
+      len = length(++r.seq);
+      n = tiles(len);
+    }
+    r.grp = (uint32_t)(left / n);
+    r.len = len;
+    r.first = first_of(len);
+    r.t0 = r.first / kTile;
+    r.t1 = r.t0 + n;
+    r.t = r.t0 + (uint32_t)(left - (uint64_t)r.grp * n);
+    return r;
+  };
+  if (tid < 2) {  // the range's borders
+    uint64_t b = (blockIdx.x + tid) * share;
+    if (b >= total) {
+      b = total;
+    } else if (b > 0) {
+      const Pair r = find(b);
+      const uint32_t in = r.t - r.t0, out = r.t1 - r.t;
+      if (min(in, out) <= kSnapTiles) b = in <= out ? b - in : b + out;
+    }
+    border_s[tid] = b;
+  }
+  __syncthreads();
+  const uint64_t b0 = border_s[0], b1 = border_s[1];
+  if (b0 == b1) return;
+  const uint64_t w0 = b0 + (b1 - b0) * warp / kWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kWarps;
+  const uint32_t count = (uint32_t)(w1 - w0);
+
+  auto advance = [&](Pair &r) {
+    if (++r.t < r.t1) return;
+    if (++r.grp == pairs) {
+      r.grp = 0;
+      if (++r.seq >= p.n) return;
+      r.len = length(r.seq);
+      r.first = first_of(r.len);
+      r.t0 = r.first / kTile;
+      r.t1 = r.t0 + tiles(r.len);
+    }
+    r.t = r.t0;
+  };
+  auto write_out = [&](uint32_t seq, uint32_t head, uint32_t d, float a, float b) {
+    if (d < p.dim) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + ((size_t)seq * p.heads + head) * p.dim + d) = pack2<BF>(a, b);
+  };
+  auto first_head = [&](uint32_t grp) { return grp / groups * per + grp % groups * C::kHeads; };
+  auto heads_of = [&](uint32_t grp) { return min(per - grp % groups * C::kHeads, C::kHeads); };
+
+  if (count) {
+    // ---- the stream: tile halves, keys and values in turn, go into the ring's places one after the other ----
+    Pair in = find(w0), at = in;
+    uint32_t left = count, entry = 0, in_page = 0, row_at = 0xffffffffu, slot_in = 0;
+    bool values = false;
+    const uint32_t ring_a = smem_addr(ring);
+    auto look_up = [&]() {  // the page of this lane's position of the tile that comes next
+      const uint32_t j = in.t * kTile + (lane & 15);
+      if (j >= in.first && j < in.len) {
+        const uint32_t q = quotient(j, p.page);
+        entry = __ldg(p.table + (size_t)in.seq * p.width + q);
+        in_page = j - q * p.page.d;
+      } else {
+        entry = kNoSlot;
+      }
+    };
+    look_up();
+    auto request = [&]() {
+      if (left) {
+        if (!values) {
+          row_at = 0xffffffffu;
+          if (entry < p.pages) row_at = (entry * p.kv_heads + in.grp / groups) * p.page.d + in_page;  // the host has checked that rows fit 32 bits
+          else if (entry != kNoSlot) raise(p.error, PAGED_BAD_PAGE);
+        }
+        const uint16_t *src = static_cast<const uint16_t *>(values ? p.vcache : p.kcache);
+        const uint32_t dst = ring_a + slot_in * C::kHalf;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+          const uint32_t c = i * 32 + lane, row = c / CH, col = c % CH;
+          const uint32_t r = __shfl_sync(0xffffffffu, row_at, row);
+          const bool there = r != 0xffffffffu && col * 8 < p.dim;
+          copy16(dst + (row * CH + (col ^ (row & 7))) * 16, there ? src + (size_t)r * p.dim + col * 8 : src, there);
+        }
+        if (values && --left) {
+          advance(in);
+          look_up();
+        }
+        values = !values;
+        slot_in = slot_in + 1 == C::kRing ? 0 : slot_in + 1;
+      }
+      copy_commit();  // one group per place, also when it is empty
+    };
+#pragma unroll 1
+    for (uint32_t i = 0; i < C::kRing; ++i) request();
+
+    // ---- the sums of the current pair: rows g of every group of eight heads; o's second half holds the low parts ----
+    float o[MG][NT][4], mx[MG], sum[MG];
+    uint32_t q[MG][KS][2];
+    uint32_t slot = 0;
+    bool begins = at.t == at.t0;
+    auto start_pair = [&]() {
+      const uint32_t h0 = first_head(at.grp), nh = heads_of(at.grp);
+#pragma unroll
+      for (int m = 0; m < MG; ++m) {
+        const uint16_t *src = static_cast<const uint16_t *>(p.q) + at.seq * p.q_ld + (h0 + m * 8 + g) * p.dim;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t d = k * 16 + e * 8 + t4 * 2;
+            q[m][k][e] = m * 8 + g < nh && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) : 0u;
+          }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
+        mx[m] = -INFINITY;
+        sum[m] = 0.f;
+      }
+    };
+    // hi + lo of one output; an infinite one has no low part (its product there is 0 times infinity)
+    auto joined = [](float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; };
+    auto keep = [&](float *to, float *to_ml) {  // this part for the ones that join it
+#pragma unroll
+      for (int m = 0; m < MG; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<float2 *>(to + (m * 8 + g) * DP + n * 8 + t4 * 2) = make_float2(joined(o[m][n][0], o[m][n][2]), joined(o[m][n][1], o[m][n][3]));
+        if (t4 == 0) to_ml[(m * 8 + g) * 2] = mx[m], to_ml[(m * 8 + g) * 2 + 1] = sum[m];
+      }
+    };
+    start_pair();
+    const float scale = p.scale * kLog2e;
+    const uint32_t lrow = lane & 7, lsel = lane >> 3;  // ldmatrix: row of a matrix, which of the four
+#pragma unroll 1
+    for (uint32_t it = 0; it < count; ++it) {
+      copy_wait<C::kRing - 1>();
+      __syncwarp();
+      // S = Q K^T: matrices (rows 0-7 | 8-15) x (k low | k high)
+      float s[MG][2][4];
+#pragma unroll
+      for (int m = 0; m < MG; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+      {
+        const uint32_t kt = ring_a + slot * C::kHalf;
+        const uint32_t row = lrow + (lsel >> 1) * 8;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t b[4];
+          ldmatrix4(b, kt + (row * CH + ((2 * k + (lsel & 1)) ^ lrow)) * 16);
+#pragma unroll
+          for (int m = 0; m < MG; ++m) {
+            mma2<BF>(s[m][0], q[m][k][0], 0, q[m][k][1], 0, b[0], b[1]);
+            mma2<BF>(s[m][1], q[m][k][0], 0, q[m][k][1], 0, b[2], b[3]);
+          }
+        }
+      }
+      slot = slot + 1 == C::kRing ? 0 : slot + 1;
+      __syncwarp();
+      request();
+      // softmax so far
+      const uint32_t j0 = at.t * kTile + t4 * 2;
+      uint32_t pa[MG][4];
+#pragma unroll
+      for (int m = 0; m < MG; ++m) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t j = j0 + (e >> 1) * 8 + (e & 1);
+          v[e] = j >= at.first && j < at.len ? s[m][e >> 1][e & 1] * scale : -INFINITY;
+        }
+        float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float now = fmaxf(mx[m], top), ref = now == -INFINITY ? 0.f : now;
+        if (__any_sync(0xffffffffu, now != mx[m])) {
+          const float c = exp2f(mx[m] - ref);
+          sum[m] *= c;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[m][n][e] *= c;
+          mx[m] = now;
+        }
+        float hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = exp2f(v[e] - ref);
+          sum[m] += v[e];
+        }
+        pa[m][0] = pack2<BF>(v[0], v[1]);
+        pa[m][2] = pack2<BF>(v[2], v[3]);
+        const float2 h01 = unpack2<BF>(pa[m][0]), h23 = unpack2<BF>(pa[m][2]);
+        hi[0] = h01.x, hi[1] = h01.y, hi[2] = h23.x, hi[3] = h23.y;
+        pa[m][1] = pack2<BF>(v[0] - hi[0], v[1] - hi[1]);
+        pa[m][3] = pack2<BF>(v[2] - hi[2], v[3] - hi[3]);
+      }
+      copy_wait<C::kRing - 1>();
+      __syncwarp();
+      {
+        const uint32_t vt = ring_a + slot * C::kHalf;
+        const uint32_t row = lrow + (lsel & 1) * 8;
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t b[4];
+          ldmatrix4_t(b, vt + (row * CH + ((n + (lsel >> 1)) ^ lrow)) * 16);
+#pragma unroll
+          for (int m = 0; m < MG; ++m) {
+            mma2<BF>(o[m][n], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b[0], b[1]);
+            mma2<BF>(o[m][n + 1], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b[2], b[3]);
+          }
+        }
+      }
+      slot = slot + 1 == C::kRing ? 0 : slot + 1;
+      __syncwarp();
+      request();
+
+      const bool ends = at.t + 1 == at.t1, over = it + 1 == count;
+      if (!ends && !over) {
+        ++at.t;
+        continue;
+      }
+      // a part is complete
+      if (begins && ends) {
+        const uint32_t h0 = first_head(at.grp), nh = heads_of(at.grp);
+#pragma unroll
+        for (int m = 0; m < MG; ++m) {
+          float all = sum[m];
+          all += __shfl_xor_sync(0xffffffffu, all, 1);
+          all += __shfl_xor_sync(0xffffffffu, all, 2);
+          const float r = at.len ? 1.0f / all : 0.f;  // nothing visible: zeros
+          if (m * 8 + g < nh) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              write_out(at.seq, h0 + m * 8 + g, n * 8 + t4 * 2, joined(o[m][n][0], o[m][n][2]) * r, joined(o[m][n][1], o[m][n][3]) * r);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < MG; ++m) {
+          sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 1);
+          sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 2);
+        }
+        if (lane == 0) part_s[warp][over] = {at.seq, at.grp, 1, begins, ends};
+        float *to = stash + warp * (C::kStash / 4);
+        if (over) {
+          copy_wait<0>();
+          __syncwarp();
+          to = reinterpret_cast<float *>(ring);
+        }
+        keep(to, ml + (warp * 2 + over) * C::kHeads * 2);
+      }
+      if (!over) {
+        advance(at);
+        start_pair();
+        begins = true;
+      }
+    }
+    copy_wait<0>();
+  }
+  __syncthreads();
+
+  // ---- parts meet. They stand in order (warp by warp, a warp's first before its last); a run of them is one pair. ----
+  auto part_o = [&](uint32_t i) { return (i & 1) ? reinterpret_cast<const float *>(smem + (i >> 1) * C::kRing * C::kHalf) : stash + (i >> 1) * (C::kStash / 4); };
+  float *scratch_o = p.scratch, *scratch_ml = p.scratch + (size_t)gridDim.x * 2 * C::kHeads * DP;
+  uint32_t run = 0;
+  Part open[2] = {};  // the CTA's pairs that began before it (0), end behind it (1)
+  for (uint32_t i = 0; i < 2 * kWarps;) {
+    Part a = part_s[i >> 1][i & 1];
+    if (!a.there) {
+      ++i;
+      continue;
+    }
+    uint32_t e = i + 1;  // the run is [i, e)
+    for (bool done = a.ends; !done && e < 2 * kWarps; ++e) {
+      const Part b = part_s[e >> 1][e & 1];
+      if (b.there) a.ends = b.ends, done = b.ends;
+    }
+    const bool whole = a.begins && a.ends;
+    const uint32_t side = a.begins ? 1 : 0;  // where it goes in scratch
+    const uint32_t h0 = first_head(a.grp), nh = heads_of(a.grp);
+    for (uint32_t h = (warp + kWarps - run % kWarps) % kWarps; h < nh; h += kWarps) {
+      float m = -INFINITY, l = 0.f;
+      for (uint32_t x = i; x < e; ++x)
+        if (part_s[x >> 1][x & 1].there) m = fmaxf(m, ml[(x * C::kHeads + h) * 2]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float2 acc[DP / 64] = {};
+      for (uint32_t x = i; x < e; ++x) {
+        if (!part_s[x >> 1][x & 1].there) continue;
+        const float c = exp2f(ml[(x * C::kHeads + h) * 2] - ref);
+        l += c * ml[(x * C::kHeads + h) * 2 + 1];
+        const float *src = part_o(x) + h * DP;
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d) {
+          const float2 v = *reinterpret_cast<const float2 *>(src + d * 64 + lane * 2);
+          acc[d].x += c * v.x, acc[d].y += c * v.y;
+        }
+      }
+      if (whole) {
+        const float r = 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d) write_out(a.seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
+      } else {
+        const size_t rec = ((size_t)blockIdx.x * 2 + side) * C::kHeads + h;
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d) *reinterpret_cast<float2 *>(scratch_o + rec * DP + d * 64 + lane * 2) = acc[d];
+        if (lane == 0) *reinterpret_cast<float2 *>(scratch_ml + rec * 2) = make_float2(m, l);
+      }
+    }
+    if (!whole) {
+      a.there = 1;
+      open[side] = a;
+    }
+    ++run;
+    i = e;
+  }
+  if (!open[0].there && !open[1].there) return;
+
+  // ---- pairs of several CTAs: cuts are the multiples of the share that lie further than kSnapTiles inside the pair ----
+  __threadfence();
+  __syncthreads();
+  uint64_t cut0[2], cut1[2];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    cut0[side] = cut1[side] = 0;
+    if (!open[side].there) continue;
+    const uint32_t s = open[side].seq, base = s / each;
+    uint64_t begin = before_s[base];
+    for (uint32_t i = base * each; i < s; ++i) begin += tiles(length(i));
+    const uint64_t n = tiles(length(s));
+    begin = begin * pairs + n * open[side].grp;
+    cut0[side] = (begin + kSnapTiles) / share + 1;
+    cut1[side] = (begin + n - kSnapTiles - 1) / share;  // cut0 <= cut1: n > 2 kSnapTiles where a cut is left
+  }
+  if (tid < 2) {
+    last_s[tid] = 0;
+    if (open[tid].there) {
+      const uint32_t c0 = (uint32_t)cut0[tid], parts = (uint32_t)(cut1[tid] - cut0[tid]) + 2;
+      __threadfence();
+      if (atomicAdd(p.counters + c0, 1u) + 1 == parts) {
+        p.counters[c0] = 0;
+        last_s[tid] = 1;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    if (!last_s[side]) continue;
+    __threadfence();
+    const Part a = open[side];
+    const uint32_t h0 = first_head(a.grp), nh = heads_of(a.grp);
+    const uint32_t c0 = (uint32_t)cut0[side], c1 = (uint32_t)cut1[side];
+    auto rec = [&](uint32_t c, uint32_t h) { return ((size_t)c * 2 + (c + 1 == c0 ? 1 : 0)) * C::kHeads + h; };  // the first part ends its CTA's range
+    for (uint32_t h = warp; h < nh; h += kWarps) {
+      float m = -INFINITY, l = 0.f;
+      for (uint32_t c = c0 - 1 + lane; c <= c1; c += 32) m = fmaxf(m, __ldcg(scratch_ml + rec(c, h) * 2));
+      m = warp_max(m);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float2 acc[DP / 64] = {};
+#pragma unroll 4
+      for (uint32_t c = c0 - 1; c <= c1; ++c) {
+        const float2 x = __ldcg(reinterpret_cast<const float2 *>(scratch_ml + rec(c, h) * 2));
+        const float w = exp2f(x.x - ref);
+        l += w * x.y;
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d) {
+          const float2 v = __ldcg(reinterpret_cast<const float2 *>(scratch_o + rec(c, h) * DP + d * 64 + lane * 2));
+          acc[d].x += w * v.x, acc[d].y += w * v.y;
+        }
+      }
+      const float r = 1.0f / l;
+#pragma unroll
+      for (int d = 0; d < DP / 64; ++d) write_out(a.seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
+    }
+  }
+}
+
+template <bool BF, int DP, int MG> cudaError_t setup_one() {
+  return cudaFuncSetAttribute(paged_token_kernel<BF, DP, MG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP, MG>::kSmem);
+}
+template <bool BF, int DP, int MG> cudaError_t run(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
+  // No more CTAs than there can be shares of.
+  const uint64_t per = p.heads / p.kv_heads, pairs = (uint64_t)p.kv_heads * ((per + 8 * MG - 1) / (8 * MG));
+  const uint64_t most = p.n * pairs * (((uint64_t)p.width * p.page.d + kTile - 1) / kTile), shares = (most + kShareTiles - 1) / kShareTiles;
+  paged_token_kernel<BF, DP, MG><<<(uint32_t)std::min<uint64_t>(sms, shares), kThreads, Cfg<DP, MG>::kSmem, s>>>(p);
+  return cudaGetLastError();
+}
+template <bool BF> cudaError_t pick(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
+  // Sixteen query heads per warp where a group has more than eight and their outputs fit the registers: keys and values are read
+  // once for all of them. Wider heads take them eight at a time, the second time from L2.
+  const bool two = p.heads / p.kv_heads > 8;
+  if (p.dim <= 64) return two ? run<BF, 64, 2>(p, sms, s) : run<BF, 64, 1>(p, sms, s);
+  if (p.dim <= 128) return two ? run<BF, 128, 2>(p, sms, s) : run<BF, 128, 1>(p, sms, s);
+  return run<BF, 256, 1>(p, sms, s);
+}
+
+}  // namespace
+
+size_t paged_token_scratch(uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t sms) {
+  const uint32_t dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, most = heads / kv_heads > 8 && dim <= 128 ? 16 : 8;
+  return (size_t)sms * 2 * most * (dp + 2) * 4;
+}
+cudaError_t setup_paged_token() {
+  for (cudaError_t e : {setup_one<false, 64, 1>(), setup_one<false, 64, 2>(), setup_one<false, 128, 1>(), setup_one<false, 128, 2>(), setup_one<false, 256, 1>(),
+                        setup_one<true, 64, 1>(), setup_one<true, 64, 2>(), setup_one<true, 128, 1>(), setup_one<true, 128, 2>(), setup_one<true, 256, 1>()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
+}
+cudaError_t launch_paged_token(const PagedAttention &p, uint32_t sms, cudaStream_t s) { return p.bf ? pick<true>(p, sms, s) : pick<false>(p, sms, s); }
+
+}  // namespace vkl

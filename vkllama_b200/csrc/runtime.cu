@@ -3,6 +3,8 @@
 // command buffers) with a CUDA device, a size-bucketed block pool and streams.
 #include "runtime.h"
 
+#include "paged.h"
+
 #include <math.h>
 #include <stdio.h>
 
@@ -425,6 +427,14 @@ int vkl_command_wait(vkl_command *cmd) {
   if (e != cudaSuccess) return fail(VKL_INTERNAL, "command_wait: %s", cudaGetErrorString(e));
   if (watched && *cmd->err_host) {
     cudaMemsetAsync(cmd->err_word, 0, 4, cmd->stream);
+    switch (*cmd->err_host) {
+      case PAGED_POOL_EMPTY: return fail(VKL_RESOURCE_EXHAUSTED, "command_wait: paged_tables: the pool has fewer pages than the sequences need; nothing was changed");
+      case PAGED_TABLE_FULL: return fail(VKL_OUT_OF_RANGE, "command_wait: a sequence is longer than its row of the page table");
+      case PAGED_ROWS: return fail(VKL_OUT_OF_RANGE, "command_wait: paged_tables: more new tokens than rows; nothing was changed");
+      case PAGED_POOL_BAD: return fail(VKL_FAILED_PRECONDITION, "command_wait: paged_tables: the pool holds more pages than it has room for; nothing was changed");
+      case PAGED_BAD_PAGE: return fail(VKL_OUT_OF_RANGE, "command_wait: a page that the cache does not have was named");
+      case PAGED_BAD_ROWS: return fail(VKL_INVALID_ARGUMENT, "command_wait: paged_attention: starts, lengths and rows do not belong together");
+    }
     return fail(VKL_INTERNAL, "command_wait: a bounded wait inside a kernel ran out (code %u)", *cmd->err_host);
   }
   return VKL_OK;
