@@ -499,3 +499,17 @@ def test_two_commands_at_once(dev):
     for cmd in cmds:
         cmd.submit_and_wait()
     assert all((o == outs[0]).all() for o in outs)
+
+
+def test_time_of_the_last_run(dev):
+    """Op::time() as of the other ops: 0 before a run, microseconds of the device after the wait."""
+    rng, cmd = np.random.default_rng(14), vk.Command(dev)
+    c = Cache(rng, [30000], 2, 128, 16, vk.FP16)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        q, op = tensor(cmd, dev, draw(rng, (1, 256), vk.FP16), vk.FP16), vk.PagedAttention(dev, cmd, 2, 2, 128, 16).init()
+        assert op.time() == 0
+    for _ in range(3):
+        with cmd:
+            op(q, k, v, table, lens)
+        assert 2 <= op.time() < 1000

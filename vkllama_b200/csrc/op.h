@@ -1,5 +1,7 @@
 // What every operator class behind the C ABI is made of.
 #pragma once
+#include <math.h>
+
 #include "runtime.h"
 
 struct vkl_op {
@@ -25,6 +27,19 @@ struct vkl_op {
     if (!inited) return vkl::fail(VKL_FAILED_PRECONDITION, "%s: init() was not called", who);
     VKL_OKAY(vkl::recording(cmd, who));
     VKL_CUDA(cudaEventRecord(e0, cmd->stream));
+    return VKL_OK;
+  }
+  // Op::time(): device microseconds of the last run, 0 before the first.
+  virtual int elapsed(uint64_t *usec) {
+    *usec = 0;
+    if (!timed) return VKL_OK;
+    float ms = 0.f;
+    const cudaError_t e = cudaEventElapsedTime(&ms, e0, e1);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return vkl::fail(VKL_FAILED_PRECONDITION, "op_time: the op's last run has not finished (wait on its command first)");
+    }
+    *usec = (uint64_t)llroundf(ms * 1000.f);
     return VKL_OK;
   }
   int leave() {

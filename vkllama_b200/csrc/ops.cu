@@ -734,16 +734,7 @@ int vkl_op_init(vkl_op *op) {
 }
 int vkl_op_time(vkl_op *op, uint64_t *usec) {
   if (!op || !usec) return fail(VKL_INVALID_ARGUMENT, "op_time: null argument");
-  *usec = 0;
-  if (!op->timed) return VKL_OK;
-  float ms = 0.f;
-  cudaError_t e = cudaEventElapsedTime(&ms, op->e0, op->e1);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    return fail(VKL_FAILED_PRECONDITION, "op_time: the op's last run has not finished (wait on its command first)");
-  }
-  *usec = (uint64_t)llroundf(ms * 1000.f);
-  return VKL_OK;
+  return op->elapsed(usec);
 }
 int vkl_op_destroy(vkl_op *op) {
   delete op;

@@ -34,6 +34,39 @@ inline Divisor divisor(uint32_t d) {
 #ifdef __CUDACC__
 __device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor &v) { return (__umulhi(n, v.mul) + n) >> v.shift; }
 __device__ __forceinline__ void raise(uint32_t *error, uint32_t code) { atomicCAS(error, 0u, code); }
+// Launches may begin before the one in front of them in the stream has ended (launch_following): nothing is read or written before
+// follow() returns, when everything in front has ended and is visible, and the launch behind may be prepared from then on.
+__device__ __forceinline__ void follow() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+template <class K, class P> cudaError_t launch_following(K kernel, dim3 grid, uint32_t threads, size_t smem, cudaStream_t s, const P &p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// When a launch began and when its last CTA ended, for Op::time(): two events around every launch would cost 5 us of device time.
+// The timer only grows, so the later end is the last launch's.
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void stamp_begin(unsigned long long *stamps) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) stamps[0] = now_ns();
+}
+__device__ __forceinline__ void stamp_end(unsigned long long *stamps) {
+  if (threadIdx.x == 0) atomicMax(stamps + 1, now_ns());
+}
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 #endif
 
@@ -45,6 +78,7 @@ struct PagedTables {
   uint32_t *map;           // [2][rows]: slots, positions of the new rows
   uint32_t *starts;        // [n + 1] first new row of every sequence
   uint32_t *arrived;       // CTAs that are through; 0 between launches
+  unsigned long long *stamps;
   uint32_t *error;
   uint32_t n, width, capacity, rows;
   Divisor page;
@@ -58,6 +92,7 @@ struct PagedUpdate {
   void *q_out;                  // [rows][heads * dim]
   void *kcache, *vcache;
   const uint32_t *map;          // [2][rows]
+  unsigned long long *stamps;
   uint32_t *error;
   uint64_t q_ld, k_ld, v_ld;
   uint32_t rows, heads, kv_heads, dim, pages;
@@ -75,6 +110,7 @@ struct PagedAttention {
   const uint32_t *starts;       // [n + 1], or null: row i is the last token of sequence i
   float *scratch;               // partial results, paged_token_scratch() bytes
   uint32_t *counters;           // [SMs + 1], 0 between launches
+  unsigned long long *stamps;
   uint32_t *error;
   uint64_t q_ld;
   uint32_t rows, n, heads, kv_heads, dim, width, pages, window;

@@ -25,7 +25,38 @@ struct OnDevice {
 };
 
 struct PagedOp : vkl_op {
+  vkl_tensor *stamps = nullptr;  // of the last launch (paged.h), in the place of the other ops' events
   using vkl_op::vkl_op;
+  ~PagedOp() override { vkl_tensor_release(stamps); }
+  int paged_init() {
+    if (!dev || !cmd) return fail(VKL_INVALID_ARGUMENT, "op: null device or command");
+    VKL_OKAY(tensor_new(dev, 1, 1, 4, VKL_UINT32, &stamps));
+    VKL_CUDA(cudaMemsetAsync(stamps->data(), 0, 16, cmd->stream));
+    uint32_t *word;
+    VKL_OKAY(command_error_word(cmd, &word));  // allocated here, so that run() does not have to
+    inited = true;
+    return VKL_OK;
+  }
+  int begin(const char *who) {
+    if (!inited) return fail(VKL_FAILED_PRECONDITION, "%s: init() was not called", who);
+    return recording(cmd, who);
+  }
+  unsigned long long *stamp() {
+    timed = true;
+    return (unsigned long long *)stamps->data();
+  }
+  int elapsed(uint64_t *usec) override {
+    *usec = 0;
+    if (!timed) return VKL_OK;
+    if (cudaStreamQuery(cmd->stream) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return fail(VKL_FAILED_PRECONDITION, "op_time: the op's last run has not finished (wait on its command first)");
+    }
+    unsigned long long t[2];
+    VKL_CUDA(cudaMemcpy(t, stamps->data(), 16, cudaMemcpyDeviceToHost));
+    *usec = t[1] > t[0] ? (t[1] - t[0] + 500) / 1000 : 0;
+    return VKL_OK;
+  }
   int check(const vkl_tensor *t, const char *who, const char *name, int dtype, bool dense = true) {
     if (!t) return fail(VKL_INVALID_ARGUMENT, "%s: null %s", who, name);
     if (t->dev->ordinal != dev->ordinal) return fail(VKL_INVALID_ARGUMENT, "%s: %s is on device %d, the op on device %d", who, name, t->dev->ordinal, dev->ordinal);
@@ -81,13 +112,12 @@ struct PagedTablesOp : PagedOp {
   }
   int init() override {
     if (inited) return VKL_OK;
+    OnDevice here(dev->ordinal);
     if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "PagedTables op: a page of %d tokens", page);
     VKL_CUDA(setup_paged_tables());
     VKL_OKAY(tensor_new(dev, 1, 1, 1, VKL_UINT32, &arrived));
     VKL_CUDA(cudaMemsetAsync(arrived->data(), 0, 4, cmd->stream));
-    uint32_t *word;
-    VKL_OKAY(command_error_word(cmd, &word));  // allocated here, so that run() does not have to
-    return base_init();
+    return paged_init();
   }
   int run(vkl_tensor *lengths, vkl_tensor *target, vkl_tensor *table, vkl_tensor *pool, size_t rows, vkl_tensor **o_map, vkl_tensor **o_starts) {
     const char *who = "paged_tables";
@@ -100,7 +130,7 @@ struct PagedTablesOp : PagedOp {
     if (pool->c != 1 || pool->h != 1 || pool->w < 1) return fail(VKL_INVALID_ARGUMENT, "%s: the pool has shape (%zu, %zu, %zu), expected (1, 1, 1 + pages)", who, pool->c, pool->h, pool->w);
     if (n > kTablesMaxSequences) return fail(VKL_OUT_OF_RANGE, "%s: %zu sequences, at most %u", who, n, kTablesMaxSequences);
     if (rows > kMaxTokens || pool->w > kMaxTokens) return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, a pool of %zu pages", who, rows, pool->w - 1);
-    VKL_OKAY(enter(who));
+    VKL_OKAY(begin(who));
     VKL_OKAY(ensure_tensor(dev, &map, 1, 2, rows, VKL_UINT32));
     VKL_OKAY(ensure_tensor(dev, &starts, 1, 1, n + 1, VKL_UINT32));
     PagedTables p = {};
@@ -112,12 +142,13 @@ struct PagedTablesOp : PagedOp {
     p.starts = (uint32_t *)starts->data();
     p.arrived = (uint32_t *)arrived->data();
     VKL_OKAY(command_error_word(cmd, &p.error));
+    p.stamps = stamp();
     p.n = (uint32_t)n, p.width = (uint32_t)table->w, p.capacity = (uint32_t)pool->w - 1, p.rows = (uint32_t)rows;
     p.page = divisor(page);
     VKL_LAUNCH(1, launch_paged_tables(p, dev->prop.multiProcessorCount, cmd->stream));
     if (o_map) *o_map = map;
     if (o_starts) *o_starts = starts;
-    return leave();
+    return VKL_OK;
   }
 };
 
@@ -133,6 +164,7 @@ struct UpdatePagedOp : PagedOp {
   }
   int init() override {
     if (inited) return VKL_OK;
+    OnDevice here(dev->ordinal);
     if (!good_dtype(dtype)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: only fp16 and bf16 dtypes are supported.");
     if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: a page of %d tokens", page);
     if (!good_dim(dim)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: head dim %d is no multiple of 8 up to 256", dim);
@@ -144,9 +176,7 @@ struct UpdatePagedOp : PagedOp {
       VKL_CUDA(cudaMemcpyAsync(turns->data(), per.data(), per.size() * 8, cudaMemcpyHostToDevice, cmd->stream));
       VKL_CUDA(cudaStreamSynchronize(cmd->stream));
     }
-    uint32_t *word;
-    VKL_OKAY(command_error_word(cmd, &word));
-    return base_init();
+    return paged_init();
   }
   int run(vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *k, vkl_tensor *v, vkl_tensor *map, vkl_tensor *q, vkl_tensor **o) {
     const char *who = "update_paged_kvcache";
@@ -169,7 +199,7 @@ struct UpdatePagedOp : PagedOp {
     VKL_OKAY(check_apart(v, who, "values"));
     if (q) VKL_OKAY(check_apart(q, who, "queries"));
     if ((q ? q->w : 0) + 2 * k->w > 1u << 24) return fail(VKL_OUT_OF_RANGE, "%s: rows of %zu values", who, (q ? q->w : 0) + 2 * k->w);
-    VKL_OKAY(enter(who));
+    VKL_OKAY(begin(who));
     if (q) VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
     if (rows) {
       PagedUpdate p = {};
@@ -183,6 +213,7 @@ struct UpdatePagedOp : PagedOp {
       p.kcache = kcache->data(), p.vcache = vcache->data();
       p.map = (const uint32_t *)map->data();
       VKL_OKAY(command_error_word(cmd, &p.error));
+      p.stamps = stamp();
       p.rows = (uint32_t)rows, p.kv_heads = (uint32_t)kv_heads, p.dim = (uint32_t)dim, p.pages = (uint32_t)kcache->c;
       p.page = divisor(page);
       p.turns = turns ? (const double *)turns->data() : nullptr;
@@ -190,7 +221,7 @@ struct UpdatePagedOp : PagedOp {
       VKL_LAUNCH(1, launch_paged_update(p, cmd->stream));
     }
     if (o) *o = q ? out : nullptr;
-    return leave();
+    return VKL_OK;
   }
 };
 
@@ -206,22 +237,21 @@ struct PagedAttentionOp : PagedOp {
   }
   int init() override {
     if (inited) return VKL_OK;
+    OnDevice here(dev->ordinal);
     if (!good_dtype(dtype)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: only fp16 and bf16 dtypes are supported.");
     if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65535)
       return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: %d heads over %d key heads", heads, kv_heads);
     if (!good_dim(dim)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: head dim %d is no multiple of 8 up to 256", dim);
     if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: a page of %d tokens", page);
     if (window < 0) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: a window of %d positions", window);
-    if (!std::isfinite(scale)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: scale is %g", scale);
+    if (scale != 0.f && !(fabsf(scale) >= 1e-20f && fabsf(scale) <= 1e20f)) return fail(VKL_INVALID_ARGUMENT, "PagedAttention op: scale is %g", scale);
     const uint32_t sms = dev->prop.multiProcessorCount;
     VKL_CUDA(setup_paged_token());
     VKL_CUDA(setup_paged_prompt());
     VKL_OKAY(tensor_new(dev, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32, &scratch));
     VKL_OKAY(tensor_new(dev, 1, 1, sms + 1, VKL_UINT32, &counters));
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
-    uint32_t *word;
-    VKL_OKAY(command_error_word(cmd, &word));
-    return base_init();
+    return paged_init();
   }
   int run(vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths, vkl_tensor *starts, vkl_tensor **o) {
     const char *who = "paged_attention";
@@ -235,9 +265,10 @@ struct PagedAttentionOp : PagedOp {
     if (starts) VKL_OKAY(check_list(starts, who, "starts", n + 1));
     if (!starts && rows != n) return fail(VKL_INVALID_ARGUMENT, "%s: %zu queries for %zu sequences of one new token each", who, rows, n);
     VKL_OKAY(check_apart(q, who, "queries"));
-    if (rows * per > kMaxTokens || n * (table->w * page / 16 + 1) > 0xffffffffu || n > kMaxTokens)
+    // the one-token form counts tiles of 16 positions of all sequences and head groups in 31 bits
+    if (rows * per > kMaxTokens || n > kMaxTokens || (!starts && n * (table->w * page / 16 + 2) * (kv_heads * ((per + 7) / 8)) > kMaxTokens))
       return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, %zu sequences of up to %zu tokens", who, rows, n, table->w * page);
-    VKL_OKAY(enter(who));
+    VKL_OKAY(begin(who));
     VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
     if (rows && n) {
       PagedAttention p = {};
@@ -250,6 +281,7 @@ struct PagedAttentionOp : PagedOp {
       p.scratch = (float *)scratch->data();
       p.counters = (uint32_t *)counters->data();
       VKL_OKAY(command_error_word(cmd, &p.error));
+      p.stamps = stamp();
       p.rows = (uint32_t)rows, p.n = (uint32_t)n, p.heads = heads, p.kv_heads = kv_heads, p.dim = dim;
       p.width = (uint32_t)table->w, p.pages = (uint32_t)kcache->c, p.window = window;
       p.page = divisor(page);
@@ -259,7 +291,7 @@ struct PagedAttentionOp : PagedOp {
       VKL_LAUNCH(1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
     }
     *o = out;
-    return leave();
+    return VKL_OK;
   }
 };
 

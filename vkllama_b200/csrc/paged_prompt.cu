@@ -35,6 +35,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, kvh = blockIdx.y;
   const uint32_t per = p.heads / p.kv_heads;
   Place at;
+  follow();
+  stamp_begin(p.stamps);
   if (!find_tile<kThreads>(p, per, kRows, blockIdx.x, at)) return;
   const uint32_t packed = at.fresh * per, r_end = min(at.first + kRows, packed), past = at.len - at.fresh;
   // positions that the tile's rows see
@@ -187,6 +189,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
     for (uint32_t x = 0; x < 8; ++x)
       if (again >> (x * 4) & 15u) row_again<BF>(p, at, kvh, at.first + warp * 16 + i * 8 + x);
   }
+  stamp_end(p.stamps);
 }
 
 template <bool BF, int DP> cudaError_t setup_one() {
@@ -196,10 +199,9 @@ template <bool BF> cudaError_t pick(const PagedAttention &p, cudaStream_t s) {
   // tiles are counted on the device; every sequence has at most one that is not full
   const uint64_t per = p.heads / p.kv_heads, tiles = p.rows * per / kRows + std::min<uint64_t>(p.n, p.rows * per);
   const dim3 grid((uint32_t)tiles, p.kv_heads);
-  if (p.dim <= 64) paged_prompt_kernel<BF, 64><<<grid, kThreads, Cfg<64>::kSmem, s>>>(p);
-  else if (p.dim <= 128) paged_prompt_kernel<BF, 128><<<grid, kThreads, Cfg<128>::kSmem, s>>>(p);
-  else paged_prompt_kernel<BF, 256><<<grid, kThreads, Cfg<256>::kSmem, s>>>(p);
-  return cudaGetLastError();
+  if (p.dim <= 64) return launch_following(paged_prompt_kernel<BF, 64>, grid, kThreads, Cfg<64>::kSmem, s, p);
+  if (p.dim <= 128) return launch_following(paged_prompt_kernel<BF, 128>, grid, kThreads, Cfg<128>::kSmem, s, p);
+  return launch_following(paged_prompt_kernel<BF, 256>, grid, kThreads, Cfg<256>::kSmem, s, p);
 }
 
 }  // namespace

@@ -22,7 +22,7 @@ namespace vkl {
 namespace {
 
 constexpr uint32_t kThreads = 512, kWarps = kThreads / 32;
-constexpr uint32_t kRowsPerCta = 4096, kPagesPerCta = 16384;
+constexpr uint32_t kRowsPerCta = 2048, kPagesPerCta = 2048;
 
 struct Counts {
   uint32_t rows, need, give;
@@ -47,6 +47,8 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const PagedTable
   __shared__ unsigned long long total_s[3];
   __shared__ uint32_t bad_s, last_s;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  follow();
+  stamp_begin(p.stamps);
   const uint32_t count = p.pool[0];
   if (tid == 0) bad_s = 0;
   if (tid < 3) total_s[tid] = 0;
@@ -123,19 +125,32 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const PagedTable
       const uint32_t i = owner(need_before, p.n, k);
       p.table[(size_t)i * p.width + pages_of(p.lengths[i], p.page) + k - need_before[i]] = taken(k);
     }
-    for (uint32_t r = t0; r < p.rows; r += step) {
-      uint32_t slot = kNoSlot, pos = 0;
-      if (r < all_rows) {
-        const uint32_t i = owner(rows_before, p.n, r), len = p.lengths[i], have = pages_of(len, p.page);
-        pos = len + r - rows_before[i];
-        const uint32_t j = quotient(pos, p.page), in = pos - j * p.page.d;
-        const uint32_t page = j < have ? p.table[(size_t)i * p.width + j] : taken(need_before[i] + j - have);
-        const unsigned long long s = (unsigned long long)page * p.page.d + in;
-        slot = s < kNoSlot ? (uint32_t)s : kNoSlot;
-        if (s >= kNoSlot) raise(p.error, PAGED_BAD_PAGE);
+    for (uint32_t r4 = t0 * 4; r4 < p.rows; r4 += step * 4) {  // four rows: one bisection, mostly one page
+      uint32_t i = 0, next = 0, len = 0, have = 0, j_at = 0xffffffffu, page = 0;
+      if (r4 < all_rows) i = owner(rows_before, p.n, r4);
+#pragma unroll
+      for (uint32_t r = r4; r < r4 + 4; ++r) {
+        if (r >= p.rows) break;
+        uint32_t slot = kNoSlot, pos = 0;
+        if (r < all_rows) {
+          if (r == r4 || r >= next) {
+            while (r >= rows_before[i + 1]) ++i;
+            next = rows_before[i + 1];
+            len = p.lengths[i];
+            have = pages_of(len, p.page);
+            j_at = 0xffffffffu;
+          }
+          pos = len + r - rows_before[i];
+          const uint32_t j = quotient(pos, p.page);
+          if (j != j_at) page = j < have ? p.table[(size_t)i * p.width + j] : taken(need_before[i] + j - have);
+          j_at = j;
+          const unsigned long long s = (unsigned long long)page * p.page.d + (pos - j * p.page.d);
+          if (s < kNoSlot) slot = (uint32_t)s;
+          else raise(p.error, PAGED_BAD_PAGE);
+        }
+        p.map[r] = slot;
+        p.map[p.rows + r] = pos;
       }
-      p.map[r] = slot;
-      p.map[p.rows + r] = pos;
     }
   }
 
@@ -153,7 +168,9 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const PagedTable
   } else {
     __syncthreads();
   }
-  if (!last || bad) return;
+  if (!last) return;
+  stamp_end(p.stamps);
+  if (bad) return;
   if (tid == 0) p.pool[0] = count + (uint32_t)total_s[2] - (uint32_t)total_s[1];
   for (uint32_t i = i0; i < i1; ++i) p.lengths[i] = p.target[i];
 }
@@ -171,8 +188,7 @@ cudaError_t launch_paged_tables(const PagedTables &p, uint32_t sms, cudaStream_t
   const uint64_t ctas = ((uint64_t)p.rows + kRowsPerCta - 1) / kRowsPerCta, more = pages / kPagesPerCta;
   uint64_t grid = ctas > more ? ctas : more;
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;
-  paged_tables_kernel<<<(uint32_t)grid, kThreads, tables_smem(p.n), s>>>(p);
-  return cudaGetLastError();
+  return launch_following(paged_tables_kernel, dim3((uint32_t)grid), kThreads, tables_smem(p.n), s, p);
 }
 
 }  // namespace vkl

@@ -6,7 +6,7 @@
 // rows of A, cached rows the columns. A tile's upper eight rows would be empty; in P.V they carry what rounding the probabilities to
 // 16 bits leaves over (p = hi + lo, both exact products, added at the end), so the result has the probabilities' 32 bits at no cost.
 //
-// Work is cut into equal shares, not by sequence: the tiles of 16 positions of all (sequence, head group) pairs stand in one row, every
+// Work is cut into equal shares, not by sequence: the tiles (of 16 or 32 positions) of all (sequence, head group) pairs stand in one row (and a place more for each pair's own cost), every
 // CTA takes a range of it and every warp of the CTA a range of that, however the lengths are spread. Ranges cut pairs: a warp keeps
 // running maximum, sum and output of its part; parts meet in shared memory, and those of several CTAs in scratch, where the CTA that
 // arrives last adds them up in their order (the result does not depend on who that is). Cuts that would leave a small piece of a pair are
@@ -24,21 +24,29 @@ namespace vkl {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kTile = 16;                // positions
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
-constexpr uint32_t kShareTiles = 16;          // a CTA's share is at least this many tiles
-constexpr uint32_t kSnapTiles = 16;           // a cut this near to a pair's border moves there
+constexpr uint32_t kShareRows = 256;          // a CTA's share is at least this many positions
+constexpr uint32_t kSnapRows = 256;           // a cut this near to a pair's border moves there
+constexpr uint32_t kPairCost = 1;             // what a pair costs beside its tiles (queries, output, short rows in the ring), in tiles
 
 // DP: padded head width, MG: groups of eight query heads.
 template <int DP, int MG> struct Cfg {
-  static constexpr uint32_t kHalf = kTile * DP * 2;  // bytes of a tile's keys, or values
-  static constexpr uint32_t kRing = DP == 64 ? 8 : DP == 128 ? (MG == 1 ? 6 : 4) : 2;
+  static constexpr uint32_t kTile = DP * MG <= 128 ? 32 : 16;  // positions of a tile: 32 where the registers suffice, half the softmax steps
+  static constexpr uint32_t kHalf = kTile * DP * 2;            // bytes of a tile's keys, or values
+  static constexpr uint32_t kRing = DP == 64 ? 5 : DP == 128 ? (MG == 1 ? 3 : 4) : 2;
   static constexpr uint32_t kHeads = 8 * MG;
   static constexpr uint32_t kStash = kHeads * DP * 4;  // a warp's first part, where its range goes on behind it
   static constexpr uint32_t kSmem = kWarps * (kRing * kHalf + kStash + 2 * kHeads * 2 * 4);
-  static_assert(kSmem + 1536 <= 227 * 1024, "shared memory of an SM");
+  static constexpr uint32_t kShare = kShareRows / kTile, kSnap = kSnapRows / kTile;
+  static_assert(kSmem + 2048 <= 227 * 1024, "shared memory of an SM");
   static_assert(kRing * kHalf >= kStash, "a warp's last part lies in its ring");
 };
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 struct Pair {        // tiles t .. t1 of a sequence and head group
   uint32_t seq, grp;
@@ -55,12 +63,12 @@ struct Part {
 template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1) paged_token_kernel(const PagedAttention p) {
   using C = Cfg<DP, MG>;
   constexpr uint32_t CH = DP / 8;            // 16-byte pieces of a row
-  constexpr uint32_t NC = kTile * CH / 32;   // of a half and lane
-  constexpr int KS = DP / 16, NT = DP / 8;
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr uint32_t T = C::kTile, NC = T * CH / 32;  // pieces of a half and lane
+  constexpr int KS = DP / 16, NT = DP / 8, SN = T / 8;
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ uint32_t before_s[kThreads + 1];  // tiles of one head group's sequences; the host has checked that they fit 32 bits
   __shared__ uint32_t warp_sum_s[kWarps];
-  __shared__ uint64_t border_s[2];
+  __shared__ uint32_t border_s[2];
   __shared__ Part part_s[kWarps][2];
   __shared__ uint32_t last_s[2];
   unsigned char *ring = smem + threadIdx.x / 32 * C::kRing * C::kHalf;
@@ -68,19 +76,25 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   float *ml = reinterpret_cast<float *>(smem + kWarps * (C::kRing * C::kHalf + C::kStash));  // [warp][2][head][2]
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const uint32_t per = p.heads / p.kv_heads, groups = (per + C::kHeads - 1) / C::kHeads, pairs = p.kv_heads * groups;
+  const float scale = fabsf(p.scale) * kLog2e;  // maxima are of the plain products; a negative scale turns the queries round
+  const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
   const uint32_t room = p.width * p.page.d;  // positions that a table holds (checked by the host to fit 31 bits)
 
+  follow();
+  stamp_begin(p.stamps);
   // ---- where this CTA's and this warp's range is ----
   auto length = [&](uint32_t i) { return min(p.lengths[i], room); };
   auto first_of = [&](uint32_t len) { return p.window && len > p.window ? len - p.window : 0u; };
-  auto tiles = [&](uint32_t len) { return max((len + kTile - 1) / kTile, 1u) - first_of(len) / kTile; };
+  // A pair's tiles, and the places that it takes up in the row of all work.
+  auto tiles = [&](uint32_t len) { return max((len + T - 1) / T, 1u) - first_of(len) / T; };
+  auto places = [&](uint32_t len) { return tiles(len) + kPairCost; };
   const uint32_t each = (p.n + kThreads - 1) / kThreads;
   {
     const uint32_t i0 = min(tid * each, p.n), i1 = min(i0 + each, p.n);
     uint32_t mine = 0;
     for (uint32_t i = i0; i < i1; ++i) {
       if (p.lengths[i] > room && blockIdx.x == 0) raise(p.error, PAGED_TABLE_FULL);
-      mine += tiles(length(i));
+      mine += places(length(i));
     }
     uint32_t up = mine;
 #pragma unroll
@@ -97,48 +111,64 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     if (tid == kThreads - 1) before_s[kThreads] = base + up;
     __syncthreads();
   }
-  const uint64_t total = (uint64_t)before_s[kThreads] * pairs;
-  const uint64_t share = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)kShareTiles);
-  auto find = [&](uint64_t pos) {  // the pair and tile at pos < total
+  const uint32_t total = before_s[kThreads] * pairs, share = max((total + gridDim.x - 1) / gridDim.x, C::kShare);
+  auto find = [&](uint32_t pos) {  // the pair at place pos < total; t: tiles of it that lie before pos
     uint32_t lo = 0, hi = kThreads;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) >> 1;
-      if ((uint64_t)before_s[mid] * pairs <= pos) lo = mid;
+      if (before_s[mid] * pairs <= pos) lo = mid;
       else hi = mid;
     }
     Pair r;
     r.seq = lo * each;
-    uint64_t left = pos - (uint64_t)before_s[lo] * pairs;
-    uint32_t len = length(r.seq), n = tiles(len);
-    while (left >= (uint64_t)n * pairs) {
-      left -= (uint64_t)n * pairs;
+    uint32_t left = pos - before_s[lo] * pairs, len = length(r.seq), n = places(len);
+    while (left >= n * pairs) {
+      left -= n * pairs;
       len = length(++r.seq);
-      n = tiles(len);
+      n = places(len);
     }
-    r.grp = (uint32_t)(left / n);
+    r.grp = left / n;
     r.len = len;
     r.first = first_of(len);
-    r.t0 = r.first / kTile;
-    r.t1 = r.t0 + n;
-    r.t = r.t0 + (uint32_t)(left - (uint64_t)r.grp * n);
+    r.t0 = r.first / T;
+    r.t1 = r.t0 + n - kPairCost;
+    r.t = r.t0 + left - r.grp * n;
     return r;
   };
   if (tid < 2) {  // the range's borders
-    uint64_t b = (blockIdx.x + tid) * share;
-    if (b >= total) {
-      b = total;
-    } else if (b > 0) {
+    uint32_t b = min((uint64_t)(blockIdx.x + tid) * share, (uint64_t)total);
+    if (b > 0 && b < total) {
       const Pair r = find(b);
-      const uint32_t in = r.t - r.t0, out = r.t1 - r.t;
-      if (min(in, out) <= kSnapTiles) b = in <= out ? b - in : b + out;
+      const uint32_t in = r.t - r.t0, out = r.t1 + kPairCost - r.t;
+      if (min(in, out) <= C::kSnap) b = in <= out ? b - in : b + out;
     }
     border_s[tid] = b;
   }
   __syncthreads();
-  const uint64_t b0 = border_s[0], b1 = border_s[1];
+  const uint32_t b0 = border_s[0], b1 = border_s[1];
   if (b0 == b1) return;
-  const uint64_t w0 = b0 + (b1 - b0) * warp / kWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kWarps;
-  const uint32_t count = (uint32_t)(w1 - w0);
+  // A warp's places: pairs' tiles, and the places behind them that stand for a pair's cost.
+  const uint32_t part = (b1 - b0) / kWarps, more = (b1 - b0) % kWarps;
+  const uint32_t w0 = b0 + part * warp + min(warp, more), w1 = w0 + part + (warp < more);
+  Pair at = {};
+  uint32_t count;  // its tiles
+  {
+    const uint32_t pos = lane & 1 ? w1 : w0;  // both ends at once
+    uint32_t before = total - p.n * pairs * kPairCost;  // tiles before pos
+    if (pos < total) {
+      at = find(pos);
+      const uint32_t in = at.t - at.t0, n = at.t1 - at.t0;
+      before = pos - (at.seq * pairs + at.grp) * kPairCost - (in > n ? in - n : 0);
+    }
+    count = __shfl_sync(0xffffffffu, before, 1) - __shfl_sync(0xffffffffu, before, 0);
+    at.seq = __shfl_sync(0xffffffffu, at.seq, 0);
+    at.grp = __shfl_sync(0xffffffffu, at.grp, 0);
+    at.t = __shfl_sync(0xffffffffu, at.t, 0);
+    at.t0 = __shfl_sync(0xffffffffu, at.t0, 0);
+    at.t1 = __shfl_sync(0xffffffffu, at.t1, 0);
+    at.len = __shfl_sync(0xffffffffu, at.len, 0);
+    at.first = __shfl_sync(0xffffffffu, at.first, 0);
+  }
 
   auto advance = [&](Pair &r) {
     if (++r.t < r.t1) return;
@@ -147,7 +177,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       if (++r.seq >= p.n) return;
       r.len = length(r.seq);
       r.first = first_of(r.len);
-      r.t0 = r.first / kTile;
+      r.t0 = r.first / T;
       r.t1 = r.t0 + tiles(r.len);
     }
     r.t = r.t0;
@@ -159,22 +189,33 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   auto heads_of = [&](uint32_t grp) { return min(per - grp % groups * C::kHeads, C::kHeads); };
 
   if (count) {
+    if (at.t >= at.t1) {  // the range begins behind a pair's last tile
+      at.t = at.t1 - 1;
+      advance(at);
+    }
     // ---- the stream: tile halves, keys and values in turn, go into the ring's places one after the other ----
-    Pair in = find(w0), at = in;
+    Pair in = at;
     uint32_t left = count, entry = 0, in_page = 0, row_at = 0xffffffffu, slot_in = 0;
     bool values = false;
     const uint32_t ring_a = smem_addr(ring);
     auto look_up = [&]() {  // the page of this lane's position of the tile that comes next
-      const uint32_t j = in.t * kTile + (lane & 15);
+      const uint32_t j = in.t * T + lane % T;
+      entry = kNoSlot;
       if (j >= in.first && j < in.len) {
-        const uint32_t q = quotient(j, p.page);
-        entry = __ldg(p.table + (size_t)in.seq * p.width + q);
-        in_page = j - q * p.page.d;
-      } else {
-        entry = kNoSlot;
+        const uint32_t n = quotient(j, p.page);
+        entry = __ldg(p.table + (size_t)in.seq * p.width + n);
+        in_page = j - n * p.page.d;
       }
     };
     look_up();
+    // Pieces of a half: lane l has piece l % CH of row l / CH of every 32 / CH rows. Piece c of row r lies at piece c ^ (r % 8), and what
+    // that exclusive-or takes from i is the same for every lane.
+    constexpr uint32_t RS = 32 / CH;
+    const uint32_t col = lane % CH, prow = lane / CH;
+    const bool col_there = col * 8 < p.dim;
+    const uint32_t piece = prow * CH * 16 + ((col ^ prow) << 4);
+    const uint64_t step = (uint64_t)RS * p.dim * 2;
+    const bool tiled_pages = p.page.d % 16 == 0;
     auto request = [&]() {
       if (left) {
         if (!values) {
@@ -182,14 +223,23 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
           if (entry < p.pages) row_at = (entry * p.kv_heads + in.grp / groups) * p.page.d + in_page;  // the host has checked that rows fit 32 bits
           else if (entry != kNoSlot) raise(p.error, PAGED_BAD_PAGE);
         }
-        const uint16_t *src = static_cast<const uint16_t *>(values ? p.vcache : p.kcache);
-        const uint32_t dst = ring_a + slot_in * C::kHalf;
+        const uint8_t *cache = static_cast<const uint8_t *>(values ? p.vcache : p.kcache);
+        const uint32_t dst = ring_a + slot_in * C::kHalf + piece;
+        if (tiled_pages && in.t * T >= in.first && in.t * T + T <= in.len && __all_sync(0xffffffffu, entry < p.pages)) {  // whole: sixteen rows follow each other in a page
 #pragma unroll
-        for (uint32_t i = 0; i < NC; ++i) {
-          const uint32_t c = i * 32 + lane, row = c / CH, col = c % CH;
-          const uint32_t r = __shfl_sync(0xffffffffu, row_at, row);
-          const bool there = r != 0xffffffffu && col * 8 < p.dim;
-          copy16(dst + (row * CH + (col ^ (row & 7))) * 16, there ? src + (size_t)r * p.dim + col * 8 : src, there);
+          for (uint32_t h = 0; h < T / 16; ++h) {
+            const uint32_t r = T == 16 ? row_at - lane % T : __shfl_sync(0xffffffffu, row_at, h * 16);
+            const uint8_t *src = cache + ((size_t)(r + prow) * p.dim + (col_there ? col * 8 : 0)) * 2;
+#pragma unroll
+            for (uint32_t i = h * NC * 16 / T; i < (h + 1) * NC * 16 / T; ++i, src += step) copy16((dst ^ (i * RS % 8) << 4) + i * 512, src, col_there);
+          }
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < NC; ++i) {
+            const uint32_t r = __shfl_sync(0xffffffffu, row_at, i * RS + prow);
+            const bool there = r != 0xffffffffu && col_there;
+            copy16((dst ^ (i * RS % 8) << 4) + i * 512, there ? cache + ((size_t)r * p.dim + col * 8) * 2 : cache, there);
+          }
         }
         if (values && --left) {
           advance(in);
@@ -218,7 +268,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t d = k * 16 + e * 8 + t4 * 2;
-            q[m][k][e] = m * 8 + g < nh && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) : 0u;
+            q[m][k][e] = m * 8 + g < nh && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) ^ flip : 0u;
           }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -240,89 +290,95 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       }
     };
     start_pair();
-    const float scale = p.scale * kLog2e;
     const uint32_t lrow = lane & 7, lsel = lane >> 3;  // ldmatrix: row of a matrix, which of the four
+    const uint32_t k_at = (lrow + (lsel >> 1) * 8) * CH * 16 + (((lsel & 1) ^ lrow) << 4);
+    const uint32_t v_at = (lrow + (lsel & 1) * 8) * CH * 16 + (((lsel >> 1) ^ lrow) << 4);
 #pragma unroll 1
     for (uint32_t it = 0; it < count; ++it) {
       copy_wait<C::kRing - 1>();
       __syncwarp();
       // S = Q K^T: matrices (rows 0-7 | 8-15) x (k low | k high)
-      float s[MG][2][4];
+      float s[MG][SN][4];
 #pragma unroll
       for (int m = 0; m < MG; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
       {
-        const uint32_t kt = ring_a + slot * C::kHalf;
-        const uint32_t row = lrow + (lsel >> 1) * 8;
+        const uint32_t kt = ring_a + slot * C::kHalf + k_at;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t b[4];
-          ldmatrix4(b, kt + (row * CH + ((2 * k + (lsel & 1)) ^ lrow)) * 16);
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int m = 0; m < MG; ++m) {
-            mma2<BF>(s[m][0], q[m][k][0], 0, q[m][k][1], 0, b[0], b[1]);
-            mma2<BF>(s[m][1], q[m][k][0], 0, q[m][k][1], 0, b[2], b[3]);
+          for (int n = 0; n < SN; n += 2) {
+            uint32_t b[4];
+            ldmatrix4(b, (kt ^ k << 5) + n * 8 * CH * 16);
+#pragma unroll
+            for (int m = 0; m < MG; ++m) {
+              mma2<BF>(s[m][n], q[m][k][0], 0, q[m][k][1], 0, b[0], b[1]);
+              mma2<BF>(s[m][n + 1], q[m][k][0], 0, q[m][k][1], 0, b[2], b[3]);
+            }
           }
-        }
       }
       slot = slot + 1 == C::kRing ? 0 : slot + 1;
       __syncwarp();
       request();
       // softmax so far
-      const uint32_t j0 = at.t * kTile + t4 * 2;
-      uint32_t pa[MG][4];
+      if (at.t * T < at.first || at.t * T + T > at.len) {
+#pragma unroll
+        for (int n = 0; n < SN; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t j = at.t * T + n * 8 + t4 * 2 + e;
+            if (j < at.first || j >= at.len) {
+#pragma unroll
+              for (int m = 0; m < MG; ++m) s[m][n][e] = -INFINITY;
+            }
+          }
+      }
+      uint32_t pa[MG][SN][2];  // high and low parts
 #pragma unroll
       for (int m = 0; m < MG; ++m) {
-        float v[4];
+        float top = mx[m];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t j = j0 + (e >> 1) * 8 + (e & 1);
-          v[e] = j >= at.first && j < at.len ? s[m][e >> 1][e & 1] * scale : -INFINITY;
-        }
-        float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(s[m][n][0], s[m][n][1]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float now = fmaxf(mx[m], top), ref = now == -INFINITY ? 0.f : now;
-        if (__any_sync(0xffffffffu, now != mx[m])) {
-          const float c = exp2f(mx[m] - ref);
+        const float ref = top == -INFINITY ? 0.f : top * scale;
+        if (__any_sync(0xffffffffu, top != mx[m])) {
+          const float c = exp2_fast(mx[m] * scale - ref);
           sum[m] *= c;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[m][n][e] *= c;
-          mx[m] = now;
+          mx[m] = top;
         }
-        float hi[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = exp2f(v[e] - ref);
-          sum[m] += v[e];
+        for (int n = 0; n < SN; ++n) {
+          const float a = exp2_fast(fmaf(s[m][n][0], scale, -ref)), b = exp2_fast(fmaf(s[m][n][1], scale, -ref));
+          sum[m] += a + b;
+          pa[m][n][0] = pack2<BF>(a, b);
+          const float2 hi = unpack2<BF>(pa[m][n][0]);
+          pa[m][n][1] = pack2<BF>(a - hi.x, b - hi.y);
         }
-        pa[m][0] = pack2<BF>(v[0], v[1]);
-        pa[m][2] = pack2<BF>(v[2], v[3]);
-        const float2 h01 = unpack2<BF>(pa[m][0]), h23 = unpack2<BF>(pa[m][2]);
-        hi[0] = h01.x, hi[1] = h01.y, hi[2] = h23.x, hi[3] = h23.y;
-        pa[m][1] = pack2<BF>(v[0] - hi[0], v[1] - hi[1]);
-        pa[m][3] = pack2<BF>(v[2] - hi[2], v[3] - hi[3]);
       }
       copy_wait<C::kRing - 1>();
       __syncwarp();
       {
-        const uint32_t vt = ring_a + slot * C::kHalf;
-        const uint32_t row = lrow + (lsel & 1) * 8;
+        const uint32_t vt = ring_a + slot * C::kHalf + v_at;
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-          uint32_t b[4];
-          ldmatrix4_t(b, vt + (row * CH + ((n + (lsel >> 1)) ^ lrow)) * 16);
+        for (int k = 0; k < SN; k += 2)
 #pragma unroll
-          for (int m = 0; m < MG; ++m) {
-            mma2<BF>(o[m][n], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b[0], b[1]);
-            mma2<BF>(o[m][n + 1], pa[m][0], pa[m][1], pa[m][2], pa[m][3], b[2], b[3]);
+          for (int n = 0; n < NT; n += 2) {
+            uint32_t b[4];
+            ldmatrix4_t(b, (vt ^ n << 4) + k * 8 * CH * 16);
+#pragma unroll
+            for (int m = 0; m < MG; ++m) {
+              mma2<BF>(o[m][n], pa[m][k][0], pa[m][k][1], pa[m][k + 1][0], pa[m][k + 1][1], b[0], b[1]);
+              mma2<BF>(o[m][n + 1], pa[m][k][0], pa[m][k][1], pa[m][k + 1][0], pa[m][k + 1][1], b[2], b[3]);
+            }
           }
-        }
       }
       slot = slot + 1 == C::kRing ? 0 : slot + 1;
       __syncwarp();
@@ -393,20 +449,26 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     const uint32_t side = a.begins ? 1 : 0;  // where it goes in scratch
     const uint32_t h0 = first_head(a.grp), nh = heads_of(a.grp);
     for (uint32_t h = (warp + kWarps - run % kWarps) % kWarps; h < nh; h += kWarps) {
+      // lane x has part x's maximum and sum
       float m = -INFINITY, l = 0.f;
-      for (uint32_t x = i; x < e; ++x)
-        if (part_s[x >> 1][x & 1].there) m = fmaxf(m, ml[(x * C::kHeads + h) * 2]);
-      const float ref = m == -INFINITY ? 0.f : m;
+      if (lane >= i && lane < e && part_s[lane >> 1][lane & 1].there) {
+        const float2 v = *reinterpret_cast<const float2 *>(ml + (lane * C::kHeads + h) * 2);
+        m = v.x, l = v.y;
+      }
+      const float top = warp_max(m), ref = top == -INFINITY ? 0.f : top * scale;
+      const float c = exp2_fast(m * scale - ref);
+      l = warp_sum(l * c);
+      m = top;
       float2 acc[DP / 64] = {};
-      for (uint32_t x = i; x < e; ++x) {
-        if (!part_s[x >> 1][x & 1].there) continue;
-        const float c = exp2f(ml[(x * C::kHeads + h) * 2] - ref);
-        l += c * ml[(x * C::kHeads + h) * 2 + 1];
+#pragma unroll
+      for (uint32_t x = 0; x < 2 * kWarps; ++x) {
+        if (x < i || x >= e || !part_s[x >> 1][x & 1].there) continue;
+        const float cx = __shfl_sync(0xffffffffu, c, x);
         const float *src = part_o(x) + h * DP;
 #pragma unroll
         for (int d = 0; d < DP / 64; ++d) {
           const float2 v = *reinterpret_cast<const float2 *>(src + d * 64 + lane * 2);
-          acc[d].x += c * v.x, acc[d].y += c * v.y;
+          acc[d].x += cx * v.x, acc[d].y += cx * v.y;
         }
       }
       if (whole) {
@@ -427,28 +489,30 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     ++run;
     i = e;
   }
-  if (!open[0].there && !open[1].there) return;
+  if (!open[0].there && !open[1].there) {
+    stamp_end(p.stamps);
+    return;
+  }
 
-  // ---- pairs of several CTAs: cuts are the multiples of the share that lie further than kSnapTiles inside the pair ----
+  // ---- pairs of several CTAs: cuts are the multiples of the share that lie further than C::kSnap inside the pair ----
   __threadfence();
   __syncthreads();
-  uint64_t cut0[2], cut1[2];
+  uint32_t cut0[2], cut1[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     cut0[side] = cut1[side] = 0;
     if (!open[side].there) continue;
-    const uint32_t s = open[side].seq, base = s / each;
-    uint64_t begin = before_s[base];
-    for (uint32_t i = base * each; i < s; ++i) begin += tiles(length(i));
-    const uint64_t n = tiles(length(s));
+    const uint32_t s = open[side].seq, base = s / each, n = places(length(s));
+    uint32_t begin = before_s[base];
+    for (uint32_t i = base * each; i < s; ++i) begin += places(length(i));
     begin = begin * pairs + n * open[side].grp;
-    cut0[side] = (begin + kSnapTiles) / share + 1;
-    cut1[side] = (begin + n - kSnapTiles - 1) / share;  // cut0 <= cut1: n > 2 kSnapTiles where a cut is left
+    cut0[side] = (begin + C::kSnap) / share + 1;
+    cut1[side] = (begin + n - C::kSnap - 1) / share;  // cut0 <= cut1: n > 2 C::kSnap where a cut is left
   }
   if (tid < 2) {
     last_s[tid] = 0;
     if (open[tid].there) {
-      const uint32_t c0 = (uint32_t)cut0[tid], parts = (uint32_t)(cut1[tid] - cut0[tid]) + 2;
+      const uint32_t c0 = cut0[tid], parts = cut1[tid] - cut0[tid] + 2;
       __threadfence();
       if (atomicAdd(p.counters + c0, 1u) + 1 == parts) {
         p.counters[c0] = 0;
@@ -463,18 +527,18 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     __threadfence();
     const Part a = open[side];
     const uint32_t h0 = first_head(a.grp), nh = heads_of(a.grp);
-    const uint32_t c0 = (uint32_t)cut0[side], c1 = (uint32_t)cut1[side];
+    const uint32_t c0 = cut0[side], c1 = cut1[side];
     auto rec = [&](uint32_t c, uint32_t h) { return ((size_t)c * 2 + (c + 1 == c0 ? 1 : 0)) * C::kHeads + h; };  // the first part ends its CTA's range
     for (uint32_t h = warp; h < nh; h += kWarps) {
       float m = -INFINITY, l = 0.f;
       for (uint32_t c = c0 - 1 + lane; c <= c1; c += 32) m = fmaxf(m, __ldcg(scratch_ml + rec(c, h) * 2));
       m = warp_max(m);
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m * scale;
       float2 acc[DP / 64] = {};
 #pragma unroll 4
       for (uint32_t c = c0 - 1; c <= c1; ++c) {
         const float2 x = __ldcg(reinterpret_cast<const float2 *>(scratch_ml + rec(c, h) * 2));
-        const float w = exp2f(x.x - ref);
+        const float w = exp2_fast(x.x * scale - ref);
         l += w * x.y;
 #pragma unroll
         for (int d = 0; d < DP / 64; ++d) {
@@ -487,17 +551,18 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       for (int d = 0; d < DP / 64; ++d) write_out(a.seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
     }
   }
+  stamp_end(p.stamps);
 }
 
 template <bool BF, int DP, int MG> cudaError_t setup_one() {
   return cudaFuncSetAttribute(paged_token_kernel<BF, DP, MG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP, MG>::kSmem);
 }
 template <bool BF, int DP, int MG> cudaError_t run(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
+  using C = Cfg<DP, MG>;
   // No more CTAs than there can be shares of.
   const uint64_t per = p.heads / p.kv_heads, pairs = (uint64_t)p.kv_heads * ((per + 8 * MG - 1) / (8 * MG));
-  const uint64_t most = p.n * pairs * (((uint64_t)p.width * p.page.d + kTile - 1) / kTile), shares = (most + kShareTiles - 1) / kShareTiles;
-  paged_token_kernel<BF, DP, MG><<<(uint32_t)std::min<uint64_t>(sms, shares), kThreads, Cfg<DP, MG>::kSmem, s>>>(p);
-  return cudaGetLastError();
+  const uint64_t most = p.n * pairs * (((uint64_t)p.width * p.page.d + C::kTile - 1) / C::kTile + kPairCost), shares = (most + C::kShare - 1) / C::kShare;
+  return launch_following(paged_token_kernel<BF, DP, MG>, dim3((uint32_t)std::min<uint64_t>(sms, shares)), kThreads, C::kSmem, s, p);
 }
 template <bool BF> cudaError_t pick(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
   // Sixteen query heads per warp where a group has more than eight and their outputs fit the registers: keys and values are read

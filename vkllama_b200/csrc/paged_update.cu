@@ -20,6 +20,8 @@ constexpr uint32_t kMaxPairs = 128;
 
 template <bool BF> __global__ void __launch_bounds__(kThreads) paged_update_kernel(const PagedUpdate p) {
   __shared__ float2 turn_s[kMaxPairs];
+  follow();
+  stamp_begin(p.stamps);
   const uint32_t row = blockIdx.x, tid = threadIdx.x, per = p.dim / 8;
   const uint32_t nq = p.q ? p.heads * per : 0, nk = p.kv_heads * per, all = nq + 2 * nk, first = blockIdx.y * kThreads * kPieces + tid;
   uint4 x[kPieces];
@@ -68,15 +70,14 @@ template <bool BF> __global__ void __launch_bounds__(kThreads) paged_update_kern
       *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(key ? p.kcache : p.vcache) + (to * per + at - head * per) * 8) = x[i];
     }
   }
+  if (blockIdx.x + 1024 >= gridDim.x) stamp_end(p.stamps);  // of the CTAs that may be the last
 }
 
 }  // namespace
 
 cudaError_t launch_paged_update(const PagedUpdate &p, cudaStream_t s) {
   const uint32_t pieces = ((p.q ? p.heads : 0) + 2 * p.kv_heads) * (p.dim / 8), parts = (pieces + kThreads * kPieces - 1) / (kThreads * kPieces);
-  if (p.bf) paged_update_kernel<true><<<dim3(p.rows, parts), kThreads, 0, s>>>(p);
-  else paged_update_kernel<false><<<dim3(p.rows, parts), kThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  return launch_following(p.bf ? paged_update_kernel<true> : paged_update_kernel<false>, dim3(p.rows, parts), kThreads, 0, s, p);
 }
 
 }  // namespace vkl
