@@ -123,7 +123,10 @@ cudaError_t launch_paged_token(const PagedAttention &p, uint32_t sms, cudaStream
 size_t paged_token_scratch(uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t sms);
 cudaError_t setup_paged_token();   // once per device
 // Any number of rows per sequence.
-cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStream_t s);
+cudaError_t launch_paged_prompt(const PagedAttention &p, cudaStream_t s);
 cudaError_t setup_paged_prompt();
+// The same on tcgen05, heads up to 128 wide.
+cudaError_t launch_paged_prompt_tc(const PagedAttention &p, cudaStream_t s);
+cudaError_t setup_paged_prompt_tc();
 
 }  // namespace vkl

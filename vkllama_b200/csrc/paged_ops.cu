@@ -248,6 +248,7 @@ struct PagedAttentionOp : PagedOp {
     const uint32_t sms = dev->prop.multiProcessorCount;
     VKL_CUDA(setup_paged_token());
     VKL_CUDA(setup_paged_prompt());
+    VKL_CUDA(setup_paged_prompt_tc());
     VKL_OKAY(tensor_new(dev, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32, &scratch));
     VKL_OKAY(tensor_new(dev, 1, 1, sms + 1, VKL_UINT32, &counters));
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
@@ -287,8 +288,7 @@ struct PagedAttentionOp : PagedOp {
       p.page = divisor(page);
       p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
       p.bf = dtype == VKL_BF16;
-      const uint32_t sms = dev->prop.multiProcessorCount;
-      VKL_LAUNCH(1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
+      VKL_LAUNCH(1, starts ? launch_paged_prompt(p, cmd->stream) : launch_paged_token(p, dev->prop.multiProcessorCount, cmd->stream));
     }
     *o = out;
     return VKL_OK;

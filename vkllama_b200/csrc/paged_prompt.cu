@@ -20,6 +20,7 @@ namespace vkl {
 namespace {
 
 constexpr uint32_t kThreads = 128, kRows = 64;
+constexpr uint32_t kTensorRows = 96;  // packed rows of a sequence on average, from which the tcgen05 kernel has them
 
 template <int DP> struct Cfg {
   static constexpr uint32_t kKeys = DP == 256 ? 32 : 64;  // positions of a tile
@@ -211,6 +212,9 @@ cudaError_t setup_paged_prompt() {
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
-cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t, cudaStream_t s) { return p.bf ? pick<true>(p, s) : pick<false>(p, s); }
+cudaError_t launch_paged_prompt(const PagedAttention &p, cudaStream_t s) {
+  if (p.dim <= 128 && (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n) return launch_paged_prompt_tc(p, s);
+  return p.bf ? pick<true>(p, s) : pick<false>(p, s);
+}
 
 }  // namespace vkl
