@@ -248,7 +248,7 @@ def test_infinite_and_missing_numbers_where_a_token_sees_them(dev):
 
 
 # ---- attention of several rows -----------------------------------------------------------------------------------------
-def prompt(dev, past, new, heads, kv, dim, page, dtype, window=0, wide=0, behind=0, std=1.0, cache=None, finite=True):
+def prompt(dev, past, new, heads, kv, dim, page, dtype, window=0, wide=0, behind=0, std=1.0, cache=None, finite=True, scale=None):
     rng = np.random.default_rng(sum(new) + dim)
     lengths = [a + b for a, b in zip(past, new)]
     cache = cache or Cache(rng, lengths, kv, dim, page, dtype, std=std)
@@ -259,7 +259,7 @@ def prompt(dev, past, new, heads, kv, dim, page, dtype, window=0, wide=0, behind
     with cmd:
         k, v, table, lens = cache.up(cmd, dev)
         q = tensor(cmd, dev, bits, dtype).view(1, rows, heads * dim)
-        op, starts_t = vk.PagedAttention(dev, cmd, heads, kv, dim, page, 0.0, window, dtype).init(), tensor(cmd, dev, starts)
+        op, starts_t = vk.PagedAttention(dev, cmd, heads, kv, dim, page, scale or 0.0, window, dtype).init(), tensor(cmd, dev, starts)
         out = op(q, k, v, table, lens, starts_t)
         cmd.upload(mark, out)
         first = cmd.download(op(q, k, v, table, lens, starts_t))
@@ -267,7 +267,7 @@ def prompt(dev, past, new, heads, kv, dim, page, dtype, window=0, wide=0, behind
     got, q = (to_values(a, dtype).reshape(rows, heads, dim) for a in (first, bits[:, :heads * dim]))
     for i, l in enumerate(lengths):
         mine = slice(starts[i], starts[i + 1])
-        want, mass, size = attend(cache, i, q[mine], list(range(past[i], l)), window)
+        want, mass, size = attend(cache, i, q[mine], list(range(past[i], l)), window, scale)
         if new[i] and finite:
             big = np.abs(to_values(cache.seq_v[i], dtype)).max(initial=0)
             check(got[mine], want, mass, size, dtype, dim, l, big, True, "sequence %d, %d behind %d" % (i, new[i], past[i]))
@@ -281,6 +281,16 @@ def prompt(dev, past, new, heads, kv, dim, page, dtype, window=0, wide=0, behind
     ([700], [260], 2, 2, 72, 7, 129), ([5], [300], 16, 1, 128, 128, 0)])
 def test_several_rows_per_sequence(dev, dtype, past, new, heads, kv, dim, page, window):
     prompt(dev, past, new, heads, kv, dim, page, dtype, window, wide=8 if len(new) > 1 else 0, behind=len(new) % 3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("past,new,heads,kv,dim,page,window,scale", [
+    ([0], [257], 1, 1, 128, 8, 0, -0.05), ([129, 0], [128, 300], 2, 2, 64, 5, 0, 0.3), ([1000], [140], 2, 1, 96, 64, 300, None), ([50, 60, 70], [200, 1, 129], 4, 4, 40, 32, 1, None),
+    ([383], [385], 1, 1, 16, 16, 0, None), ([0, 100], [120, 140], 6, 2, 120, 48, 90, 0.02)])
+def test_whole_tiles_of_rows(dev, dtype, past, new, heads, kv, dim, page, window, scale):
+    """Tiles of 128 rows and positions: borders on and beside them, pages that boxes of rows divide and ones that they do not, windows smaller
+    than a tile, turned scores."""
+    prompt(dev, past, new, heads, kv, dim, page, dtype, window, scale=scale, behind=1)
 
 
 def test_many_short_prompts_and_a_long_one(dev):

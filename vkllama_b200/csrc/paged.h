@@ -40,7 +40,7 @@ __device__ __forceinline__ void follow() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
 }
-template <class K, class P> cudaError_t launch_following(K kernel, dim3 grid, uint32_t threads, size_t smem, cudaStream_t s, const P &p) {
+template <class K, class... P> cudaError_t launch_following(K kernel, dim3 grid, uint32_t threads, size_t smem, cudaStream_t s, const P &...p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -51,7 +51,7 @@ template <class K, class P> cudaError_t launch_following(K kernel, dim3 grid, ui
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p...);
 }
 
 // When a launch began and when its last CTA ended, for Op::time(): two events around every launch would cost 5 us of device time.

@@ -6,9 +6,8 @@
 // for one, the exponentials of the other are computed, which take as long (16 per clock and SM: 1024 cycles for 128 x 128, like the two
 // products). Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
-//             that it grew by more than 2^8: until then the probabilities stay below 2^8 and O as it is; only then O is multiplied. Reads S
-//             twice (maximum, exponentials) instead of keeping 128 values.
-//   8, 9      fetch Q, then K_j and V_j by cp.async into rings of two stages, in the 128-byte swizzle of the matrix descriptors: K is K-major and
+//             that it grew by more than 2^8: until then the probabilities stay below 2^8 and O as it is; only then O is multiplied.
+//   8, 9      fetch Q, then K_j and V_j into rings of two stages, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte swizzle of the matrix descriptors: K is K-major and
 //             V, as it lies in the cache, MN-major (64 dimensions of a position are a row of 128 bytes in both).
 //   10        issues the MMAs. They complete in order, so the commit behind S_i(j + 1) also says that P_i(j) V_j is in O_i.
 // Every wait is bounded; after one that ran out all warps leave, and the error word is raised.
@@ -37,37 +36,85 @@ __device__ __forceinline__ void mma_tmem(uint32_t acc, uint32_t a_tmem, uint32_t
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(acc), "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
                "r"(r[14]), "r"(r[15])
                : "memory");
 }
+// A thread's 128 columns. The wait is part of the statement, so that nothing touches the registers before it.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,"
+      "%58,%59,%60,%61,%62,%63,%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,"
+      "%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,"
+      "%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
+      "}, [%128];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]),
+        "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]),
+        "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]),
+        "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
+        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]),
+        "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]),
+        "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]),
+        "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]),
+        "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ float2 of_pair(uint64_t v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_wait_short(uint32_t bar, uint32_t parity) {
+  uint32_t ok = 0;
+  for (uint32_t i = 0; !ok && i < 1u << 14; ++i)
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1) paged_prompt_tc_kernel(const PagedAttention p) {
+// Sixteen columns times c.
+__device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
+  uint32_t u[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]),
+                 "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+               : "r"(taddr)
+               : "memory");
+#pragma unroll
+  for (int x = 0; x < 16; ++x) u[x] = __float_as_uint(__uint_as_float(u[x]) * c);
+  tmem_st16(taddr, u);
+}
+
+template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
+    paged_prompt_tc_kernel(const PagedAttention p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t box) {
   using C = Cfg<DP>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], o_full[2];
-  __shared__ uint32_t tmem_s, row_s[kFetchWarps][2][kKeys];
+  __shared__ uint32_t tmem_s;
   __shared__ volatile uint32_t failed_s;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, per = p.heads / p.kv_heads;
   follow();
@@ -122,74 +169,64 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1) paged_
       const uint32_t pos = past + min(r, packed - 1) / per, w_lo = past + w0 / per, w_hi = past + w1 / per;
       const uint32_t w_first = p.window && w_hi + 1 > p.window ? w_hi + 1 - p.window : 0;  // every row of the warp sees [w_first, w_lo]
       const uint32_t first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
-      const float scale = p.scale * kLog2e;
+      const float scale = fabsf(p.scale) * kLog2e;  // a negative scale is the MMA's negated operand
       const uint32_t lanes = (quad * 32u) << 16, s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * DP;
-      float top = -INFINITY, ref = 0.f, sum = 0.f;  // of scaled scores: reference, and what is subtracted (0 where the reference is -infinity)
+      float top = -INFINITY, ref = 0.f, sum = 0.f;  // the reference, and what is subtracted from scaled scores (0 where it is -infinity)
       bool ok = true;
       uint32_t phase = 0;
       const uint32_t bi = b[i], ei = e[i];
       for (uint32_t t = bi; t < ei; ++t, phase ^= 1) {
         if (!(ok = wait_warp(&s_full[i], phase))) break;
         tc_after();
-        const bool whole = t * kKeys >= w_first && t * kKeys + kKeys - 1 <= w_lo;
-        auto take = [&](uint32_t c, float (&v)[32]) {
-          uint32_t u[32];
-          tmem_ld32(s_t + c * 32, u);
+        uint32_t u[128];
+        tmem_ld128(s_t, u);
+        if (t * kKeys < w_first || t * kKeys + kKeys - 1 > w_lo) {  // some row does not see all of it
+          const uint32_t lo = first > t * kKeys ? first - t * kKeys : 0, hi = pos >= t * kKeys ? pos - t * kKeys : 0;
+          const bool none = pos < t * kKeys;
 #pragma unroll
-          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(u[x]) * scale;
-          if (!whole) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              const uint32_t j = t * kKeys + c * 32 + x;
-              if (j > pos || j < first) v[x] = -INFINITY;
-            }
-          }
-        };
-        float m = -INFINITY;
-#pragma unroll
-        for (uint32_t c = 0; c < 4; ++c) {
-          float v[32];
-          take(c, v);
-#pragma unroll
-          for (int x = 0; x < 32; ++x) m = fmaxf(m, v[x]);
+          for (uint32_t x = 0; x < 128; ++x)
+            if (x < lo || x > hi || none) u[x] = 0xff800000u;
         }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (uint32_t x = 0; x < 128; x += 8)
+#pragma unroll
+          for (uint32_t y = 0; y < 4; ++y) m4[y] = fmaxf(fmaxf(m4[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + 4 + y]));
+        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if (t == bi) {
           top = m;
-          ref = m == -INFINITY ? 0.f : m;
+          ref = m == -INFINITY ? 0.f : m * scale;
         } else {
-          const bool grown = m - ref > 8.0f || (top == -INFINITY && m != -INFINITY);
+          const bool grown = m * scale - ref > 8.0f || (top == -INFINITY && m != -INFINITY);
           if (__any_sync(0xffffffffu, grown)) {
             float c = 1.0f;
             if (grown) {
-              c = exp2_fast(top - m);
-              top = ref = m;
+              c = exp2_fast((top - m) * scale);
+              top = m;
+              ref = m * scale;
             }
             sum *= c;
 #pragma unroll 1
-            for (uint32_t d = 0; d < DP; d += 32) {
-              uint32_t u[32];
-              tmem_ld32(o_t + d, u);
-#pragma unroll
-              for (int x = 0; x < 32; ++x) u[x] = __float_as_uint(__uint_as_float(u[x]) * c);
-              tmem_st32(o_t + d, u);
-            }
+            for (uint32_t d = 0; d < DP; d += 16) rescale16(o_t + d, c);
             tmem_stored();
           }
         }
+        const uint64_t scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
+        uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (uint32_t c = 0; c < 4; ++c) {
-          float v[32];
-          uint32_t u[16];
-          take(c, v);
+          uint32_t w[16];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            v[x] = exp2_fast(v[x] - ref);
-            sum += v[x];
+          for (uint32_t x = 0; x < 16; ++x) {
+            const float2 y = of_pair(fma_pair(pair_of(__uint_as_float(u[c * 32 + 2 * x]), __uint_as_float(u[c * 32 + 2 * x + 1])), scale2, ref2));
+            const float a = exp2_fast(y.x), z = exp2_fast(y.y);
+            sum2[x & 1] = add_pair(sum2[x & 1], pair_of(a, z));
+            w[x] = pack2<BF>(a, z);
           }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) u[x] = pack2<BF>(v[2 * x], v[2 * x + 1]);
-          tmem_st16(s_t + c * 16, u);
+          tmem_st16(s_t + c * 16, w);
         }
+        const float2 part = of_pair(add_pair(sum2[0], sum2[1]));
+        sum += part.x + part.y;
         tmem_stored();
         tc_before();
         __syncwarp();
@@ -224,38 +261,75 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1) paged_
     }
   } else if (warp < kSoftmaxWarps + kFetchWarps) {
     // --------------------------------------------------------------------------------------------------------- fetch
-    constexpr uint32_t CH = DP / 8, FT = kFetchWarps * 32, RS = FT / CH;  // pieces of a row; rows that the warps fetch at a time
-    const uint32_t ft = tid - kSoftmaxWarps * 32, col = ft % CH, frow = ft / CH;
+    constexpr uint32_t CH = DP / 8, FT = kFetchWarps * 32, RS = FT / CH, BLOCKS = DP / 64;  // pieces of a row; rows that the warps fetch at a time
+    const uint32_t fw = warp - kSoftmaxWarps, ft = tid - kSoftmaxWarps * 32, col = ft % CH, frow = ft / CH;
     const bool col_there = col * 8 < p.dim;
     auto place = [&](uint32_t row) { return (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4); };
-    auto landed = [&](uint64_t *bar) {  // this thread's oldest pieces are there: the tensor core may read them
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    const uint32_t j_first = p.window && past + at.first / per + 1 > p.window ? past + at.first / per + 1 - p.window : 0;
+    const uint32_t j_last = past + (min(at.first + 2 * kRows, packed) - 1) / per;
+    auto cache_row = [&](uint32_t j) {  // of position j; behind the last one where there is none
+      const uint32_t n = quotient(j, p.page), page = __ldg(p.table + (size_t)at.seq * p.width + n);
+      if (page < p.pages) return (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
+      raise(p.error, PAGED_BAD_PAGE);
+      return 0xffffffffu;
+    };
+    // What a warp has requested by cp.async is reported behind its next request.
+    uint64_t *late = nullptr;
+    auto landed = [&]() {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core may read them
       __syncwarp();
-      if (lane == 0) arrive(sa(bar));
+      if (lane == 0) arrive(sa(late));
+      late = nullptr;
     };
-    const uint32_t j_first = past + at.first / per + 1 > p.window && p.window ? past + at.first / per + 1 - p.window : 0, j_last = past + (min(at.first + 2 * kRows, packed) - 1) / per;
-    uint32_t(*rows)[kKeys] = row_s[warp - kSoftmaxWarps];  // each warp looks up for itself: the fetching warps never wait for each other
-    auto look_up = [&](uint32_t t) {  // cache rows of the tile's positions
-#pragma unroll
-      for (uint32_t x = lane; x < kKeys; x += 32) {
-        const uint32_t j = t * kKeys + x;
-        uint32_t r = 0xffffffffu;
-        if (j >= j_first && j <= j_last) {
-          const uint32_t n = quotient(j, p.page), page = __ldg(p.table + (size_t)at.seq * p.width + n);
-          if (page < p.pages) r = (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
-          else raise(p.error, PAGED_BAD_PAGE);
-        }
-        rows[t & 1][x] = r;
-      }
-    };
-    auto request = [&](const void *cache, uint32_t dst, uint32_t t) {
-#pragma unroll 8
-      for (uint32_t i = 0; i < kKeys / RS; ++i) {
-        const uint32_t row = i * RS + frow, r = rows[t & 1][row];
-        const bool there = r != 0xffffffffu && col_there;
-        copy16(dst + place(row), static_cast<const uint16_t *>(cache) + (there ? (size_t)r * p.dim + col * 8 : 0), there);
-      }
+    auto requested = [&](uint64_t *bar, bool pieces) {
       copy_commit();
+      if (late) {
+        copy_wait<1>();
+        landed();
+      }
+      if (pieces) {
+        late = bar;
+      } else {
+        __syncwarp();
+        if (lane == 0) arrive(sa(bar));
+      }
+    };
+    // Of a tile, the boxes of rows that lie in one page and exist whole are tensor copies, one lane each; what is left, and pages of which
+    // no eight rows make a box, goes piece by piece. Positions that no row of the CTA sees count as zeros.
+    const uint32_t boxes = box ? kKeys / box : 0, my_box = lane / BLOCKS, my_x = lane % BLOCKS * 64;
+    uint32_t my_row = 0, box_lo = 0, box_hi = 0, look_row = 0;
+    auto look_up = [&](uint32_t t) {  // this lane's box of a tile that will be requested
+      const uint32_t j = t * kKeys + my_box * box;
+      if (fw == 0 && my_box < boxes && j + box > j_first && j + box <= at.len) look_row = cache_row(j);
+    };
+    auto turn_to = [&](uint32_t t) {
+      my_row = look_row;
+      if (box) {
+        const uint32_t j = t * kKeys;
+        box_lo = j_first > j ? min((j_first - j) / box, boxes) : 0;
+        box_hi = at.len > j ? min((at.len - j) / box, boxes) : 0;
+        box_hi = max(box_hi, box_lo);
+      }
+    };
+    auto request = [&](const void *cache, const CUtensorMap *map, uint32_t dst, uint32_t t, uint64_t *bar) {
+      const uint32_t lo = box_lo * box, hi = box_hi * box;
+      if (fw == 0 && hi > lo) {
+        if (lane == 0) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"((hi - lo) * DP * 2) : "memory");
+        __syncwarp();
+        if (my_box >= box_lo && my_box < box_hi)  // a row behind the cache reads as zeros
+          tma_load_2d(dst + my_x / 64 * (128 * 128) + my_box * box * 128, map, my_x, min(my_row, p.pages * p.kv_heads * p.page.d), sa(bar));
+      }
+      if (hi - lo < kKeys) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < kKeys / RS; ++i) {
+          const uint32_t row = i * RS + frow, j = t * kKeys + row;
+          if (row >= lo && row < hi) continue;
+          const uint32_t r = j >= j_first && j <= j_last ? cache_row(j) : 0xffffffffu;
+          const bool there = r != 0xffffffffu && col_there;
+          copy16(dst + place(row), static_cast<const uint16_t *>(cache) + (there ? (size_t)r * p.dim + col * 8 : 0), there);
+        }
+      }
+      requested(bar, hi - lo < kKeys);
     };
     look_up(t0);
 #pragma unroll 4
@@ -266,36 +340,32 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1) paged_
       const uint16_t *src = static_cast<const uint16_t *>(p.q);
       copy16(q_a + (row >> 7) * C::kTile + place(row & 127), there ? src + (at.row0 + rt) * p.q_ld + (kvh * per + r - rt * per) * p.dim + col * 8 : src, there);
     }
-    copy_commit();
-    __syncwarp();
-    request(p.kcache, k_a, t0);
-    copy_wait<1>();
-    landed(&q_full);
-    // a tile's values are requested before its keys have landed, the next tile's keys before its values have
-    bool ok = true;
+    requested(&q_full, true);
+    turn_to(t0);
+    request(p.kcache, &map_k, k_a, t0, &k_full[0]);
+    uint32_t n = 0, keys = 1;  // tiles whose values, keys have been requested
     for (uint32_t t = t0; t < t1; ++t) {
-      const uint32_t n = t - t0, s = n % kStages, parity = (n / kStages + 1) & 1;  // of the stage's last release
-      if (n >= kStages && !(ok = wait_warp(&v_empty[s], parity))) break;
-      request(p.vcache, v_a + s * C::kTile, t);
-      copy_wait<1>();
-      landed(&k_full[s]);
-      if (t + 1 < t1) {
-        look_up(t + 1);  // its place was last read for tile t - 1
-        __syncwarp();
-        const uint32_t n1 = n + 1, s1 = n1 % kStages;
-        if (n1 >= kStages && !(ok = wait_warp(&k_empty[s1], (n1 / kStages + 1) & 1))) break;
-        request(p.kcache, k_a + s1 * C::kTile, t + 1);
-        copy_wait<1>();
-      } else {
-        copy_wait<0>();
-      }
-      landed(&v_full[s]);
+      if (n >= kStages && !wait_warp(&v_empty[n % kStages], (n / kStages + 1) & 1)) break;  // the stage's last release
+      if (t + 1 < t1) look_up(t + 1);
+      request(p.vcache, &map_v, v_a + n % kStages * C::kTile, t, &v_full[n % kStages]);
+      ++n;
+      if (t + 1 == t1) break;
+      if (keys >= kStages && !wait_warp(&k_empty[keys % kStages], (keys / kStages + 1) & 1)) break;
+      turn_to(t + 1);
+      request(p.kcache, &map_k, k_a + keys % kStages * C::kTile, t + 1, &k_full[keys % kStages]);
+      ++keys;
     }
     copy_wait<0>();
+    if (late) landed();
+    if (failed_s && fw == 0 && lane == 0) {  // nothing may land when the CTA has gone
+      for (uint32_t x = n > kStages ? n - kStages : 0; x < n; ++x) mbar_wait_short(sa(&v_full[x % kStages]), x / kStages & 1);
+      for (uint32_t x = keys > kStages ? keys - kStages : 0; x < keys; ++x) mbar_wait_short(sa(&k_full[x % kStages]), x / kStages & 1);
+    }
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------------------------------------------------------- MMA
     if (elect_one()) {
-      constexpr uint32_t idesc_s = instr_desc(kRows, kKeys, BF), idesc_o = instr_desc(kRows, DP, BF) | 1u << 16;  // the second: B is MN-major
+      const uint32_t idesc_s = instr_desc(kRows, kKeys, BF) | (p.scale < 0.f ? 1u << 13 : 0u);  // negates A
+      constexpr uint32_t idesc_o = instr_desc(kRows, DP, BF) | 1u << 16;  // the second: B is MN-major
       const uint32_t q0 = desc_lo(q_a), k0 = desc_lo(k_a);
       const uint32_t v0 = ((v_a & 0x3FFFFu) >> 4) | (128u * 128 >> 4) << 16;  // 64 dimensions are 16 KB from the next 64
       bool ok = wait(&q_full, 0);
@@ -353,7 +423,12 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1) paged_
 
 template <bool BF, int DP> cudaError_t run(const PagedAttention &p, cudaStream_t s) {
   const uint64_t per = p.heads / p.kv_heads, tiles = p.rows * per / (2 * kRows) + std::min<uint64_t>(p.n, p.rows * per);
-  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)tiles, p.kv_heads), kThreads, Cfg<DP>::kSmem, s, p);
+  const uint64_t cache_rows = (uint64_t)p.pages * p.kv_heads * p.page.d;
+  CUtensorMap map_k = {}, map_v = {};
+  uint32_t box = kKeys;  // the most rows, a power of two, of which pages consist; coordinates are signed
+  while (p.page.d % box) box /= 2;
+  if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) || !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF)) box = 0;
+  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)tiles, p.kv_heads), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
   return cudaFuncSetAttribute(paged_prompt_tc_kernel<BF, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);
