@@ -114,7 +114,7 @@ struct PagedAttention {
   uint32_t *error;
   uint64_t q_ld;
   uint32_t rows, n, heads, kv_heads, dim, width, pages, window;
-  Divisor page;
+  Divisor page, group;          // query heads of a key head
   float scale;                  // on the scores
   bool bf;
 };

@@ -267,7 +267,7 @@ struct PagedAttentionOp : PagedOp {
     if (!starts && rows != n) return fail(VKL_INVALID_ARGUMENT, "%s: %zu queries for %zu sequences of one new token each", who, rows, n);
     VKL_OKAY(check_apart(q, who, "queries"));
     // the one-token form counts tiles of 16 positions of all sequences and head groups in 31 bits
-    if (rows * per > kMaxTokens || n > kMaxTokens || (!starts && n * (table->w * page / 16 + 2) * (kv_heads * ((per + 7) / 8)) > kMaxTokens))
+    if (rows * per > kMaxTokens || n > kMaxTokens || (rows * per / 64 + n) * kv_heads > kMaxTokens || (!starts && n * (table->w * page / 16 + 2) * (kv_heads * ((per + 7) / 8)) > kMaxTokens))
       return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, %zu sequences of up to %zu tokens", who, rows, n, table->w * page);
     VKL_OKAY(begin(who));
     VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
@@ -286,6 +286,7 @@ struct PagedAttentionOp : PagedOp {
       p.rows = (uint32_t)rows, p.n = (uint32_t)n, p.heads = heads, p.kv_heads = kv_heads, p.dim = dim;
       p.width = (uint32_t)table->w, p.pages = (uint32_t)kcache->c, p.window = window;
       p.page = divisor(page);
+      p.group = divisor((uint32_t)per);
       p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
       p.bf = dtype == VKL_BF16;
       VKL_LAUNCH(1, starts ? launch_paged_prompt(p, cmd->stream) : launch_paged_token(p, dev->prop.multiProcessorCount, cmd->stream));

@@ -33,12 +33,22 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
   constexpr int KS = DP / 16, NT = DP / 8, SN = KT / 8;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t row_s[2][KT];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, kvh = blockIdx.y;
-  const uint32_t per = p.heads / p.kv_heads;
-  Place at;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const uint32_t per = p.heads / p.kv_heads, tile = blockIdx.x / p.kv_heads, kvh = blockIdx.x - tile * p.kv_heads;
+  __shared__ Place at_s;
+  __shared__ bool found_s;
   follow();
   stamp_begin(p.stamps);
-  if (!find_tile<kThreads>(p, per, kRows, blockIdx.x, at)) return;
+  if (warp == 0) {
+    Place found = {};
+    const bool there = find_tile(p, per, kRows, tile, found);
+    if (lane == 0) at_s = found, found_s = there;
+  } else if (warp == 1 && blockIdx.x == 0) {
+    check_rows(p);
+  }
+  __syncthreads();
+  if (!found_s) return;
+  const Place at = at_s;
   const uint32_t packed = at.fresh * per, r_end = min(at.first + kRows, packed), past = at.len - at.fresh;
   // positions that the tile's rows see
   const uint32_t lo_pos = past + at.first / per, hi_pos = past + (r_end - 1) / per;
@@ -199,7 +209,7 @@ template <bool BF, int DP> cudaError_t setup_one() {
 template <bool BF> cudaError_t pick(const PagedAttention &p, cudaStream_t s) {
   // tiles are counted on the device; every sequence has at most one that is not full
   const uint64_t per = p.heads / p.kv_heads, tiles = p.rows * per / kRows + std::min<uint64_t>(p.n, p.rows * per);
-  const dim3 grid((uint32_t)tiles, p.kv_heads);
+  const dim3 grid((uint32_t)(tiles * p.kv_heads));  // all heads of a tile, then the next tile
   if (p.dim <= 64) return launch_following(paged_prompt_kernel<BF, 64>, grid, kThreads, Cfg<64>::kSmem, s, p);
   if (p.dim <= 128) return launch_following(paged_prompt_kernel<BF, 128>, grid, kThreads, Cfg<128>::kSmem, s, p);
   return launch_following(paged_prompt_kernel<BF, 256>, grid, kThreads, Cfg<256>::kSmem, s, p);

@@ -7,7 +7,7 @@
 // products). Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
 //             that it grew by more than 2^8: until then the probabilities stay below 2^8 and O as it is; only then O is multiplied.
-//   8, 9      fetch Q, then K_j and V_j into rings of two stages, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte swizzle of the matrix descriptors: K is K-major and
+//   8, 9      fetch K_j and V_j into a ring, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte swizzle of the matrix descriptors: K is K-major and
 //             V, as it lies in the cache, MN-major (64 dimensions of a position are a row of 128 bytes in both).
 //   10        issues the MMAs. They complete in order, so the commit behind S_i(j + 1) also says that P_i(j) V_j is in O_i.
 // Every wait is bounded; after one that ran out all warps leave, and the error word is raised.
@@ -20,13 +20,16 @@ namespace vkl {
 namespace {
 
 constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // the twelfth idles: more than 12 warps would have 128 registers each
-constexpr uint32_t kRows = 128, kKeys = 128, kStages = 2;
+constexpr uint32_t kRows = 128, kKeys = 128;
 constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20;
 
 template <int DP> struct Cfg {
   static constexpr uint32_t kTile = 128 * DP * 2;  // bytes of 128 rows
-  // One CTA per SM, which takes all of its TMEM: more than half of the shared memory, whatever the head width.
-  static constexpr uint32_t kSmem = std::max((2 + 2 * kStages) * kTile, 120u * 1024) + 1024;
+  // One CTA per SM, which takes all of its TMEM: more than half of the shared memory, whatever the head width. K and V tiles take
+  // turns in one ring: with two places each (373 -> 238 us) the MMAs still waited 1000 of 4000 cycles a tile for keys.
+  static constexpr uint32_t kStages = DP == 64 ? 8 : 5;
+  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;
+  static_assert(kSmem > 114 * 1024 && kSmem + 1024 <= 227 * 1024, "one CTA per SM");
 };
 
 __device__ __forceinline__ void mma_tmem(uint32_t acc, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
@@ -113,14 +116,38 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<DP>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], o_full[2];
+  __shared__ __align__(8) uint64_t q_full[2], full[C::kStages], empty[C::kStages], s_full[2], p_full[2][2], o_full[2];
   __shared__ uint32_t tmem_s;
   __shared__ volatile uint32_t failed_s;
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, per = p.heads / p.kv_heads;
+  __shared__ Place at_s;
+  __shared__ bool found_s;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = p.heads / p.kv_heads, tile = blockIdx.x / p.kv_heads, kvh = blockIdx.x - tile * p.kv_heads;
+  if (tid == 0) {
+    auto init = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"(n) : "memory"); };
+    for (uint32_t s = 0; s < C::kStages; ++s) init(&full[s], kFetchWarps), init(&empty[s], 1);
+    for (uint32_t i = 0; i < 2; ++i) init(&q_full[i], 4), init(&s_full[i], 1), init(&p_full[i][0], 4), init(&p_full[i][1], 4), init(&o_full[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    failed_s = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc<512>(sa(&tmem_s));
   follow();
   stamp_begin(p.stamps);
-  Place at;
-  if (!find_tile<kThreads>(p, per, 2 * kRows, blockIdx.x, at)) return;
+  if (warp == kMmaWarp + 1) {
+    Place found = {};
+    const bool there = find_tile(p, per, 2 * kRows, tile, found);
+    if (lane == 0) at_s = found, found_s = there;
+  } else if (warp == 0 && blockIdx.x == 0) {
+    check_rows(p);
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_s;
+  if (!found_s) {
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    return;
+  }
+  const Place &at = at_s;
   const uint32_t packed = at.fresh * per, past = at.len - at.fresh;
   // per tile of rows: its rows that exist, and the tiles of positions [b, e) that they see
   const bool both = at.first + kRows < packed;
@@ -132,19 +159,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     e[i] = hi / kKeys + 1;
   }
   const uint32_t t0 = b[0], t1 = e[1], tiles = both ? 2 : 1;  // b and e grow with the rows
-  if (tid == 0) {
-    auto init = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"(n) : "memory"); };
-    init(&q_full, kFetchWarps);
-    for (uint32_t s = 0; s < kStages; ++s) init(&k_full[s], kFetchWarps), init(&v_full[s], kFetchWarps), init(&k_empty[s], 1), init(&v_empty[s], 1);
-    for (uint32_t i = 0; i < 2; ++i) init(&s_full[i], 1), init(&p_full[i], 4), init(&o_full[i], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    failed_s = 0;
-  }
-  if (warp == kMmaWarp) tmem_alloc<512>(sa(&tmem_s));
-  tc_before();
-  __syncthreads();
-  tc_after();
-  const uint32_t tmem = tmem_s, q_a = sa(smem), k_a = q_a + 2 * C::kTile, v_a = k_a + kStages * C::kTile;
+  const uint32_t q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
   // False when the wait ran out, or anyone's did.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     const uint32_t a = sa(bar);
@@ -169,6 +184,25 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t pos = past + min(r, packed - 1) / per, w_lo = past + w0 / per, w_hi = past + w1 / per;
       const uint32_t w_first = p.window && w_hi + 1 > p.window ? w_hi + 1 - p.window : 0;  // every row of the warp sees [w_first, w_lo]
       const uint32_t first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
+      // the warp's 32 rows of Q, in the swizzle of the operand
+      {
+        constexpr uint32_t CH = DP / 8, RS = 32 / CH;  // pieces of a row; rows at a time
+        const uint32_t col = lane % CH;
+        const uint16_t *src = static_cast<const uint16_t *>(p.q);
+#pragma unroll 8
+        for (uint32_t x = 0; x < 32 / RS; ++x) {
+          const uint32_t row = quad * 32 + x * RS + lane / CH, qr = at.first + i * kRows + row;
+          const bool there = qr < packed && col * 8 < p.dim;
+          const uint32_t rt = quotient(qr, p.group);
+          copy16(q_a + i * C::kTile + (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4),
+                 there ? src + (at.row0 + rt) * p.q_ld + (kvh * per + qr - rt * per) * p.dim + col * 8 : src, there);
+        }
+        copy_commit();
+        copy_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(sa(&q_full[i]));
+      }
       const float scale = fabsf(p.scale) * kLog2e;  // a negative scale is the MMA's negated operand
       const uint32_t lanes = (quad * 32u) << 16, s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * DP;
       float top = -INFINITY, ref = 0.f, sum = 0.f;  // the reference, and what is subtracted from scaled scores (0 where it is -infinity)
@@ -224,13 +258,19 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
             w[x] = pack2<BF>(a, z);
           }
           tmem_st16(s_t + c * 16, w);
+          if (c == 1) {  // the product with the first 64 positions' values can begin
+            tmem_stored();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) arrive(sa(&p_full[i][0]));
+          }
         }
         const float2 part = of_pair(add_pair(sum2[0], sum2[1]));
         sum += part.x + part.y;
         tmem_stored();
         tc_before();
         __syncwarp();
-        if (lane == 0) arrive(sa(&p_full[i]));
+        if (lane == 0) arrive(sa(&p_full[i][1]));
       }
       if (ok && wait_warp(&o_full[i], 0)) {
         tc_after();
@@ -332,83 +372,80 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       requested(bar, hi - lo < kKeys);
     };
     look_up(t0);
-#pragma unroll 4
-    for (uint32_t i = 0; i < tiles * kRows / RS; ++i) {
-      const uint32_t row = i * RS + frow, r = at.first + row;
-      const bool there = r < packed && col_there;
-      const uint32_t rt = r / per;
-      const uint16_t *src = static_cast<const uint16_t *>(p.q);
-      copy16(q_a + (row >> 7) * C::kTile + place(row & 127), there ? src + (at.row0 + rt) * p.q_ld + (kvh * per + r - rt * per) * p.dim + col * 8 : src, there);
-    }
-    requested(&q_full, true);
-    turn_to(t0);
-    request(p.kcache, &map_k, k_a, t0, &k_full[0]);
-    uint32_t n = 0, keys = 1;  // tiles whose values, keys have been requested
+    uint32_t n = 0, stage = 0, phase = 1;  // requests: keys, values, keys, ...; place and the parity of its last release
     for (uint32_t t = t0; t < t1; ++t) {
-      if (n >= kStages && !wait_warp(&v_empty[n % kStages], (n / kStages + 1) & 1)) break;  // the stage's last release
-      if (t + 1 < t1) look_up(t + 1);
-      request(p.vcache, &map_v, v_a + n % kStages * C::kTile, t, &v_full[n % kStages]);
-      ++n;
-      if (t + 1 == t1) break;
-      if (keys >= kStages && !wait_warp(&k_empty[keys % kStages], (keys / kStages + 1) & 1)) break;
-      turn_to(t + 1);
-      request(p.kcache, &map_k, k_a + keys % kStages * C::kTile, t + 1, &k_full[keys % kStages]);
-      ++keys;
+      turn_to(t);
+      bool ok = true;
+#pragma unroll 1
+      for (uint32_t values = 0; values < 2; ++values) {
+        if (n >= C::kStages && !(ok = wait_warp(&empty[stage], phase))) break;
+        if (!values && t + 1 < t1) look_up(t + 1);
+        request(values ? p.vcache : p.kcache, values ? &map_v : &map_k, ring_a + stage * C::kTile, t, &full[stage]);
+        ++n;
+        if (++stage == C::kStages) stage = 0, phase ^= 1;
+      }
+      if (!ok) break;
     }
     copy_wait<0>();
     if (late) landed();
     if (failed_s && fw == 0 && lane == 0) {  // nothing may land when the CTA has gone
-      for (uint32_t x = n > kStages ? n - kStages : 0; x < n; ++x) mbar_wait_short(sa(&v_full[x % kStages]), x / kStages & 1);
-      for (uint32_t x = keys > kStages ? keys - kStages : 0; x < keys; ++x) mbar_wait_short(sa(&k_full[x % kStages]), x / kStages & 1);
+      for (uint32_t x = n > C::kStages ? n - C::kStages : 0; x < n; ++x) mbar_wait_short(sa(&full[x % C::kStages]), x / C::kStages & 1);
     }
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------------------------------------------------------- MMA
     if (elect_one()) {
       const uint32_t idesc_s = instr_desc(kRows, kKeys, BF) | (p.scale < 0.f ? 1u << 13 : 0u);  // negates A
       constexpr uint32_t idesc_o = instr_desc(kRows, DP, BF) | 1u << 16;  // the second: B is MN-major
-      const uint32_t q0 = desc_lo(q_a), k0 = desc_lo(k_a);
-      const uint32_t v0 = ((v_a & 0x3FFFFu) >> 4) | (128u * 128 >> 4) << 16;  // 64 dimensions are 16 KB from the next 64
-      bool ok = wait(&q_full, 0);
-      uint32_t p_phase = 0;  // bit i
-      // Before tile t's turn: S of t for the tiles of rows that see it.
-      auto scores = [&](uint32_t i, uint32_t t) {
-        const uint32_t st = ((t - t0) % kStages) * (C::kTile >> 4), qi = q0 + i * (C::kTile >> 4);
-#pragma unroll
-        for (uint32_t k = 0; k < DP / 16; ++k) {
-          const uint32_t off = (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2;
-          mma_f16<1>(tmem + i * 128, qi + off, k0 + st + off, idesc_s, k != 0);
-        }
-        mma_commit(sa(&s_full[i]));
-      };
-      // t0 - 1 stands for what comes before the first tile
+      const uint32_t q0 = desc_lo(q_a), k0 = desc_lo(ring_a);
+      const uint32_t v0 = ((ring_a & 0x3FFFFu) >> 4) | (128u * 128 >> 4) << 16;  // 64 dimensions are 16 KB from the next 64
+      bool ok = true;
+      uint32_t p_phase = 0;               // bit i
+      RingPos<(int)C::kStages> keys, vals;  // tile t's keys are request 2 t, its values 2 t + 1
+      vals.next();
+      // step n: output of tile t - 1, scores of tile t, for one tile of rows after the other
       for (uint32_t n = 0; ok && n <= t1 - t0; ++n) {
-        const uint32_t t = t0 + n;  // scores of t, output of t - 1
-        bool keys = false;
-        if (n > 0 && !(ok = wait(&v_full[(n - 1) % kStages], ((n - 1) / kStages) & 1))) break;
+        const uint32_t t = t0 + n;
+        bool waited = false;
+        if (n > 0 && !(ok = wait(&full[vals.s], vals.phase))) break;
         for (uint32_t i = 0; ok && i < tiles; ++i) {
           if (n > 0 && t - 1 >= b[i] && t - 1 < e[i]) {
-            if (!(ok = wait(&p_full[i], p_phase >> i & 1))) break;
+            const uint32_t st = v0 + vals.s * (C::kTile >> 4), parity = p_phase >> i & 1;
             p_phase ^= 1u << i;
-            tc_after();
-            const uint32_t st = v0 + ((n - 1) % kStages) * (C::kTile >> 4);
 #pragma unroll
-            for (uint32_t k = 0; k < kKeys / 16; ++k)
-              mma_tmem(tmem + 256 + i * DP, tmem + i * 128 + k * 8, st + k * (2048 >> 4), idesc_o, k != 0 || t - 1 > b[i]);
+            for (uint32_t half = 0; half < 2; ++half) {
+              if (!(ok = wait(&p_full[i][half], parity))) break;
+              tc_after();
+#pragma unroll
+              for (uint32_t k = half * 4; k < half * 4 + 4; ++k)
+                mma_tmem(tmem + 256 + i * DP, tmem + i * 128 + k * 8, st + k * (2048 >> 4), idesc_o, k != 0 || t - 1 > b[i]);
+            }
+            if (!ok) break;
             if (t == e[i]) mma_commit(sa(&o_full[i]));
           }
+          if (n > 0 && i + 1 == tiles) mma_commit(sa(&empty[vals.s]));
           if (t < t1 && t >= b[i] && t < e[i]) {
-            if (!keys && !(ok = wait(&k_full[n % kStages], (n / kStages) & 1))) break;
-            keys = true;
+            if (n == 0 || t == b[i]) {
+              if (!(ok = wait(&q_full[i], 0))) break;
+            }
+            if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;
+            waited = true;
             tc_after();
-            scores(i, t);
+            const uint32_t st = k0 + keys.s * (C::kTile >> 4), qi = q0 + i * (C::kTile >> 4);
+#pragma unroll
+            for (uint32_t k = 0; k < DP / 16; ++k) {
+              const uint32_t off = (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2;
+              mma_f16<1>(tmem + i * 128, qi + off, st + off, idesc_s, k != 0);
+            }
+            mma_commit(sa(&s_full[i]));
           }
         }
         if (!ok) break;
-        if (n > 0) mma_commit(sa(&v_empty[(n - 1) % kStages]));
         if (t < t1) {
-          if (!keys && !(ok = wait(&k_full[n % kStages], (n / kStages) & 1))) break;  // nobody sees it (between windows): still given back
-          mma_commit(sa(&k_empty[n % kStages]));
+          if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;  // nobody sees it (between windows): still given back
+          mma_commit(sa(&empty[keys.s]));
+          keys.next(), keys.next();
         }
+        if (n > 0) vals.next(), vals.next();
       }
     }
     __syncwarp();
@@ -428,7 +465,7 @@ template <bool BF, int DP> cudaError_t run(const PagedAttention &p, cudaStream_t
   uint32_t box = kKeys;  // the most rows, a power of two, of which pages consist; coordinates are signed
   while (p.page.d % box) box /= 2;
   if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) || !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF)) box = 0;
-  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)tiles, p.kv_heads), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, box);
+  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)(tiles * p.kv_heads)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
   return cudaFuncSetAttribute(paged_prompt_tc_kernel<BF, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);

@@ -23,48 +23,40 @@ __device__ __forceinline__ uint32_t fresh_rows(const PagedAttention &p, uint32_t
   return 0;
 }
 
-// The place of tile `tile` when every sequence has ceil(new * per / rows) of them; false beyond the last.
-template <uint32_t THREADS> __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint64_t back, Place &at) {
-  __shared__ uint64_t before_s[THREADS + 1], sums_s[THREADS / 32];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t each = (p.n + THREADS - 1) / THREADS, i0 = min(tid * each, p.n), i1 = min(i0 + each, p.n);
+// The place of tile `index` when every sequence has ceil(new * per / rows) of them, by one warp; false beyond the last. A sequence's last tiles
+// see most and come first.
+__device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint32_t index, Place &at) {
+  const uint32_t lane = threadIdx.x & 31;
   bool bad = false;
-  uint64_t mine = 0;
-  auto tiles = [&](uint32_t i) { return ((uint64_t)fresh_rows(p, i, bad) * per + rows - 1) / rows; };
-  for (uint32_t i = i0; i < i1; ++i) mine += tiles(i);
-  if (bad && blockIdx.x == 0 && blockIdx.y == 0) raise(p.error, PAGED_BAD_ROWS);
-  uint64_t up = mine;
+  uint64_t before = 0;
+  for (uint32_t i0 = 0; i0 < p.n; i0 += 32) {
+    const uint32_t i = i0 + lane, fresh = i < p.n ? fresh_rows(p, i, bad) : 0;
+    const uint64_t mine = ((uint64_t)fresh * per + rows - 1) / rows;
+    uint64_t up = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t a = __shfl_up_sync(0xffffffffu, up, o);
-    if (lane >= o) up += a;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t a = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += a;
+    }
+    const uint32_t behind = __ballot_sync(0xffffffffu, before + up > index);
+    if (behind) {
+      const uint32_t x = __ffs(behind) - 1;
+      at.seq = i0 + x;
+      at.fresh = __shfl_sync(0xffffffffu, fresh, x);
+      at.first = ((uint32_t)(__shfl_sync(0xffffffffu, before + up, x) - index) - 1) * rows;
+      at.row0 = p.starts[at.seq];
+      at.len = p.lengths[at.seq];
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, up, 31);
   }
-  if (lane == 31) sums_s[warp] = up;
-  __syncthreads();
-  uint64_t base = 0;
-  for (uint32_t w = 0; w < warp; ++w) base += sums_s[w];
-  before_s[tid] = base + up - mine;
-  if (tid == THREADS - 1) before_s[THREADS] = base + up;
-  __syncthreads();
-  if (back >= before_s[THREADS]) return false;
-  const uint64_t tile = before_s[THREADS] - 1 - back;  // the last tiles of a sequence see most: they start first
-  uint32_t lo = 0, hi = THREADS;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (before_s[mid] <= tile) lo = mid;
-    else hi = mid;
-  }
-  uint64_t left = tile - before_s[lo];
-  at.seq = lo * each;
-  for (uint64_t n = tiles(at.seq); left >= n; n = tiles(at.seq)) {
-    left -= n;
-    ++at.seq;
-  }
-  at.fresh = fresh_rows(p, at.seq, bad);
-  at.row0 = p.starts[at.seq];
-  at.len = p.lengths[at.seq];
-  at.first = (uint32_t)left * rows;
-  return true;
+  return false;
+}
+// Starts and lengths that do not belong together are reported by the first CTA's first warp.
+__device__ __forceinline__ void check_rows(const PagedAttention &p) {
+  bool bad = false;
+  for (uint32_t i = threadIdx.x & 31; i < p.n; i += 32) fresh_rows(p, i, bad);
+  if (bad) raise(p.error, PAGED_BAD_ROWS);
 }
 
 // One packed row by a warp, from the definition in fp32. In the tiles' second product a position that a row does not see has the
