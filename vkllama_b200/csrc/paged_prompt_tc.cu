@@ -124,7 +124,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = p.heads / p.kv_heads, tile = blockIdx.x / p.kv_heads, kvh = blockIdx.x - tile * p.kv_heads;
   if (tid == 0) {
     auto init = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"(n) : "memory"); };
-    for (uint32_t s = 0; s < C::kStages; ++s) init(&full[s], kFetchWarps), init(&empty[s], 1);
+    for (uint32_t s = 0; s < C::kStages; ++s) init(&full[s], 1), init(&empty[s], 1);
     for (uint32_t i = 0; i < 2; ++i) init(&q_full[i], 4), init(&s_full[i], 1), init(&p_full[i][0], 4), init(&p_full[i][1], 4), init(&o_full[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed_s = 0;
@@ -300,96 +300,84 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < kSoftmaxWarps + kFetchWarps) {
-    // --------------------------------------------------------------------------------------------------------- fetch
-    constexpr uint32_t CH = DP / 8, FT = kFetchWarps * 32, RS = FT / CH, BLOCKS = DP / 64;  // pieces of a row; rows that the warps fetch at a time
-    const uint32_t fw = warp - kSoftmaxWarps, ft = tid - kSoftmaxWarps * 32, col = ft % CH, frow = ft / CH;
+    // ------------------------------------------------------------------------------------- fetch: keys one warp, values the other
+    constexpr uint32_t CH = DP / 8, RS = 32 / CH, BLOCKS = DP / 64;  // pieces of a row; rows at a time
+    const uint32_t values = warp - kSoftmaxWarps, col = lane % CH, frow = lane / CH;
     const bool col_there = col * 8 < p.dim;
-    auto place = [&](uint32_t row) { return (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4); };
+    const uint16_t *cache = static_cast<const uint16_t *>(values ? p.vcache : p.kcache);
+    const CUtensorMap *map = values ? &map_v : &map_k;
     const uint32_t j_first = p.window && past + at.first / per + 1 > p.window ? past + at.first / per + 1 - p.window : 0;
-    const uint32_t j_last = past + (min(at.first + 2 * kRows, packed) - 1) / per;
+    const uint32_t j_last = past + (min(at.first + 2 * kRows, packed) - 1) / per, len = at.len;
+    const uint32_t *pages = p.table + (size_t)at.seq * p.width;
     auto cache_row = [&](uint32_t j) {  // of position j; behind the last one where there is none
-      const uint32_t n = quotient(j, p.page), page = __ldg(p.table + (size_t)at.seq * p.width + n);
+      const uint32_t n = quotient(j, p.page), page = __ldg(pages + n);
       if (page < p.pages) return (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
       raise(p.error, PAGED_BAD_PAGE);
       return 0xffffffffu;
     };
-    // What a warp has requested by cp.async is reported behind its next request.
-    uint64_t *late = nullptr;
+    // Of a tile, the boxes of rows that lie in one page and exist whole are tensor copies; what is left, and pages of which no eight rows
+    // make a box, goes piece by piece. Positions that no row of the CTA sees count as zeros.
+    const uint32_t boxes = box ? kKeys / box : 0, rows_all = p.pages * p.kv_heads * p.page.d;
+    uint32_t look_row = 0;
+    auto look_up = [&](uint32_t t) {  // lane x: box x of a tile
+      const uint32_t j = t * kKeys + lane * box;
+      if (lane < boxes && j + box > j_first && j + box <= len) look_row = cache_row(j);
+    };
+    uint64_t *late = nullptr;  // pieces by cp.async are reported behind the next request
     auto landed = [&]() {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core may read them
       __syncwarp();
       if (lane == 0) arrive(sa(late));
       late = nullptr;
     };
-    auto requested = [&](uint64_t *bar, bool pieces) {
+    look_up(t0);
+    RingPos<(int)C::kStages> pos;  // tile t's keys are request 2 (t - t0), its values the one behind
+    if (values) pos.next();
+    uint32_t x = values;
+    for (uint32_t t = t0; t < t1; ++t, x += 2, pos.next(), pos.next()) {
+      const uint32_t my_row = min(look_row, rows_all), j0 = t * kKeys;  // a row behind the cache reads as zeros
+      const uint32_t lo = box && j_first > j0 ? min((j_first - j0) / box, boxes) : 0, hi = max(box && len > j0 ? min((len - j0) / box, boxes) : 0, lo);
+      if (x >= C::kStages && !wait_warp(&empty[pos.s], pos.phase ^ 1)) break;
+      const uint32_t dst = ring_a + pos.s * C::kTile, bar = sa(&full[pos.s]);
+      const bool pieces = (hi - lo) * box < kKeys;
+      if (hi > lo) {
+        if (elect_one()) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((hi - lo) * box * DP * 2) : "memory");
+        for (uint32_t g = lo; g < hi; ++g) {
+          const uint32_t row = __shfl_sync(0xffffffffu, my_row, g);
+          if (elect_one()) {  // one lane, known to the compiler: copies from several lanes at once became a loop, 2000 cycles a tile
+#pragma unroll
+            for (uint32_t k = 0; k < BLOCKS; ++k) tma_load_2d(dst + k * (128 * 128) + g * box * 128, map, k * 64, row, bar);
+          }
+        }
+      }
+      if (pieces) {
+#pragma unroll 4
+        for (uint32_t i = 0; i < kKeys / RS; ++i) {
+          const uint32_t row = i * RS + frow, j = j0 + row;
+          if (row >= lo * box && row < hi * box) continue;
+          const uint32_t r = j >= j_first && j <= j_last ? cache_row(j) : 0xffffffffu;
+          const bool there = r != 0xffffffffu && col_there;
+          copy16(dst + (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), cache + (there ? (size_t)r * p.dim + col * 8 : 0), there);
+        }
+      }
       copy_commit();
       if (late) {
         copy_wait<1>();
         landed();
       }
       if (pieces) {
-        late = bar;
+        late = &full[pos.s];
       } else {
         __syncwarp();
-        if (lane == 0) arrive(sa(bar));
+        if (lane == 0) arrive(bar);
       }
-    };
-    // Of a tile, the boxes of rows that lie in one page and exist whole are tensor copies, one lane each; what is left, and pages of which
-    // no eight rows make a box, goes piece by piece. Positions that no row of the CTA sees count as zeros.
-    const uint32_t boxes = box ? kKeys / box : 0, my_box = lane / BLOCKS, my_x = lane % BLOCKS * 64;
-    uint32_t my_row = 0, box_lo = 0, box_hi = 0, look_row = 0;
-    auto look_up = [&](uint32_t t) {  // this lane's box of a tile that will be requested
-      const uint32_t j = t * kKeys + my_box * box;
-      if (fw == 0 && my_box < boxes && j + box > j_first && j + box <= at.len) look_row = cache_row(j);
-    };
-    auto turn_to = [&](uint32_t t) {
-      my_row = look_row;
-      if (box) {
-        const uint32_t j = t * kKeys;
-        box_lo = j_first > j ? min((j_first - j) / box, boxes) : 0;
-        box_hi = at.len > j ? min((at.len - j) / box, boxes) : 0;
-        box_hi = max(box_hi, box_lo);
-      }
-    };
-    auto request = [&](const void *cache, const CUtensorMap *map, uint32_t dst, uint32_t t, uint64_t *bar) {
-      const uint32_t lo = box_lo * box, hi = box_hi * box;
-      if (fw == 0 && hi > lo) {
-        if (lane == 0) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"((hi - lo) * DP * 2) : "memory");
-        __syncwarp();
-        if (my_box >= box_lo && my_box < box_hi)  // a row behind the cache reads as zeros
-          tma_load_2d(dst + my_x / 64 * (128 * 128) + my_box * box * 128, map, my_x, min(my_row, p.pages * p.kv_heads * p.page.d), sa(bar));
-      }
-      if (hi - lo < kKeys) {
-#pragma unroll 4
-        for (uint32_t i = 0; i < kKeys / RS; ++i) {
-          const uint32_t row = i * RS + frow, j = t * kKeys + row;
-          if (row >= lo && row < hi) continue;
-          const uint32_t r = j >= j_first && j <= j_last ? cache_row(j) : 0xffffffffu;
-          const bool there = r != 0xffffffffu && col_there;
-          copy16(dst + place(row), static_cast<const uint16_t *>(cache) + (there ? (size_t)r * p.dim + col * 8 : 0), there);
-        }
-      }
-      requested(bar, hi - lo < kKeys);
-    };
-    look_up(t0);
-    uint32_t n = 0, stage = 0, phase = 1;  // requests: keys, values, keys, ...; place and the parity of its last release
-    for (uint32_t t = t0; t < t1; ++t) {
-      turn_to(t);
-      bool ok = true;
-#pragma unroll 1
-      for (uint32_t values = 0; values < 2; ++values) {
-        if (n >= C::kStages && !(ok = wait_warp(&empty[stage], phase))) break;
-        if (!values && t + 1 < t1) look_up(t + 1);
-        request(values ? p.vcache : p.kcache, values ? &map_v : &map_k, ring_a + stage * C::kTile, t, &full[stage]);
-        ++n;
-        if (++stage == C::kStages) stage = 0, phase ^= 1;
-      }
-      if (!ok) break;
+      if (t + 1 < t1) look_up(t + 1);
     }
     copy_wait<0>();
     if (late) landed();
-    if (failed_s && fw == 0 && lane == 0) {  // nothing may land when the CTA has gone
-      for (uint32_t x = n > C::kStages ? n - C::kStages : 0; x < n; ++x) mbar_wait_short(sa(&full[x % C::kStages]), x / C::kStages & 1);
+    if (failed_s && lane == 0) {  // nothing may land when the CTA has gone
+      for (uint32_t y = x > C::kStages ? x - C::kStages : 0; y < x; ++y)
+        if ((y & 1) == values) mbar_wait_short(sa(&full[y % C::kStages]), y / C::kStages & 1);
     }
   } else if (warp == kMmaWarp) {
     // ----------------------------------------------------------------------------------------------------------- MMA
