@@ -198,7 +198,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
     const uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f);  // NaN
     __syncwarp();
     for (uint32_t x = 0; x < 8; ++x)
-      if (again >> (x * 4) & 15u) row_again<BF>(p, at, kvh, at.first + warp * 16 + i * 8 + x);
+      if (again >> (x * 4) & 15u) row_again<BF>(p, at, kvh, at.first + warp * 16 + i * 8 + x, 0, DP);
   }
   stamp_end(p.stamps);
 }

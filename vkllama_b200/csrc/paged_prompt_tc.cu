@@ -28,8 +28,14 @@ template <int DP> struct Cfg {
   // One CTA per SM, which takes all of its TMEM: more than half of the shared memory, whatever the head width. K and V tiles take
   // turns in one ring: with two places each (373 -> 238 us) the MMAs still waited 1000 of 4000 cycles a tile for keys.
   static constexpr uint32_t kStages = DP == 64 ? 8 : 5;
-  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;
-  static_assert(kSmem > 114 * 1024 && kSmem + 1024 <= 227 * 1024, "one CTA per SM");
+  struct Shared {  // behind the tiles
+    uint64_t q_full[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4];
+    Place at;
+    uint32_t tmem, found;
+    volatile uint32_t failed;
+  };
+  static constexpr uint32_t kSmem = (2 + kStages) * kTile + sizeof(Shared);
+  static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA per SM");
 };
 
 __device__ __forceinline__ void mma_tmem(uint32_t acc, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
@@ -98,6 +104,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Sixteen columns times c.
 __device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
   uint32_t u[16];
@@ -114,40 +125,39 @@ __device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
 template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     paged_prompt_tc_kernel(const PagedAttention p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t box) {
   using C = Cfg<DP>;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full[2], full[C::kStages], empty[C::kStages], s_full[2], p_full[2][2], o_full[2];
-  __shared__ uint32_t tmem_s;
-  __shared__ volatile uint32_t failed_s;
-  __shared__ Place at_s;
-  __shared__ bool found_s;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  typename C::Shared &sh = *reinterpret_cast<typename C::Shared *>(smem + (2 + C::kStages) * C::kTile);
+  auto &q_full = sh.q_full, &s_full = sh.s_full, &o_full = sh.o_full;
+  auto &full = sh.full, &empty = sh.empty;
+  auto &p_full = sh.p_full;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = p.heads / p.kv_heads, tile = blockIdx.x / p.kv_heads, kvh = blockIdx.x - tile * p.kv_heads;
   if (tid == 0) {
     auto init = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"(n) : "memory"); };
     for (uint32_t s = 0; s < C::kStages; ++s) init(&full[s], 1), init(&empty[s], 1);
     for (uint32_t i = 0; i < 2; ++i) init(&q_full[i], 4), init(&s_full[i], 1), init(&p_full[i][0], 4), init(&p_full[i][1], 4), init(&o_full[i], 1);
+    sh.failed = 0;
+    for (uint32_t i = 0; i < 8; ++i) init(&sh.turn[i >> 2][i & 3], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    failed_s = 0;
   }
-  if (warp == kMmaWarp) tmem_alloc<512>(sa(&tmem_s));
+  if (warp == kMmaWarp) tmem_alloc<512>(sa(&sh.tmem));
   follow();
   stamp_begin(p.stamps);
   if (warp == kMmaWarp + 1) {
     Place found = {};
     const bool there = find_tile(p, per, 2 * kRows, tile, found);
-    if (lane == 0) at_s = found, found_s = there;
+    if (lane == 0) sh.at = found, sh.found = there;
   } else if (warp == 0 && blockIdx.x == 0) {
     check_rows(p);
   }
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = tmem_s;
-  if (!found_s) {
+  const uint32_t tmem = sh.tmem;
+  if (!sh.found) {
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     return;
   }
-  const Place &at = at_s;
+  const Place &at = sh.at;
   const uint32_t packed = at.fresh * per, past = at.len - at.fresh;
   // per tile of rows: its rows that exist, and the tiles of positions [b, e) that they see
   const bool both = at.first + kRows < packed;
@@ -160,19 +170,18 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   }
   const uint32_t t0 = b[0], t1 = e[1], tiles = both ? 2 : 1;  // b and e grow with the rows
   const uint32_t q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
-  // False when the wait ran out, or anyone's did.
+  // False when the wait ran out. The loop is one statement: its instructions are between every two steps of a tile.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    const uint32_t a = sa(bar);
-    for (uint32_t n = 0; n < kPolls / 64; ++n) {
-      for (uint32_t k = 0; k < 64; ++k) {
-        uint32_t ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(a), "r"(parity) : "memory");
-        if (ok) return true;
-      }
-      if (failed_s) return false;
-    }
-    failed_s = 1;
-    return false;
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
+        "there:\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(sa(bar)), "r"(parity), "n"(kPolls)
+        : "memory");
+    if (!ok) sh.failed = 1;
+    return ok != 0;
   };
   auto wait_warp = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };  // the lanes agree
 
@@ -187,15 +196,13 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       // the warp's 32 rows of Q, in the swizzle of the operand
       {
         constexpr uint32_t CH = DP / 8, RS = 32 / CH;  // pieces of a row; rows at a time
-        const uint32_t col = lane % CH;
-        const uint16_t *src = static_cast<const uint16_t *>(p.q);
+        const uint32_t col = lane % CH, qr0 = at.first + warp * 32 + lane / CH, dst = q_a + i * C::kTile + (col >> 3) * (128 * 128);
+        const uint16_t *src = static_cast<const uint16_t *>(p.q), *mine = src + at.row0 * p.q_ld + kvh * per * p.dim + col * 8;
 #pragma unroll 8
         for (uint32_t x = 0; x < 32 / RS; ++x) {
-          const uint32_t row = quad * 32 + x * RS + lane / CH, qr = at.first + i * kRows + row;
+          const uint32_t row = quad * 32 + x * RS + lane / CH, qr = qr0 + x * RS, rt = quotient(qr, p.group);
           const bool there = qr < packed && col * 8 < p.dim;
-          const uint32_t rt = quotient(qr, p.group);
-          copy16(q_a + i * C::kTile + (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4),
-                 there ? src + (at.row0 + rt) * p.q_ld + (kvh * per + qr - rt * per) * p.dim + col * 8 : src, there);
+          copy16(dst + row * 128 + (((col & 7) ^ (row & 7)) << 4), there ? mine + rt * p.q_ld + (qr - rt * per) * p.dim : src, there);
         }
         copy_commit();
         copy_wait<0>();
@@ -214,18 +221,23 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
         tc_after();
         uint32_t u[128];
         tmem_ld128(s_t, u);
-        if (t * kKeys < w_first || t * kKeys + kKeys - 1 > w_lo) {  // some row does not see all of it
-          const uint32_t lo = first > t * kKeys ? first - t * kKeys : 0, hi = pos >= t * kKeys ? pos - t * kKeys : 0;
-          const bool none = pos < t * kKeys;
+        if (t * kKeys + kKeys - 1 > w_lo) {  // positions that some row of the warp does not see yet
+          const int hi = (int)pos - (int)(t * kKeys);
 #pragma unroll
-          for (uint32_t x = 0; x < 128; ++x)
-            if (x < lo || x > hi || none) u[x] = 0xff800000u;
+          for (int x = 0; x < 128; ++x)
+            if (x > hi) u[x] = 0xff800000u;
+        }
+        if (t * kKeys < w_first) {  // and no more
+          const int lo = (int)first - (int)(t * kKeys);
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x < lo) u[x] = 0xff800000u;
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (uint32_t x = 0; x < 128; x += 8)
 #pragma unroll
-          for (uint32_t y = 0; y < 4; ++y) m4[y] = fmaxf(fmaxf(m4[y], __uint_as_float(u[x + y])), __uint_as_float(u[x + 4 + y]));
+          for (uint32_t y = 0; y < 4; ++y) m4[y] = max3(m4[y], __uint_as_float(u[x + y]), __uint_as_float(u[x + 4 + y]));
         const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if (t == bi) {
           top = m;
@@ -245,6 +257,11 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
             tmem_stored();
           }
         }
+        // The special function unit of a scheduler belongs to one tile's warp at a time: the other's products run meanwhile.
+        const bool shared_tile = tiles == 2 && t >= b[1] && t < e[0];
+        if (shared_tile && (i || t > b[1])) {
+          if (!(ok = wait_warp(&sh.turn[i][quad], (t - b[1] - (i ^ 1)) & 1))) break;
+        }
         const uint64_t scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -252,8 +269,9 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
           uint32_t w[16];
 #pragma unroll
           for (uint32_t x = 0; x < 16; ++x) {
-            const float2 y = of_pair(fma_pair(pair_of(__uint_as_float(u[c * 32 + 2 * x]), __uint_as_float(u[c * 32 + 2 * x + 1])), scale2, ref2));
-            const float a = exp2_fast(y.x), z = exp2_fast(y.y);
+            const uint64_t y = fma_pair(pair_of(__uint_as_float(u[c * 32 + 2 * x]), __uint_as_float(u[c * 32 + 2 * x + 1])), scale2, ref2);
+            const float2 v = of_pair(y);
+            const float a = exp2_fast(v.x), z = exp2_fast(v.y);
             sum2[x & 1] = add_pair(sum2[x & 1], pair_of(a, z));
             w[x] = pack2<BF>(a, z);
           }
@@ -265,6 +283,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) arrive(sa(&p_full[i][0]));
           }
         }
+        if (shared_tile && lane == 0) arrive(sa(&sh.turn[i ^ 1][quad]));
         const float2 part = of_pair(add_pair(sum2[0], sum2[1]));
         sum += part.x + part.y;
         tmem_stored();
@@ -275,28 +294,36 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       if (ok && wait_warp(&o_full[i], 0)) {
         tc_after();
         const float inv = 1.0f / sum;
-        const uint32_t row = min(r, packed - 1), rt = row / per, h = kvh * per + row - rt * per;
-        uint16_t *out = static_cast<uint16_t *>(p.out) + ((size_t)(at.row0 + rt) * p.heads + h) * p.dim;
+        // through shared memory (the tile's queries are through), so that a row is stored by neighbouring lanes
+        constexpr uint32_t CH = DP / 8, RS = 32 / CH;
+        unsigned char *mine = smem + i * C::kTile + quad * 32 * DP * 2;
         float finite = 0.f;
-#pragma unroll 1
+#pragma unroll
         for (uint32_t d = 0; d < DP; d += 32) {
           uint32_t u[32];
           tmem_ld32(o_t + d, u);
 #pragma unroll
-          for (int x = 0; x < 32; x += 8) {
+          for (uint32_t x = 0; x < 32; x += 8) {
             float v[8];
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              v[y] = __uint_as_float(u[x + y]) * inv;
-              finite += v[y] * 0.f;
-            }
-            if (r < packed && d + x < p.dim)
-              *reinterpret_cast<uint4 *>(out + d + x) = make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+            for (int y = 0; y < 8; ++y) v[y] = __uint_as_float(u[x + y]) * inv;
+            finite += ((v[0] * 0.f + v[1] * 0.f) + (v[2] * 0.f + v[3] * 0.f)) + ((v[4] * 0.f + v[5] * 0.f) + (v[6] * 0.f + v[7] * 0.f));
+            *reinterpret_cast<uint4 *>(mine + lane * DP * 2 + ((((d + x) / 8) ^ (lane & 7)) << 4)) =
+                make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
           }
+        }
+        __syncwarp();
+        const uint32_t col = lane % CH, qr0 = at.first + warp * 32 + lane / CH;
+        uint16_t *out = static_cast<uint16_t *>(p.out) + ((size_t)at.row0 * p.heads + kvh * per) * p.dim + col * 8;
+#pragma unroll 4
+        for (uint32_t x = 0; x < 32 / RS; ++x) {
+          const uint32_t row = x * RS + lane / CH, qr = qr0 + x * RS, rt = quotient(qr, p.group);
+          if (qr < packed && col * 8 < p.dim)
+            *reinterpret_cast<uint4 *>(out + ((size_t)rt * p.heads + qr - rt * per) * p.dim) = *reinterpret_cast<const uint4 *>(mine + row * DP * 2 + ((col ^ (row & 7)) << 4));
         }
         uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f && r < packed);  // NaN
         __syncwarp();
-        for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1);
+        for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
       }
     }
   } else if (warp < kSoftmaxWarps + kFetchWarps) {
@@ -375,7 +402,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     }
     copy_wait<0>();
     if (late) landed();
-    if (failed_s && lane == 0) {  // nothing may land when the CTA has gone
+    if (sh.failed && lane == 0) {  // nothing may land when the CTA has gone
       for (uint32_t y = x > C::kStages ? x - C::kStages : 0; y < x; ++y)
         if ((y & 1) == values) mbar_wait_short(sa(&full[y % C::kStages]), y / C::kStages & 1);
     }
@@ -441,7 +468,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   tc_before();
   __syncthreads();
   tc_after();
-  if (tid == 0 && failed_s) raise(p.error, kWaitCode);
+  if (tid == 0 && sh.failed) raise(p.error, kWaitCode);
   stamp_end(p.stamps);
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }

@@ -23,8 +23,8 @@ __device__ __forceinline__ uint32_t fresh_rows(const PagedAttention &p, uint32_t
   return 0;
 }
 
-// The place of tile `index` when every sequence has ceil(new * per / rows) of them, by one warp; false beyond the last. A sequence's last tiles
-// see most and come first.
+// The place of tile `index` when every sequence has ceil(new * per / rows) of them, by one warp; false beyond the last. What takes longest
+// comes first: a sequence's last tiles, which see most, and of up to 32 sequences the longest.
 __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint32_t index, Place &at) {
   const uint32_t lane = threadIdx.x & 31;
   bool bad = false;
@@ -32,15 +32,24 @@ __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per,
   for (uint32_t i0 = 0; i0 < p.n; i0 += 32) {
     const uint32_t i = i0 + lane, fresh = i < p.n ? fresh_rows(p, i, bad) : 0;
     const uint64_t mine = ((uint64_t)fresh * per + rows - 1) / rows;
-    uint64_t up = mine;
+    uint64_t up = mine;  // and all of the chunk's sequences that come before
+    if (p.n <= 32) {
+      const uint32_t len = fresh ? p.lengths[i] : 0;
+      for (uint32_t x = 0; x < p.n; ++x) {
+        const uint32_t other = __shfl_sync(0xffffffffu, len, x);
+        const uint64_t its = __shfl_sync(0xffffffffu, mine, x);
+        if (other > len || (other == len && x < lane)) up += its;
+      }
+    } else {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t a = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += a;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t a = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += a;
+      }
     }
-    const uint32_t behind = __ballot_sync(0xffffffffu, before + up > index);
-    if (behind) {
-      const uint32_t x = __ffs(behind) - 1;
+    const uint32_t it = __ballot_sync(0xffffffffu, before + up > index && before + up - mine <= index);
+    if (it) {
+      const uint32_t x = __ffs(it) - 1;
       at.seq = i0 + x;
       at.fresh = __shfl_sync(0xffffffffu, fresh, x);
       at.first = ((uint32_t)(__shfl_sync(0xffffffffu, before + up, x) - index) - 1) * rows;
@@ -48,7 +57,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per,
       at.len = p.lengths[at.seq];
       return true;
     }
-    before += __shfl_sync(0xffffffffu, up, 31);
+    if (p.n > 32) before += __shfl_sync(0xffffffffu, up, 31);
   }
   return false;
 }
@@ -59,10 +68,10 @@ __device__ __forceinline__ void check_rows(const PagedAttention &p) {
   if (bad) raise(p.error, PAGED_BAD_ROWS);
 }
 
-// One packed row by a warp, from the definition in fp32. In the tiles' second product a position that a row does not see has the
+// Dimensions [d0, d1) of one packed row by a warp, from the definition in fp32. In the tiles' second product a position that a row does not see has the
 // probability 0, and 0 times an infinity or a NaN in that position's value is NaN: rows that come out of it not finite are computed
 // again here, from the positions that they see. (So a value that is not finite costs time, and reaches only the rows that see it.)
-template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &p, const Place &at, uint32_t kvh, uint32_t packed) {
+template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &p, const Place &at, uint32_t kvh, uint32_t packed, uint32_t d0, uint32_t d1) {
   const uint32_t lane = threadIdx.x & 31, per = p.heads / p.kv_heads, t = packed / per, h = kvh * per + packed - t * per;
   const uint32_t pos = at.len - at.fresh + t, first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
   const uint16_t *q = static_cast<const uint16_t *>(p.q) + (at.row0 + t) * p.q_ld + h * p.dim;
@@ -114,7 +123,7 @@ template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t d = lane * 2 + 64 * i;
-    if (d < p.dim) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + ((size_t)(at.row0 + t) * p.heads + h) * p.dim + d) = pack2<BF>(o[i].x * r, o[i].y * r);
+    if (d >= d0 && d < d1 && d < p.dim) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + ((size_t)(at.row0 + t) * p.heads + h) * p.dim + d) = pack2<BF>(o[i].x * r, o[i].y * r);
   }
 }
 
