@@ -26,7 +26,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
 constexpr uint32_t kShareRows = 256;          // a CTA's share is at least this many positions
-constexpr uint32_t kSnapRows = 256;           // a cut this near to a pair's border moves there
+// A cut this near to a pair's border moves there. A cut costs some 5 us at the end (the parts of several CTAs meet in L2); a tile of 32 more
+// for one CTA costs 0.4 us where HBM is the limit, and an eighth of 1 us where the whole call is short.
+constexpr uint32_t kSnapRows = 256, kSnapRowsShort = 512, kShortRows = 1024;
 constexpr uint32_t kPairCost = 1;             // what a pair costs beside its tiles (queries, output, short rows in the ring), in tiles
 
 // DP: padded head width, MG: groups of eight query heads.
@@ -37,7 +39,7 @@ template <int DP, int MG> struct Cfg {
   static constexpr uint32_t kHeads = 8 * MG;
   static constexpr uint32_t kStash = kHeads * DP * 4;  // a warp's first part, where its range goes on behind it
   static constexpr uint32_t kSmem = kWarps * (kRing * kHalf + kStash + 2 * kHeads * 2 * 4);
-  static constexpr uint32_t kShare = kShareRows / kTile, kSnap = kSnapRows / kTile;
+  static constexpr uint32_t kShare = kShareRows / kTile, kSnap = kSnapRows / kTile, kSnapShort = kSnapRowsShort / kTile, kShort = kShortRows / kTile;
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory of an SM");
   static_assert(kRing * kHalf >= kStash, "a warp's last part lies in its ring");
 };
@@ -52,6 +54,7 @@ struct Pair {        // tiles t .. t1 of a sequence and head group
   uint32_t seq, grp;
   uint32_t t, t0, t1;
   uint32_t len, first;  // visible positions
+  uint32_t place;       // of tile t in the row of all work
 };
 
 // One record per part of a pair that ends inside a CTA.
@@ -68,7 +71,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ uint32_t before_s[kThreads + 1];  // tiles of one head group's sequences; the host has checked that they fit 32 bits
   __shared__ uint32_t warp_sum_s[kWarps];
-  __shared__ uint32_t border_s[2];
+  __shared__ uint32_t border_s[2], cut_s[2][2];  // the range's ends, and the first and last cut of the pairs that they cut
   __shared__ Part part_s[kWarps][2];
   __shared__ uint32_t last_s[2];
   unsigned char *ring = smem + threadIdx.x / 32 * C::kRing * C::kHalf;
@@ -112,14 +115,14 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     __syncthreads();
   }
   const uint32_t total = before_s[kThreads] * pairs, share = max((total + gridDim.x - 1) / gridDim.x, C::kShare);
-  auto find = [&](uint32_t pos) {  // the pair at place pos < total; t: tiles of it that lie before pos
-    uint32_t lo = 0, hi = kThreads;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if (before_s[mid] * pairs <= pos) lo = mid;
-      else hi = mid;
-    }
+  const uint32_t snap = share <= C::kShort ? C::kSnapShort : C::kSnap;
+  auto find = [&](uint32_t pos) {  // by a warp: the pair at place pos < total; t may lie behind its last tile, in the place that stands for its cost
+    uint32_t m = __ballot_sync(0xffffffffu, before_s[lane * 8] * pairs <= pos);
+    uint32_t lo = (31 - __clz(m)) * 8;
+    m = __ballot_sync(0xffffffffu, before_s[lo + (lane & 7)] * pairs <= pos) & 0xffu;
+    lo += 31 - __clz(m);
     Pair r;
+    r.place = pos;
     r.seq = lo * each;
     uint32_t left = pos - before_s[lo] * pairs, len = length(r.seq), n = places(len);
     while (left >= n * pairs) {
@@ -135,43 +138,31 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     r.t = r.t0 + left - r.grp * n;
     return r;
   };
-  if (tid < 2) {  // the range's borders
-    uint32_t b = min((uint64_t)(blockIdx.x + tid) * share, (uint64_t)total);
+  if (warp < 2) {  // the range's ends
+    uint32_t b = min((uint64_t)(blockIdx.x + warp) * share, (uint64_t)total);
     if (b > 0 && b < total) {
       const Pair r = find(b);
-      const uint32_t in = r.t - r.t0, out = r.t1 + kPairCost - r.t;
-      if (min(in, out) <= C::kSnap) b = in <= out ? b - in : b + out;
+      const uint32_t in = r.t - r.t0, out = r.t1 + kPairCost - r.t, begin = b - in;
+      if (min(in, out) <= snap) {
+        b = in <= out ? begin : b + out;
+      } else if (lane == 0) {  // all cuts of the pair: multiples of the share further than `snap` inside it
+        cut_s[warp][0] = (begin + snap) / share + 1;
+        cut_s[warp][1] = (begin + in + out - snap - 1) / share;
+      }
     }
-    border_s[tid] = b;
+    if (lane == 0) border_s[warp] = b;
   }
   __syncthreads();
   const uint32_t b0 = border_s[0], b1 = border_s[1];
   if (b0 == b1) return;
-  // A warp's places: pairs' tiles, and the places behind them that stand for a pair's cost.
+  // a warp's places
   const uint32_t part = (b1 - b0) / kWarps, more = (b1 - b0) % kWarps;
   const uint32_t w0 = b0 + part * warp + min(warp, more), w1 = w0 + part + (warp < more);
-  Pair at = {};
-  uint32_t count;  // its tiles
-  {
-    const uint32_t pos = lane & 1 ? w1 : w0;  // both ends at once
-    uint32_t before = total - p.n * pairs * kPairCost;  // tiles before pos
-    if (pos < total) {
-      at = find(pos);
-      const uint32_t in = at.t - at.t0, n = at.t1 - at.t0;
-      before = pos - (at.seq * pairs + at.grp) * kPairCost - (in > n ? in - n : 0);
-    }
-    count = __shfl_sync(0xffffffffu, before, 1) - __shfl_sync(0xffffffffu, before, 0);
-    at.seq = __shfl_sync(0xffffffffu, at.seq, 0);
-    at.grp = __shfl_sync(0xffffffffu, at.grp, 0);
-    at.t = __shfl_sync(0xffffffffu, at.t, 0);
-    at.t0 = __shfl_sync(0xffffffffu, at.t0, 0);
-    at.t1 = __shfl_sync(0xffffffffu, at.t1, 0);
-    at.len = __shfl_sync(0xffffffffu, at.len, 0);
-    at.first = __shfl_sync(0xffffffffu, at.first, 0);
-  }
 
   auto advance = [&](Pair &r) {
+    ++r.place;
     if (++r.t < r.t1) return;
+    r.place += kPairCost;
     if (++r.grp == pairs) {
       r.grp = 0;
       if (++r.seq >= p.n) return;
@@ -188,15 +179,21 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   auto first_head = [&](uint32_t grp) { return grp / groups * per + grp % groups * C::kHeads; };
   auto heads_of = [&](uint32_t grp) { return min(per - grp % groups * C::kHeads, C::kHeads); };
 
-  if (count) {
+  Pair at = {};
+  at.place = w1;
+  if (w0 < w1) {
+    at = find(w0);
     if (at.t >= at.t1) {  // the range begins behind a pair's last tile
+      at.place += at.t1 + kPairCost - at.t - 1 - kPairCost;
       at.t = at.t1 - 1;
       advance(at);
     }
+  }
+  if (at.place < w1) {
     // ---- the stream: tile halves, keys and values in turn, go into the ring's places one after the other ----
-    Pair in = at;
-    uint32_t left = count, entry = 0, in_page = 0, row_at = 0xffffffffu, slot_in = 0;
-    bool values = false;
+    Pair in = at;  // the tile whose page has been looked up
+    uint32_t entry = 0, in_page = 0, row_at = 0xffffffffu, slot_in = 0;
+    bool values = false, whole = false;
     const uint32_t ring_a = smem_addr(ring);
     auto look_up = [&]() {  // the page of this lane's position of the tile that comes next
       const uint32_t j = in.t * T + lane % T;
@@ -215,23 +212,26 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     const bool col_there = col * 8 < p.dim;
     const uint32_t piece = prow * CH * 16 + ((col ^ prow) << 4);
     const uint64_t step = (uint64_t)RS * p.dim * 2;
-    const bool tiled_pages = p.page.d % 16 == 0;
+    const bool runs = p.page.d % 8 == 0;  // eight rows from a multiple of eight on follow each other in a page
     auto request = [&]() {
-      if (left) {
+      if (values || in.place < w1) {
         if (!values) {
           row_at = 0xffffffffu;
           if (entry < p.pages) row_at = (entry * p.kv_heads + in.grp / groups) * p.page.d + in_page;  // the host has checked that rows fit 32 bits
           else if (entry != kNoSlot) raise(p.error, PAGED_BAD_PAGE);
+          whole = runs && in.t * T >= in.first && in.t * T + T <= in.len && __all_sync(0xffffffffu, entry < p.pages);
+          advance(in);
+          if (in.place < w1) look_up();
         }
         const uint8_t *cache = static_cast<const uint8_t *>(values ? p.vcache : p.kcache);
         const uint32_t dst = ring_a + slot_in * C::kHalf + piece;
-        if (tiled_pages && in.t * T >= in.first && in.t * T + T <= in.len && __all_sync(0xffffffffu, entry < p.pages)) {  // whole: sixteen rows follow each other in a page
+        if (whole) {
 #pragma unroll
-          for (uint32_t h = 0; h < T / 16; ++h) {
-            const uint32_t r = T == 16 ? row_at - lane % T : __shfl_sync(0xffffffffu, row_at, h * 16);
+          for (uint32_t h = 0; h < T / 8; ++h) {
+            const uint32_t r = __shfl_sync(0xffffffffu, row_at, h * 8);
             const uint8_t *src = cache + ((size_t)(r + prow) * p.dim + (col_there ? col * 8 : 0)) * 2;
 #pragma unroll
-            for (uint32_t i = h * NC * 16 / T; i < (h + 1) * NC * 16 / T; ++i, src += step) copy16((dst ^ (i * RS % 8) << 4) + i * 512, src, col_there);
+            for (uint32_t i = h * 8 / RS; i < (h + 1) * 8 / RS; ++i, src += step) copy16((dst ^ (i * RS % 8) << 4) + i * 512, src, col_there);
           }
         } else {
 #pragma unroll
@@ -240,10 +240,6 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
             const bool there = r != 0xffffffffu && col_there;
             copy16((dst ^ (i * RS % 8) << 4) + i * 512, there ? cache + ((size_t)r * p.dim + col * 8) * 2 : cache, there);
           }
-        }
-        if (values && --left) {
-          advance(in);
-          look_up();
         }
         values = !values;
         slot_in = slot_in + 1 == C::kRing ? 0 : slot_in + 1;
@@ -294,7 +290,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     const uint32_t k_at = (lrow + (lsel >> 1) * 8) * CH * 16 + (((lsel & 1) ^ lrow) << 4);
     const uint32_t v_at = (lrow + (lsel & 1) * 8) * CH * 16 + (((lsel >> 1) ^ lrow) << 4);
 #pragma unroll 1
-    for (uint32_t it = 0; it < count; ++it) {
+    for (;;) {
       copy_wait<C::kRing - 1>();
       __syncwarp();
       // S = Q K^T: matrices (rows 0-7 | 8-15) x (k low | k high)
@@ -384,9 +380,10 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       __syncwarp();
       request();
 
-      const bool ends = at.t + 1 == at.t1, over = it + 1 == count;
+      const bool ends = at.t + 1 == at.t1, over = at.place + 1 + (ends ? kPairCost : 0) >= w1;
       if (!ends && !over) {
         ++at.t;
+        ++at.place;
         continue;
       }
       // a part is complete
@@ -419,11 +416,10 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
         }
         keep(to, ml + (warp * 2 + over) * C::kHeads * 2);
       }
-      if (!over) {
-        advance(at);
-        start_pair();
-        begins = true;
-      }
+      if (over) break;
+      advance(at);
+      start_pair();
+      begins = true;
     }
     copy_wait<0>();
   }
@@ -432,26 +428,22 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   // ---- parts meet. They stand in order (warp by warp, a warp's first before its last); a run of them is one pair. ----
   auto part_o = [&](uint32_t i) { return (i & 1) ? reinterpret_cast<const float *>(smem + (i >> 1) * C::kRing * C::kHalf) : stash + (i >> 1) * (C::kStash / 4); };
   float *scratch_o = p.scratch, *scratch_ml = p.scratch + (size_t)gridDim.x * 2 * C::kHeads * DP;
-  uint32_t run = 0;
-  Part open[2] = {};  // the CTA's pairs that began before it (0), end behind it (1)
-  for (uint32_t i = 0; i < 2 * kWarps;) {
-    Part a = part_s[i >> 1][i & 1];
-    if (!a.there) {
-      ++i;
-      continue;
-    }
-    uint32_t e = i + 1;  // the run is [i, e)
-    for (bool done = a.ends; !done && e < 2 * kWarps; ++e) {
-      const Part b = part_s[e >> 1][e & 1];
-      if (b.there) a.ends = b.ends, done = b.ends;
-    }
-    const bool whole = a.begins && a.ends;
-    const uint32_t side = a.begins ? 1 : 0;  // where it goes in scratch
-    const uint32_t h0 = first_head(a.grp), nh = heads_of(a.grp);
+  uint32_t run = 0, open_there = 0;
+  uint32_t open_seq[2] = {}, open_grp[2] = {};  // the CTA's pairs that began before it (0), end behind it (1)
+  const Part mine = part_s[(lane & 15) >> 1][lane & 1];
+  const uint32_t all_there = __ballot_sync(0xffffffffu, lane < 16 && mine.there), all_begin = __ballot_sync(0xffffffffu, mine.begins);
+  const uint32_t all_end = __ballot_sync(0xffffffffu, lane < 16 && mine.there && mine.ends);
+  for (uint32_t rest = all_there; rest; ++run) {
+    const uint32_t i = __ffs(rest) - 1, end = all_end & -(1u << i), in_run = rest & (end ? (2u << (__ffs(end) - 1)) - 1 : 0xffffu);
+    rest &= ~in_run;
+    const bool begins = all_begin >> i & 1, whole = begins && end;
+    const uint32_t side = begins ? 1 : 0;  // where it goes in scratch
+    const uint32_t seq = __shfl_sync(0xffffffffu, mine.seq, i), grp = __shfl_sync(0xffffffffu, mine.grp, i);
+    const uint32_t h0 = first_head(grp), nh = heads_of(grp);
     for (uint32_t h = (warp + kWarps - run % kWarps) % kWarps; h < nh; h += kWarps) {
       // lane x has part x's maximum and sum
       float m = -INFINITY, l = 0.f;
-      if (lane >= i && lane < e && part_s[lane >> 1][lane & 1].there) {
+      if (in_run >> lane & 1) {
         const float2 v = *reinterpret_cast<const float2 *>(ml + (lane * C::kHeads + h) * 2);
         m = v.x, l = v.y;
       }
@@ -462,7 +454,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       float2 acc[DP / 64] = {};
 #pragma unroll
       for (uint32_t x = 0; x < 2 * kWarps; ++x) {
-        if (x < i || x >= e || !part_s[x >> 1][x & 1].there) continue;
+        if (!(in_run >> x & 1)) continue;
         const float cx = __shfl_sync(0xffffffffu, c, x);
         const float *src = part_o(x) + h * DP;
 #pragma unroll
@@ -474,7 +466,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       if (whole) {
         const float r = 1.0f / l;
 #pragma unroll
-        for (int d = 0; d < DP / 64; ++d) write_out(a.seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
+        for (int d = 0; d < DP / 64; ++d) write_out(seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
       } else {
         const size_t rec = ((size_t)blockIdx.x * 2 + side) * C::kHeads + h;
 #pragma unroll
@@ -483,36 +475,22 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       }
     }
     if (!whole) {
-      a.there = 1;
-      open[side] = a;
+      open_there |= 1u << side;
+      open_seq[side] = seq, open_grp[side] = grp;
     }
-    ++run;
-    i = e;
   }
-  if (!open[0].there && !open[1].there) {
+  if (!open_there) {
     stamp_end(p.stamps);
     return;
   }
 
-  // ---- pairs of several CTAs: cuts are the multiples of the share that lie further than C::kSnap inside the pair ----
+  // ---- pairs of several CTAs ----
   __threadfence();
   __syncthreads();
-  uint32_t cut0[2], cut1[2];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    cut0[side] = cut1[side] = 0;
-    if (!open[side].there) continue;
-    const uint32_t s = open[side].seq, base = s / each, n = places(length(s));
-    uint32_t begin = before_s[base];
-    for (uint32_t i = base * each; i < s; ++i) begin += places(length(i));
-    begin = begin * pairs + n * open[side].grp;
-    cut0[side] = (begin + C::kSnap) / share + 1;
-    cut1[side] = (begin + n - C::kSnap - 1) / share;  // cut0 <= cut1: n > 2 C::kSnap where a cut is left
-  }
   if (tid < 2) {
     last_s[tid] = 0;
-    if (open[tid].there) {
-      const uint32_t c0 = cut0[tid], parts = cut1[tid] - cut0[tid] + 2;
+    if (open_there >> tid & 1) {
+      const uint32_t c0 = cut_s[tid][0], parts = cut_s[tid][1] - c0 + 2;
       __threadfence();
       if (atomicAdd(p.counters + c0, 1u) + 1 == parts) {
         p.counters[c0] = 0;
@@ -525,9 +503,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   for (int side = 0; side < 2; ++side) {
     if (!last_s[side]) continue;
     __threadfence();
-    const Part a = open[side];
-    const uint32_t h0 = first_head(a.grp), nh = heads_of(a.grp);
-    const uint32_t c0 = cut0[side], c1 = cut1[side];
+    const uint32_t seq = open_seq[side], grp = open_grp[side], h0 = first_head(grp), nh = heads_of(grp), c0 = cut_s[side][0], c1 = cut_s[side][1];
     auto rec = [&](uint32_t c, uint32_t h) { return ((size_t)c * 2 + (c + 1 == c0 ? 1 : 0)) * C::kHeads + h; };  // the first part ends its CTA's range
     for (uint32_t h = warp; h < nh; h += kWarps) {
       float m = -INFINITY, l = 0.f;
@@ -548,7 +524,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       }
       const float r = 1.0f / l;
 #pragma unroll
-      for (int d = 0; d < DP / 64; ++d) write_out(a.seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
+      for (int d = 0; d < DP / 64; ++d) write_out(seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
     }
   }
   stamp_end(p.stamps);
