@@ -583,46 +583,60 @@ class ReadKVCache(Op):
         return self._out(out)
 
 
-class PagedTables(Op):
+class _PagedOp(Op):
+    """What the operators of a paged cache share: called once per layer and token, they build nothing that the call before has left.
+    An output is the same Tensor as long as the op keeps it (its shape is unchanged)."""
+
+    def __init__(self, dev, command, outputs):
+        super().__init__(dev, command)
+        self._outs = [vp() for _ in range(outputs)]
+        self._refs = [C.byref(o) for o in self._outs]
+        self._kept = [None] * outputs
+
+    def _output(self, i):
+        kept = self._kept[i]
+        if kept is None or kept.h.value != self._outs[i].value:
+            kept = self._kept[i] = self._out(vp(self._outs[i].value))
+        return kept
+
+
+class PagedTables(_PagedOp):
     """Page tables and slots of sequences that grow or shrink, over a pool of free pages (include/vkllama_b200.h)."""
 
     def __init__(self, dev, command, page_size):
-        super().__init__(dev, command)
+        super().__init__(dev, command, 2)
         _ck(self.L.vkl_paged_tables_create(dev.h, command.h, page_size, C.byref(self.h)))
 
     def __call__(self, lengths, target, table, pool, rows):
         """lengths becomes target, table and pool follow. Returns the map [1, 2, rows] (slots, positions) and starts [1, 1, n + 1]
         of the new tokens."""
-        m, s = vp(), vp()
-        _ck(self.L.vkl_paged_tables_run(self.h, _h(lengths), _h(target), _h(table), _h(pool), rows, C.byref(m), C.byref(s)))
-        return self._out(m), self._out(s)
+        _ck(self.L.vkl_paged_tables_run(self.h, _h(lengths), _h(target), _h(table), _h(pool), rows, *self._refs))
+        return self._output(0), self._output(1)
 
 
-class UpdatePagedKVCache(Op):
+class UpdatePagedKVCache(_PagedOp):
     """New keys and values into the pages of their sequences, keys (and queries) rotated by their positions on the way."""
 
     def __init__(self, dev, command, dim, page_size, theta=10000.0, dtype=FP16):
-        super().__init__(dev, command)
+        super().__init__(dev, command, 1)
         _ck(self.L.vkl_update_paged_kvcache_create(dev.h, command.h, dim, page_size, theta, dtype, C.byref(self.h)))
 
     def __call__(self, kcache, vcache, k, v, map, q=None):
         """Returns the rotated queries, or None where there are none."""
-        out = vp()
-        _ck(self.L.vkl_update_paged_kvcache_run(self.h, _h(kcache), _h(vcache), _h(k), _h(v), _h(map), _h(q), C.byref(out)))
-        return self._out(out) if q is not None else None
+        _ck(self.L.vkl_update_paged_kvcache_run(self.h, _h(kcache), _h(vcache), _h(k), _h(v), _h(map), _h(q), self._refs[0]))
+        return self._output(0) if q is not None else None
 
 
-class PagedAttention(Op):
+class PagedAttention(_PagedOp):
     """Attention over a paged cache: of one new token per sequence, or of the rows that `starts` gives every sequence."""
 
     def __init__(self, dev, command, heads, kv_heads, dim, page_size, scale=0.0, window=0, dtype=FP16):
-        super().__init__(dev, command)
+        super().__init__(dev, command, 1)
         _ck(self.L.vkl_paged_attention_create(dev.h, command.h, heads, kv_heads, dim, page_size, scale, window, dtype, C.byref(self.h)))
 
     def __call__(self, q, kcache, vcache, table, lengths, starts=None):
-        out = vp()
-        _ck(self.L.vkl_paged_attention_run(self.h, _h(q), _h(kcache), _h(vcache), _h(table), _h(lengths), _h(starts), C.byref(out)))
-        return self._out(out)
+        _ck(self.L.vkl_paged_attention_run(self.h, _h(q), _h(kcache), _h(vcache), _h(table), _h(lengths), _h(starts), self._refs[0]))
+        return self._output(0)
 
 
 class Transpose(Op):

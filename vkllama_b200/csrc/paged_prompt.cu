@@ -4,7 +4,7 @@
 //
 // The query heads of a key head share its keys and values, so a tile's rows are (row, head of the group) pairs, 64 of them: with
 // grouped heads a tile has fewer rows of the sequence and the same use of every key that is fetched. One CTA of four warps has a tile;
-// keys and values come through shared memory by cp.async, a tile ahead, and both products run on mma.sync (m16n8k16, fp32 sums) with
+// keys and values come through shared memory by cp.async, two tiles ahead, and both products run on mma.sync (m16n8k16, fp32 sums) with
 // a running maximum and sum per row. Probabilities are rounded to 16 bits for the second product, as its operand has to be (relative
 // 2^-12 or 2^-9 each, as much as the rounding of the output); their sum is taken before. Positions that a row does not see are masked
 // only in the tiles that some row of the warp does not see whole; a row whose result is not finite is computed again from its own
@@ -27,7 +27,7 @@ template <int DP> struct Cfg {
   static constexpr uint32_t kSmem = 2 * 2 * kKeys * DP * 2;
 };
 
-template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_prompt_kernel(const PagedAttention p) {
+template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 3) paged_prompt_kernel(const PagedAttention p) {
   using C = Cfg<DP>;
   constexpr uint32_t CH = DP / 8, KT = C::kKeys;
   constexpr int KS = DP / 16, NT = DP / 8, SN = KT / 8;
@@ -85,9 +85,10 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
     copy_commit();
   };
   look_up(t0);
+  look_up(t0 + 1);
   __syncthreads();
   request(t0);
-  look_up(t0 + 1);
+  request(t0 + 1);
 
   // this thread's rows: g and g + 8 of its warp's sixteen
   uint32_t q[KS][4], pos[2];
@@ -118,9 +119,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
 
 #pragma unroll 1
   for (uint32_t t = t0; t < t1; ++t) {
-    copy_wait<0>();
-    __syncthreads();  // the tile is there, everyone is through with the one before, the next one's rows are looked up
-    request(t + 1);
+    copy_wait<1>();
+    __syncthreads();  // the tile is there, and its rows' places may be looked up anew
     look_up(t + 2);
     const uint32_t kt = smem_a + (t & 1) * 2 * KT * DP * 2, vt = kt + KT * DP * 2;
     float s[SN][4] = {};
@@ -178,6 +178,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads) paged_pro
         mma2<BF>(o[n + 1], a0, a1, a2, a3, b[2], b[3]);
       }
     }
+    __syncthreads();  // everyone is through with the tile
+    request(t + 2);
   }
   copy_wait<0>();
 #pragma unroll
