@@ -293,6 +293,16 @@ def test_whole_tiles_of_rows(dev, dtype, past, new, heads, kv, dim, page, window
     prompt(dev, past, new, heads, kv, dim, page, dtype, window, scale=scale, behind=1)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_call_with_sequences_for_either_kernel(dev, dtype):
+    """A few rows behind many positions and behind few, prompts short and long: two launches share the sequences."""
+    before = vk.kernel_launches()
+    prompt(dev, [2000, 0, 600, 0, 510, 511, 0, 30], [3, 40, 1, 130, 1, 1, 0, 66], 2, 2, 64, 16, dtype, behind=2)
+    assert vk.kernel_launches() - before == 4
+    prompt(dev, [700, 3, 900], [2, 2, 7], 12, 2, 128, 8, dtype, window=600)
+    prompt(dev, [700, 3, 900], [2, 2, 7], 4, 2, 200, 8, dtype)
+
+
 def test_many_short_prompts_and_a_long_one(dev):
     rng = np.random.default_rng(8)
     new = [int(x) for x in rng.integers(0, 40, 150)] + [700]

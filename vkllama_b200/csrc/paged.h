@@ -117,12 +117,14 @@ struct PagedAttention {
   Divisor page, group;          // query heads of a key head
   float scale;                  // on the scores
   bool bf;
+  uint32_t part;                // of a prompt call's sequences, those that the launch takes: 0 all, 1 or 2 by paged_rows.cuh's rule
 };
 // One new token per sequence.
 cudaError_t launch_paged_token(const PagedAttention &p, uint32_t sms, cudaStream_t s);
 size_t paged_token_scratch(uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t sms);
 cudaError_t setup_paged_token();   // once per device
-// Any number of rows per sequence.
+// Any number of rows per sequence; in one launch or two.
+uint32_t paged_prompt_launches(const PagedAttention &p);
 cudaError_t launch_paged_prompt(const PagedAttention &p, cudaStream_t s);
 cudaError_t setup_paged_prompt();
 // The same on tcgen05, heads up to 128 wide.

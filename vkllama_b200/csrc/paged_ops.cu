@@ -289,7 +289,7 @@ struct PagedAttentionOp : PagedOp {
       p.group = divisor((uint32_t)per);
       p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
       p.bf = dtype == VKL_BF16;
-      VKL_LAUNCH(1, starts ? launch_paged_prompt(p, cmd->stream) : launch_paged_token(p, dev->prop.multiProcessorCount, cmd->stream));
+      VKL_LAUNCH(starts ? paged_prompt_launches(p) : 1, starts ? launch_paged_prompt(p, cmd->stream) : launch_paged_token(p, dev->prop.multiProcessorCount, cmd->stream));
     }
     *o = out;
     return VKL_OK;

@@ -20,7 +20,6 @@ namespace vkl {
 namespace {
 
 constexpr uint32_t kThreads = 128, kRows = 64;
-constexpr uint32_t kTensorRows = 96;  // packed rows of a sequence on average, from which the tcgen05 kernel has them
 
 template <int DP> struct Cfg {
   static constexpr uint32_t kKeys = DP == 256 ? 32 : 64;  // positions of a tile
@@ -224,9 +223,21 @@ cudaError_t setup_paged_prompt() {
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
+// The host knows the rows of all sequences together, and how many positions a table can hold. Where that does not say enough, each kernel takes the
+// sequences that are its own (the second finds nothing to do in 2 to 3 us).
+uint32_t paged_prompt_launches(const PagedAttention &p) {
+  const bool many = (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n;
+  return p.dim > 128 || many || p.width * p.page.d < kTensorLength ? 1 : 2;
+}
 cudaError_t launch_paged_prompt(const PagedAttention &p, cudaStream_t s) {
-  if (p.dim <= 128 && (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n) return launch_paged_prompt_tc(p, s);
-  return p.bf ? pick<true>(p, s) : pick<false>(p, s);
+  const bool many = (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n;
+  if (paged_prompt_launches(p) == 1) return p.dim <= 128 && many ? launch_paged_prompt_tc(p, s) : p.bf ? pick<true>(p, s) : pick<false>(p, s);
+  PagedAttention q = p;
+  q.part = 1;
+  const cudaError_t e = p.bf ? pick<true>(q, s) : pick<false>(q, s);
+  if (e != cudaSuccess) return e;
+  q.part = 2;
+  return launch_paged_prompt_tc(q, s);
 }
 
 }  // namespace vkl

@@ -141,7 +141,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == kMmaWarp) tmem_alloc<512>(sa(&sh.tmem));
   follow();
-  stamp_begin(p.stamps);
+  if (p.part != 2) stamp_begin(p.stamps);  // else the launch in front of this one did
   if (warp == kMmaWarp + 1) {
     Place found = {};
     const bool there = find_tile(p, per, 2 * kRows, tile, found);

@@ -23,6 +23,17 @@ __device__ __forceinline__ uint32_t fresh_rows(const PagedAttention &p, uint32_t
   return 0;
 }
 
+// Which kernel takes a sequence: tcgen05 (part 2) where its tiles of 256 packed rows are filled far enough or there are many positions to see, the
+// tiles of 64 on mma.sync (part 1) else. us, 32 heads of 128, mma.sync / tcgen05: 8 prompts of 64 12.4 / 24.3, of 128 22.8 / 18.3; 4 times 64 rows behind
+// 2000 106 / 41; 32 drafts of 5 rows, 8 key heads, behind 1000 69 / 47.
+constexpr uint32_t kTensorRows = 96, kTensorLength = 512;
+__device__ __forceinline__ uint32_t rows_here(const PagedAttention &p, uint32_t i, uint32_t per, bool &bad) {
+  const uint32_t fresh = fresh_rows(p, i, bad);
+  if (p.part == 0) return fresh;
+  const bool tensor = (uint64_t)fresh * per >= kTensorRows || p.lengths[i] >= kTensorLength;
+  return tensor == (p.part == 2) ? fresh : 0;
+}
+
 // The place of tile `index` when every sequence has ceil(new * per / rows) of them, by one warp; false beyond the last. What takes longest
 // comes first: a sequence's last tiles, which see most, and of up to 32 sequences the longest.
 __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint32_t index, Place &at) {
@@ -30,7 +41,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per,
   bool bad = false;
   uint64_t before = 0;
   for (uint32_t i0 = 0; i0 < p.n; i0 += 32) {
-    const uint32_t i = i0 + lane, fresh = i < p.n ? fresh_rows(p, i, bad) : 0;
+    const uint32_t i = i0 + lane, fresh = i < p.n ? rows_here(p, i, per, bad) : 0;
     const uint64_t mine = ((uint64_t)fresh * per + rows - 1) / rows;
     uint64_t up = mine;  // and all of the chunk's sequences that come before
     if (p.n <= 32) {
