@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const PagedTable
   __syncthreads();
   bad = bad_s;
   if (!bad && total_s[0] > p.rows) bad = PAGED_ROWS;
-  if (!bad && (count > p.capacity || count + total_s[2] > p.capacity)) bad = PAGED_POOL_BAD;
+  if (!bad && p.n && (count > p.capacity || count + total_s[2] > p.capacity)) bad = PAGED_POOL_BAD;
   if (!bad && total_s[1] > count + total_s[2]) bad = PAGED_POOL_EMPTY;
   if (bad) {
     for (uint32_t r = blockIdx.x * kThreads + tid; r < p.rows; r += gridDim.x * kThreads) p.map[r] = kNoSlot, p.map[p.rows + r] = 0;
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const PagedTable
   if (!last) return;
   stamp_end(p.stamps);
   if (bad) return;
-  if (tid == 0) p.pool[0] = count + (uint32_t)total_s[2] - (uint32_t)total_s[1];
+  if (tid == 0 && p.n) p.pool[0] = count + (uint32_t)total_s[2] - (uint32_t)total_s[1];
   for (uint32_t i = i0; i < i1; ++i) p.lengths[i] = p.target[i];
 }
 
