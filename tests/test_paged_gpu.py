@@ -374,7 +374,8 @@ def test_refusals(dev):
         assert code_of(vk.UpdatePagedKVCache(dev, cmd, 64, 16, theta).init) == 3
     for heads, kv in ((4, 3), (0, 1), (4, 0), (2, 4), (-4, 2)):
         assert code_of(vk.PagedAttention(dev, cmd, heads, kv, 64, 16).init) == 3
-    assert code_of(vk.PagedAttention(dev, cmd, 4, 4, 64, 16, float("inf")).init) == 3
+    for scale in (float("inf"), float("nan"), 1e-30, -1e30):
+        assert code_of(vk.PagedAttention(dev, cmd, 4, 4, 64, 16, scale).init) == 3
     assert code_of(vk.PagedAttention(dev, cmd, 4, 4, 64, 16, 0.0, -1).init) == 3
     for dtype in (vk.FP32, vk.Q8_0, vk.INT8, vk.UINT32):
         assert code_of(vk.PagedAttention(dev, cmd, 4, 4, 64, 16, dtype=dtype).init) == 3
@@ -405,9 +406,18 @@ def test_refusals(dev):
         assert code_of(lambda: att(*(other if j == i else a for j, a in enumerate(good)))) == 3, i
     assert code_of(lambda: att(T(1, n + 1, 256), *good[1:5])) == 3  # a query without a sequence
     assert code_of(lambda: att(T(1, n, 260).view(1, n, 256), *good[1:5])) == 12
+    out = att(q, *good[1:5])
+    assert code_of(lambda: att(out, *good[1:5])) == 3  # its own output
+    assert code_of(lambda: update(cache, cache, k, k, m)) == 3  # one cache for both
     far = vk.PagedAttention(dev, cmd, 4, 2, 64, 1 << 20).init()
     assert code_of(lambda: far(q, T(1, 2 << 20, 64), T(1, 2 << 20, 64), U(1, n, 2048), U(1, 1, n))) == 11
     assert cmd.L.vkl_paged_attention_run(tables.h, q.h, cache.h, cache.h, good[3].h, good[4].h, None, C.byref(C.c_void_p())) == 3  # another kind of op
+    cmd.end()
+    try:
+        cmd.submit_and_wait()  # the tensors above hold what they hold
+    except vk.VklError:
+        pass
+    cmd.begin()
     # nothing to do is no error
     assert update(cache, good[2], T(1, 0, 128), T(1, 0, 128), U(1, 2, 0), T(1, 0, 256)).shape() == (1, 0, 256)
     assert att(T(1, 0, 256), cache, good[2], U(1, 0, 4), U(1, 1, 0)).shape() == (1, 0, 256)
@@ -533,3 +543,27 @@ def test_time_of_the_last_run(dev):
         with cmd:
             op(q, k, v, table, lens)
         assert 2 <= op.time() < 1000
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(vk.FP16, 128, 256), (vk.BF16, 256, 24)])
+def test_caches_beyond_32_bits(dev, dtype, dim, page):
+    """Pages whose first value lies past 2^32 values (and past 2^32 bytes) of the cache; slots past 2^24."""
+    rng, cmd = np.random.default_rng(15), vk.Command(dev)
+    rows = 2 ** 32 // dim + 40 * page
+    pages, new = rows // page, 150
+    table = np.arange(pages - 1, pages - 1 - 2 * (-(-new // page) + 1), -2, dtype=np.uint32)[None]  # the last ones, every other
+    pos = np.arange(new)
+    slots = (table[0, pos // page].astype(np.uint64) * page + pos % page).astype(np.uint32)
+    assert (int(table[0, 0]) * page + 1) * dim > 2 ** 32
+    x = [draw(rng, (new, h * dim), dtype) for h in (2, 1, 1)]
+    with cmd:
+        kc, vc = (vk.Tensor(pages, page, dim, dev, dtype) for _ in range(2))
+        q, k, v = (tensor(cmd, dev, a, dtype) for a in x)
+        vk.UpdatePagedKVCache(dev, cmd, dim, page, 0.0, dtype).init()(kc, vc, k, v, tensor(cmd, dev, np.stack([slots, pos]).astype(np.uint32)))
+        op, t = vk.PagedAttention(dev, cmd, 2, 1, dim, page, dtype=dtype).init(), tensor(cmd, dev, table)
+        many = cmd.download(op(q, kc, vc, t, tensor(cmd, dev, np.array([new], np.uint32)), tensor(cmd, dev, np.array([0, new], np.uint32))))
+        one = cmd.download(op(tensor(cmd, dev, x[0][-1:], dtype), kc, vc, t, tensor(cmd, dev, np.array([new], np.uint32))))
+    q, k, v = (to_values(a, dtype).reshape(new, -1, dim) for a in x)
+    want, mass, size = P.attention(q, pos, k.transpose(1, 0, 2), v.transpose(1, 0, 2))
+    check(to_values(many, dtype).reshape(new, 2, dim), want, mass, size, dtype, dim, new, 5.0, True)
+    check(to_values(one, dtype).reshape(1, 2, dim), want[-1:], mass[-1:], size[-1:], dtype, dim, new, 5.0, False)

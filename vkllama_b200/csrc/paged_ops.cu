@@ -30,7 +30,7 @@ struct PagedOp : vkl_op {
   ~PagedOp() override { vkl_tensor_release(stamps); }
   int paged_init() {
     if (!dev || !cmd) return fail(VKL_INVALID_ARGUMENT, "op: null device or command");
-    VKL_OKAY(tensor_new(dev, 1, 1, 4, VKL_UINT32, &stamps));
+    VKL_OKAY(ensure_tensor(dev, &stamps, 1, 1, 4, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(stamps->data(), 0, 16, cmd->stream));
     uint32_t *word;
     VKL_OKAY(command_error_word(cmd, &word));  // allocated here, so that run() does not have to
@@ -48,7 +48,8 @@ struct PagedOp : vkl_op {
   int elapsed(uint64_t *usec) override {
     *usec = 0;
     if (!timed) return VKL_OK;
-    if (cudaStreamQuery(cmd->stream) != cudaSuccess) {
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;  // a query would end a capture
+    if (cudaStreamIsCapturing(cmd->stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone || cudaStreamQuery(cmd->stream) != cudaSuccess) {
       (void)cudaGetLastError();
       return fail(VKL_FAILED_PRECONDITION, "op_time: the op's last run has not finished (wait on its command first)");
     }
@@ -115,7 +116,7 @@ struct PagedTablesOp : PagedOp {
     OnDevice here(dev->ordinal);
     if (!good_page(page)) return fail(VKL_INVALID_ARGUMENT, "PagedTables op: a page of %d tokens", page);
     VKL_CUDA(setup_paged_tables());
-    VKL_OKAY(tensor_new(dev, 1, 1, 1, VKL_UINT32, &arrived));
+    VKL_OKAY(ensure_tensor(dev, &arrived, 1, 1, 1, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(arrived->data(), 0, 4, cmd->stream));
     return paged_init();
   }
@@ -172,7 +173,7 @@ struct UpdatePagedOp : PagedOp {
     if (theta != 0.f) {
       std::vector<double> per(dim / 2);
       for (int k = 0; k < dim / 2; ++k) per[k] = std::pow((double)theta, -2.0 * k / dim) / (2.0 * std::acos(-1.0));
-      VKL_OKAY(tensor_new(dev, 1, 1, dim, VKL_FP32, &turns));
+      VKL_OKAY(ensure_tensor(dev, &turns, 1, 1, dim, VKL_FP32));
       VKL_CUDA(cudaMemcpyAsync(turns->data(), per.data(), per.size() * 8, cudaMemcpyHostToDevice, cmd->stream));
       VKL_CUDA(cudaStreamSynchronize(cmd->stream));
     }
@@ -198,6 +199,7 @@ struct UpdatePagedOp : PagedOp {
     VKL_OKAY(check_apart(k, who, "keys"));
     VKL_OKAY(check_apart(v, who, "values"));
     if (q) VKL_OKAY(check_apart(q, who, "queries"));
+    if (kcache->data() == vcache->data()) return fail(VKL_INVALID_ARGUMENT, "%s: keys and values have one cache", who);
     if ((q ? q->w : 0) + 2 * k->w > 1u << 24) return fail(VKL_OUT_OF_RANGE, "%s: rows of %zu values", who, (q ? q->w : 0) + 2 * k->w);
     VKL_OKAY(begin(who));
     if (q) VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
@@ -249,8 +251,8 @@ struct PagedAttentionOp : PagedOp {
     VKL_CUDA(setup_paged_token());
     VKL_CUDA(setup_paged_prompt());
     VKL_CUDA(setup_paged_prompt_tc());
-    VKL_OKAY(tensor_new(dev, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32, &scratch));
-    VKL_OKAY(tensor_new(dev, 1, 1, sms + 1, VKL_UINT32, &counters));
+    VKL_OKAY(ensure_tensor(dev, &scratch, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32));
+    VKL_OKAY(ensure_tensor(dev, &counters, 1, 1, sms + 1, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
     return paged_init();
   }
@@ -270,6 +272,7 @@ struct PagedAttentionOp : PagedOp {
     if (rows * per > kMaxTokens || n > kMaxTokens || (rows * per / 64 + n) * kv_heads > kMaxTokens || (!starts && n * (table->w * page / 16 + 2) * (kv_heads * ((per + 7) / 8)) > kMaxTokens))
       return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, %zu sequences of up to %zu tokens", who, rows, n, table->w * page);
     VKL_OKAY(begin(who));
+    if (out && q->data() == out->data()) return fail(VKL_INVALID_ARGUMENT, "%s: the queries are this op's own output", who);
     VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
     if (rows && n) {
       PagedAttention p = {};

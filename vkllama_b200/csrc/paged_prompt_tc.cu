@@ -29,7 +29,7 @@ template <int DP> struct Cfg {
   // turns in one ring: with two places each (373 -> 238 us) the MMAs still waited 1000 of 4000 cycles a tile for keys.
   static constexpr uint32_t kStages = DP == 64 ? 8 : 5;
   struct Shared {  // behind the tiles
-    uint64_t q_full[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4];
+    uint64_t q_full[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4], drained;
     Place at;
     uint32_t tmem, found;
     volatile uint32_t failed;
@@ -135,6 +135,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     auto init = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"(n) : "memory"); };
     for (uint32_t s = 0; s < C::kStages; ++s) init(&full[s], 1), init(&empty[s], 1);
     for (uint32_t i = 0; i < 2; ++i) init(&q_full[i], 4), init(&s_full[i], 1), init(&p_full[i][0], 4), init(&p_full[i][1], 4), init(&o_full[i], 1);
+    init(&sh.drained, 1);
     sh.failed = 0;
     for (uint32_t i = 0; i < 8; ++i) init(&sh.turn[i >> 2][i & 3], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -461,6 +462,10 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
           keys.next(), keys.next();
         }
         if (n > 0) vals.next(), vals.next();
+      }
+      if (!ok) {  // nothing may be in work when the TMEM is given back
+        mma_commit(sa(&sh.drained));
+        mbar_wait_short(sa(&sh.drained), 0);
       }
     }
     __syncwarp();
