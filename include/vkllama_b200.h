@@ -242,8 +242,8 @@ int vkl_update_paged_kvcache_run(vkl_op *op, vkl_tensor *kcache, vkl_tensor *vca
  *   of no tokens gives zeros.
  *   else q [1, rows, heads * dim]: sequence i's new tokens are the last starts[i + 1] - starts[i] of its lengths[i]; each sees the
  *   positions up to its own. Sequences without new rows are skipped; output rows that belong to no sequence are left as they were.
- * q may be a view of wider rows (16-byte row starts). Values at positions that a row does not see never reach it, whatever they
- * are. In the one-token form an infinite value that weighs less than 2^-25 may come out as NaN. */
+ * q may be a view of wider rows (16-byte row starts). Values at positions that a row does not see never reach it, whatever they are;
+ * infinities and NaN at ones that it sees come out as the sum in fp32 has them (such rows are computed a second time, slowly). */
 int vkl_paged_attention_create(vkl_device *dev, vkl_command *cmd, int heads, int kv_heads, int dim, int page_size, float scale, int window,
                                int dtype, vkl_op **out);
 int vkl_paged_attention_run(vkl_op *op, vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths,

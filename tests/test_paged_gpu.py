@@ -205,7 +205,8 @@ def token(dev, lengths, heads, kv, dim, page, dtype, window=0, scale=None, wide=
 @pytest.mark.parametrize("lengths,heads,kv,dim,page,window", [
     ([1], 1, 1, 8, 1, 0), ([300], 32, 32, 128, 16, 0), ([17, 0, 1, 16, 15, 33, 0], 4, 4, 128, 16, 0), ([5000], 8, 1, 128, 64, 0), ([0, 0], 4, 2, 64, 16, 0),
     ([1200, 3, 801, 640], 12, 4, 64, 8, 0), ([257, 1, 900], 40, 5, 80, 24, 100), ([100, 2000, 31], 12, 1, 128, 16, 0), ([1500, 700], 16, 1, 72, 32, 33),
-    ([900, 20], 24, 1, 256, 16, 0), ([63, 64, 65, 1000], 6, 2, 192, 5, 0), ([2500], 40, 1, 128, 16, 1000), ([40, 41, 42], 48, 2, 96, 16, 7)])
+    ([900, 20], 24, 1, 256, 16, 0), ([63, 64, 65, 1000], 6, 2, 192, 5, 0), ([2500], 40, 1, 128, 16, 1000), ([40, 41, 42], 48, 2, 96, 16, 7),
+    ([3000, 40, 0, 900], 16, 1, 256, 16, 0), ([700, 20], 11, 1, 136, 24, 100), ([4000], 48, 3, 64, 16, 0)])
 def test_one_token_per_sequence(dev, dtype, lengths, heads, kv, dim, page, window):
     token(dev, lengths, heads, kv, dim, page, dtype, window, wide=16 if len(lengths) > 2 else 0)
 
@@ -229,21 +230,27 @@ def test_scores_far_apart(dev, dtype):
     token(dev, [777], 4, 4, 128, 16, dtype, scale=-1.0)
 
 
-def test_infinite_and_missing_numbers_where_a_token_sees_them(dev):
+@pytest.mark.parametrize("heads,dim,long", [(4, 64, 0), (12, 64, 0), (4, 128, 5000), (16, 200, 0), (20, 128, 3000)])
+def test_infinite_and_missing_numbers_where_a_token_sees_them(dev, heads, dim, long):
+    """Also where the weight is far below 16 bits, in whole pairs, in parts that warps and CTAs join."""
     rng = np.random.default_rng(6)
-    c = Cache(rng, [100, 100, 100], 1, 64, 16, vk.FP16)
-    q = draw(rng, (3, 4 * 64), vk.FP16, 0.1)
-    c.seq_v[0][0, 40, 3] = 0x7c00
+    n = 100 + long
+    c = Cache(rng, [n, n, n, n], 1, dim, 16, vk.FP16)
+    q = draw(rng, (4, heads * dim), vk.FP16, 0.1)
+    q[3] = to_bits(np.ones(heads * dim), vk.FP16)
+    c.seq_v[0][0, 40, 3] = c.seq_v[3][0, 50, 7] = 0x7c00
     c.seq_v[1][0, 99, 5] = 0x7e00
-    for i in range(2):
+    c.seq_k[3][0, 50] = to_bits(np.full(dim, -40 / np.sqrt(dim)), vk.FP16)  # a score of -40
+    for i in (0, 1, 3):
         c.put(c.v, i, c.seq_v[i])
+        c.put(c.k, i, c.seq_k[i])
     cmd = vk.Command(dev)
     with cmd:
         k, v, table, lens = c.up(cmd, dev)
-        out = vk.PagedAttention(dev, cmd, 4, 1, 64, 16).init()(tensor(cmd, dev, q, vk.FP16), k, v, table, lens)
-        got = to_values(cmd.download(out), vk.FP16).reshape(3, 4, 64)
-    for i, d, ok in ((0, 3, np.isposinf), (1, 5, np.isnan)):
-        assert ok(got[i, :, d]).all() and np.isfinite(np.delete(got[i], d, 1)).all()
+        out = vk.PagedAttention(dev, cmd, heads, 1, dim, 16).init()(tensor(cmd, dev, q, vk.FP16), k, v, table, lens)
+        got = to_values(cmd.download(out), vk.FP16).reshape(4, heads, dim)
+    for i, d, ok in ((0, 3, np.isposinf), (1, 5, np.isnan), (3, 7, np.isposinf)):
+        assert ok(got[i, :, d]).all() and np.isfinite(np.delete(got[i], d, 1)).all(), i
     assert np.isfinite(got[2]).all()
 
 

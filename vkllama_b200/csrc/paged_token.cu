@@ -1,42 +1,48 @@
 // Attention of one new token per sequence over a paged cache:
 //   out = sum_j softmax_j(scale q.k_j) v_j over the positions max(0, length - window) <= j < length.
 //
-// Every visible key and value is read once for all query heads of its group, so HBM bounds it: 4 dim bytes a position and key head.
-// The products run on mma.sync (m16n8k16, fp32 sums) because a group's queries share the fragments: 8 (or 16) query heads are the
-// rows of A, cached rows the columns. A tile's upper eight rows would be empty; in P.V they carry what rounding the probabilities to
-// 16 bits leaves over (p = hi + lo, both exact products, added at the end), so the result has the probabilities' 32 bits at no cost.
+// Every visible key and value is read once for all query heads of its group (sixteen of them at a time), so HBM bounds it: 4 dim bytes a
+// position and key head. The products run on mma.sync (m16n8k16, fp32 sums) because a group's queries share the fragments: its query
+// heads are the rows of A, cached rows the columns. Probabilities go into the second product as two 16-bit numbers, p = hi + lo, both
+// products exact, so the result has their 32 bits. Up to eight heads lo has the upper eight rows of A, which would be empty, and costs nothing;
+// beyond, a second product with the same fragment of V.
 //
-// Work is cut into equal shares, not by sequence: the tiles (of 16 or 32 positions) of all (sequence, head group) pairs stand in one row (and a place more for each pair's own cost), every
-// CTA takes a range of it and every warp of the CTA a range of that, however the lengths are spread. Ranges cut pairs: a warp keeps
+// Work is cut into equal shares, not by sequence: the tiles (of 16 or 32 positions) of all (sequence, head group) pairs stand in one row, with
+// a place more for each pair's own cost; every CTA takes a range of it and every warp of the CTA a range of that, however the lengths are spread. Ranges cut pairs: a warp keeps
 // running maximum, sum and output of its part; parts meet in shared memory, and those of several CTAs in scratch, where the CTA that
 // arrives last adds them up in their order (the result does not depend on who that is). Cuts that would leave a small piece of a pair are
 // moved to its border.
 //
 // A warp streams its range through a ring of its own (cp.async, tiles of keys and of values alternating, swizzled for ldmatrix):
 // no barrier inside the stream, the next pages are looked up a tile ahead. Rows that are not visible are not read and count as zeros.
+//
+// Measured on sequences that hold 0.37 GB together (57 us at the rate of a copy): 71 ... 76 us, 4.9 ... 5.2 TB/s, with up to eight heads to a
+// key head whatever the width, the page and the lengths; 87 us with 12 or 16 heads of 128, 103 us with 16 of 256 (shared memory and the
+// products are the limit there), 122 us with 32 on one key head, which reads everything twice. What is left up to eight heads is the
+// machine's: under full load 24 of the 148 SMs take 12 % longer for the same bytes, and shares are fixed before anyone knows which.
 #include <algorithm>
 
 #include "common.cuh"
 #include "paged.h"
+#include "paged_rows.cuh"
 #include "paged_value.cuh"
 
 namespace vkl {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kWarps = 8, kThreads = kWarps * 32;
 constexpr uint32_t kShareRows = 256;          // a CTA's share is at least this many positions
 // A cut this near to a pair's border moves there. A cut costs some 5 us at the end (the parts of several CTAs meet in L2); a tile of 32 more
 // for one CTA costs 0.4 us where HBM is the limit, and an eighth of 1 us where the whole call is short.
 constexpr uint32_t kSnapRows = 256, kSnapRowsShort = 512, kShortRows = 1024;
 constexpr uint32_t kPairCost = 1;             // what a pair costs beside its tiles (queries, output, short rows in the ring), in tiles
 
-// DP: padded head width, MG: groups of eight query heads.
-template <int DP, int MG> struct Cfg {
-  static constexpr uint32_t kTile = DP * MG <= 128 ? 32 : 16;  // positions of a tile: 32 where the registers suffice, half the softmax steps
-  static constexpr uint32_t kHalf = kTile * DP * 2;            // bytes of a tile's keys, or values
-  static constexpr uint32_t kRing = DP == 64 ? 5 : DP == 128 ? (MG == 1 ? 3 : 4) : 2;
-  static constexpr uint32_t kHeads = 8 * MG;
+// DP: padded head width. WIDE: sixteen query heads in the rows of A; else eight, and the low parts of their probabilities in the others.
+template <int DP, bool WIDE> struct Cfg {
+  static constexpr uint32_t kWarps = DP == 256 && WIDE ? 6 : 8, kThreads = kWarps * 32;
+  static constexpr uint32_t kTile = DP == 64 || (DP == 128 && !WIDE) ? 32 : 16;  // positions of a tile
+  static constexpr uint32_t kHalf = kTile * DP * 2;                            // bytes of a tile's keys, or values
+  static constexpr uint32_t kRing = DP == 64 ? 5 : DP == 128 ? (WIDE ? 4 : 3) : 2;
+  static constexpr uint32_t kHeads = WIDE ? 16 : 8;
   static constexpr uint32_t kStash = kHeads * DP * 4;  // a warp's first part, where its range goes on behind it
   static constexpr uint32_t kSmem = kWarps * (kRing * kHalf + kStash + 2 * kHeads * 2 * 4);
   static constexpr uint32_t kShare = kShareRows / kTile, kSnap = kSnapRows / kTile, kSnapShort = kSnapRowsShort / kTile, kShort = kShortRows / kTile;
@@ -63,8 +69,10 @@ struct Part {
   uint8_t there, begins, ends;  // the pair begins, ends in this part
 };
 
-template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1) paged_token_kernel(const PagedAttention p) {
-  using C = Cfg<DP, MG>;
+template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, WIDE>::kThreads, 1) paged_token_kernel(const PagedAttention p) {
+  using C = Cfg<DP, WIDE>;
+  constexpr uint32_t kWarps = C::kWarps, kThreads = C::kThreads;
+  constexpr int NR = WIDE ? 2 : 1;           // query heads of a thread's fragments: rows g (and g + 8)
   constexpr uint32_t CH = DP / 8;            // 16-byte pieces of a row
   constexpr uint32_t T = C::kTile, NC = T * CH / 32;  // pieces of a half and lane
   constexpr int KS = DP / 16, NT = DP / 8, SN = T / 8;
@@ -117,9 +125,9 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   const uint32_t total = before_s[kThreads] * pairs, share = max((total + gridDim.x - 1) / gridDim.x, C::kShare);
   const uint32_t snap = share <= C::kShort ? C::kSnapShort : C::kSnap;
   auto find = [&](uint32_t pos) {  // by a warp: the pair at place pos < total; t may lie behind its last tile, in the place that stands for its cost
-    uint32_t m = __ballot_sync(0xffffffffu, before_s[lane * 8] * pairs <= pos);
-    uint32_t lo = (31 - __clz(m)) * 8;
-    m = __ballot_sync(0xffffffffu, before_s[lo + (lane & 7)] * pairs <= pos) & 0xffu;
+    uint32_t m = __ballot_sync(0xffffffffu, before_s[lane * kWarps] * pairs <= pos);
+    uint32_t lo = (31 - __clz(m)) * kWarps;
+    m = __ballot_sync(0xffffffffu, lane < kWarps && before_s[lo + min(lane, kWarps - 1)] * pairs <= pos);
     lo += 31 - __clz(m);
     Pair r;
     r.place = pos;
@@ -175,6 +183,12 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   };
   auto write_out = [&](uint32_t seq, uint32_t head, uint32_t d, float a, float b) {
     if (d < p.dim) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.out) + ((size_t)seq * p.heads + head) * p.dim + d) = pack2<BF>(a, b);
+  };
+  // A row that is not finite, from the definition (paged_rows.cuh): a value that is not may have met a part of a probability that is 0.
+  auto redo = [&](uint32_t seq, uint32_t head) {
+    const Place one = {seq, seq, 1, length(seq), 0};
+    const uint32_t kvh = head / per;
+    row_again<BF>(p, one, kvh, head - kvh * per, 0, DP);
   };
   auto first_head = [&](uint32_t grp) { return grp / groups * per + grp % groups * C::kHeads; };
   auto heads_of = [&](uint32_t grp) { return min(per - grp % groups * C::kHeads, C::kHeads); };
@@ -250,39 +264,42 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
     for (uint32_t i = 0; i < C::kRing; ++i) request();
 
     // ---- the sums of the current pair: rows g of every group of eight heads; o's second half holds the low parts ----
-    float o[MG][NT][4], mx[MG], sum[MG];
-    uint32_t q[MG][KS][2];
+    float o[NT][4], mx[NR], sum[NR];
+    uint32_t q[KS][2 * NR];
     uint32_t slot = 0;
     bool begins = at.t == at.t0;
     auto start_pair = [&]() {
       const uint32_t h0 = first_head(at.grp), nh = heads_of(at.grp);
 #pragma unroll
-      for (int m = 0; m < MG; ++m) {
-        const uint16_t *src = static_cast<const uint16_t *>(p.q) + at.seq * p.q_ld + (h0 + m * 8 + g) * p.dim;
+      for (int r = 0; r < NR; ++r) {
+        const uint16_t *src = static_cast<const uint16_t *>(p.q) + at.seq * p.q_ld + (h0 + r * 8 + g) * p.dim;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t d = k * 16 + e * 8 + t4 * 2;
-            q[m][k][e] = m * 8 + g < nh && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) ^ flip : 0u;
+            q[k][e * NR + r] = r * 8 + g < nh && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) ^ flip : 0u;
           }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
-        mx[m] = -INFINITY;
-        sum[m] = 0.f;
+        mx[r] = -INFINITY;
+        sum[r] = 0.f;
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
     };
-    // hi + lo of one output; an infinite one has no low part (its product there is 0 times infinity)
-    auto joined = [](float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; };
+    // Output e of row r of a pair of dimensions. High and low part lie apart in the narrow form; an infinite high part has no low one (its
+    // product there is 0 times infinity).
+    auto result = [&](int n, int r, int e) {
+      if constexpr (WIDE) return o[n][2 * r + e];
+      else return fabsf(o[n][e]) < INFINITY ? o[n][e] + o[n][2 + e] : o[n][e];
+    };
     auto keep = [&](float *to, float *to_ml) {  // this part for the ones that join it
 #pragma unroll
-      for (int m = 0; m < MG; ++m) {
+      for (int r = 0; r < NR; ++r) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          *reinterpret_cast<float2 *>(to + (m * 8 + g) * DP + n * 8 + t4 * 2) = make_float2(joined(o[m][n][0], o[m][n][2]), joined(o[m][n][1], o[m][n][3]));
-        if (t4 == 0) to_ml[(m * 8 + g) * 2] = mx[m], to_ml[(m * 8 + g) * 2 + 1] = sum[m];
+        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2 *>(to + (r * 8 + g) * DP + n * 8 + t4 * 2) = make_float2(result(n, r, 0), result(n, r, 1));
+        if (t4 == 0) to_ml[(r * 8 + g) * 2] = mx[r], to_ml[(r * 8 + g) * 2 + 1] = sum[r];
       }
     };
     start_pair();
@@ -294,13 +311,7 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       copy_wait<C::kRing - 1>();
       __syncwarp();
       // S = Q K^T: matrices (rows 0-7 | 8-15) x (k low | k high)
-      float s[MG][SN][4];
-#pragma unroll
-      for (int m = 0; m < MG; ++m)
-#pragma unroll
-        for (int n = 0; n < SN; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+      float s[SN][4] = {};
       {
         const uint32_t kt = ring_a + slot * C::kHalf + k_at;
 #pragma unroll
@@ -309,11 +320,8 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
           for (int n = 0; n < SN; n += 2) {
             uint32_t b[4];
             ldmatrix4(b, (kt ^ k << 5) + n * 8 * CH * 16);
-#pragma unroll
-            for (int m = 0; m < MG; ++m) {
-              mma2<BF>(s[m][n], q[m][k][0], 0, q[m][k][1], 0, b[0], b[1]);
-              mma2<BF>(s[m][n + 1], q[m][k][0], 0, q[m][k][1], 0, b[2], b[3]);
-            }
+            mma2<BF>(s[n], q[k][0], WIDE ? q[k][1] : 0, q[k][NR], WIDE ? q[k][2 * NR - 1] : 0, b[0], b[1]);
+            mma2<BF>(s[n + 1], q[k][0], WIDE ? q[k][1] : 0, q[k][NR], WIDE ? q[k][2 * NR - 1] : 0, b[2], b[3]);
           }
       }
       slot = slot + 1 == C::kRing ? 0 : slot + 1;
@@ -328,37 +336,46 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
             const uint32_t j = at.t * T + n * 8 + t4 * 2 + e;
             if (j < at.first || j >= at.len) {
 #pragma unroll
-              for (int m = 0; m < MG; ++m) s[m][n][e] = -INFINITY;
+              for (int r = 0; r < NR; ++r) s[n][2 * r + e] = -INFINITY;
             }
           }
       }
-      uint32_t pa[MG][SN][2];  // high and low parts
+      uint32_t hi[SN][NR], lo[SN][NR];  // the probabilities' high and low parts
+      bool grown = false;
+      float ref[NR], top[NR];
 #pragma unroll
-      for (int m = 0; m < MG; ++m) {
-        float top = mx[m];
+      for (int r = 0; r < NR; ++r) {
+        top[r] = mx[r];
 #pragma unroll
-        for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(s[m][n][0], s[m][n][1]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float ref = top == -INFINITY ? 0.f : top * scale;
-        if (__any_sync(0xffffffffu, top != mx[m])) {
-          const float c = exp2_fast(mx[m] * scale - ref);
-          sum[m] *= c;
+        for (int n = 0; n < SN; ++n) top[r] = fmaxf(top[r], fmaxf(s[n][2 * r], s[n][2 * r + 1]));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        ref[r] = top[r] == -INFINITY ? 0.f : top[r] * scale;
+        grown |= top[r] != mx[r];
+      }
+      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < NR; ++r) {
+          const float c = exp2_fast(mx[r] * scale - ref[r]);
+          sum[r] *= c;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[m][n][e] *= c;
-          mx[m] = top;
-        }
-#pragma unroll
-        for (int n = 0; n < SN; ++n) {
-          const float a = exp2_fast(fmaf(s[m][n][0], scale, -ref)), b = exp2_fast(fmaf(s[m][n][1], scale, -ref));
-          sum[m] += a + b;
-          pa[m][n][0] = pack2<BF>(a, b);
-          const float2 hi = unpack2<BF>(pa[m][n][0]);
-          pa[m][n][1] = pack2<BF>(a - hi.x, b - hi.y);
+          for (int n = 0; n < NT; ++n) {
+            o[n][2 * r] *= c, o[n][2 * r + 1] *= c;
+            if constexpr (!WIDE) o[n][2] *= c, o[n][3] *= c;
+          }
+          mx[r] = top[r];
         }
       }
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int n = 0; n < SN; ++n) {
+          const float a = exp2_fast(fmaf(s[n][2 * r], scale, -ref[r])), b = exp2_fast(fmaf(s[n][2 * r + 1], scale, -ref[r]));
+          sum[r] += a + b;
+          hi[n][r] = pack2<BF>(a, b);
+          const float2 h = unpack2<BF>(hi[n][r]);
+          lo[n][r] = pack2<BF>(a - h.x, b - h.y);
+        }
       copy_wait<C::kRing - 1>();
       __syncwarp();
       {
@@ -369,10 +386,14 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
           for (int n = 0; n < NT; n += 2) {
             uint32_t b[4];
             ldmatrix4_t(b, (vt ^ n << 4) + k * 8 * CH * 16);
-#pragma unroll
-            for (int m = 0; m < MG; ++m) {
-              mma2<BF>(o[m][n], pa[m][k][0], pa[m][k][1], pa[m][k + 1][0], pa[m][k + 1][1], b[0], b[1]);
-              mma2<BF>(o[m][n + 1], pa[m][k][0], pa[m][k][1], pa[m][k + 1][0], pa[m][k + 1][1], b[2], b[3]);
+            if constexpr (WIDE) {
+              mma2<BF>(o[n], hi[k][0], hi[k][1], hi[k + 1][0], hi[k + 1][1], b[0], b[1]);
+              mma2<BF>(o[n + 1], hi[k][0], hi[k][1], hi[k + 1][0], hi[k + 1][1], b[2], b[3]);
+              mma2<BF>(o[n], lo[k][0], lo[k][1], lo[k + 1][0], lo[k + 1][1], b[0], b[1]);
+              mma2<BF>(o[n + 1], lo[k][0], lo[k][1], lo[k + 1][0], lo[k + 1][1], b[2], b[3]);
+            } else {
+              mma2<BF>(o[n], hi[k][0], lo[k][0], hi[k + 1][0], lo[k + 1][0], b[0], b[1]);
+              mma2<BF>(o[n + 1], hi[k][0], lo[k][0], hi[k + 1][0], lo[k + 1][0], b[2], b[3]);
             }
           }
       }
@@ -387,26 +408,31 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
         continue;
       }
       // a part is complete
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+      }
       if (begins && ends) {
         const uint32_t h0 = first_head(at.grp), nh = heads_of(at.grp);
 #pragma unroll
-        for (int m = 0; m < MG; ++m) {
-          float all = sum[m];
-          all += __shfl_xor_sync(0xffffffffu, all, 1);
-          all += __shfl_xor_sync(0xffffffffu, all, 2);
-          const float r = at.len ? 1.0f / all : 0.f;  // nothing visible: zeros
-          if (m * 8 + g < nh) {
+        for (int r = 0; r < NR; ++r) {
+          const float inv = at.len ? 1.0f / sum[r] : 0.f;  // nothing visible: zeros
+          float finite = 0.f;
+          if (r * 8 + g < nh) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-              write_out(at.seq, h0 + m * 8 + g, n * 8 + t4 * 2, joined(o[m][n][0], o[m][n][2]) * r, joined(o[m][n][1], o[m][n][3]) * r);
+            for (int n = 0; n < NT; ++n) {
+              const float a = result(n, r, 0) * inv, b = result(n, r, 1) * inv;
+              finite += a * 0.f + b * 0.f;
+              write_out(at.seq, h0 + r * 8 + g, n * 8 + t4 * 2, a, b);
+            }
           }
+          const uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f);  // NaN
+          __syncwarp();
+          for (uint32_t x = 0; x < 8; ++x)
+            if (again >> (x * 4) & 15u) redo(at.seq, h0 + r * 8 + x);
         }
       } else {
-#pragma unroll
-        for (int m = 0; m < MG; ++m) {
-          sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 1);
-          sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 2);
-        }
         if (lane == 0) part_s[warp][over] = {at.seq, at.grp, 1, begins, ends};
         float *to = stash + warp * (C::kStash / 4);
         if (over) {
@@ -430,9 +456,9 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
   float *scratch_o = p.scratch, *scratch_ml = p.scratch + (size_t)gridDim.x * 2 * C::kHeads * DP;
   uint32_t run = 0, open_there = 0;
   uint32_t open_seq[2] = {}, open_grp[2] = {};  // the CTA's pairs that began before it (0), end behind it (1)
-  const Part mine = part_s[(lane & 15) >> 1][lane & 1];
-  const uint32_t all_there = __ballot_sync(0xffffffffu, lane < 16 && mine.there), all_begin = __ballot_sync(0xffffffffu, mine.begins);
-  const uint32_t all_end = __ballot_sync(0xffffffffu, lane < 16 && mine.there && mine.ends);
+  const Part mine = part_s[min(lane >> 1, kWarps - 1)][lane & 1];
+  const uint32_t all_there = __ballot_sync(0xffffffffu, lane < 2 * kWarps && mine.there), all_begin = __ballot_sync(0xffffffffu, mine.begins);
+  const uint32_t all_end = __ballot_sync(0xffffffffu, lane < 2 * kWarps && mine.there && mine.ends);
   for (uint32_t rest = all_there; rest; ++run) {
     const uint32_t i = __ffs(rest) - 1, end = all_end & -(1u << i), in_run = rest & (end ? (2u << (__ffs(end) - 1)) - 1 : 0xffffu);
     rest &= ~in_run;
@@ -465,8 +491,17 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
       }
       if (whole) {
         const float r = 1.0f / l;
+        float finite = 0.f;
 #pragma unroll
-        for (int d = 0; d < DP / 64; ++d) write_out(seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
+        for (int d = 0; d < DP / 64; ++d) {
+        const float a = acc[d].x * r, b = acc[d].y * r;
+        finite += a * 0.f + b * 0.f;
+        write_out(seq, h0 + h, d * 64 + lane * 2, a, b);
+      }
+      if (__any_sync(0xffffffffu, finite != 0.f)) {
+        __syncwarp();
+        redo(seq, h0 + h);
+      }
       } else {
         const size_t rec = ((size_t)blockIdx.x * 2 + side) * C::kHeads + h;
 #pragma unroll
@@ -523,41 +558,50 @@ template <bool BF, int DP, int MG> __global__ void __launch_bounds__(kThreads, 1
         }
       }
       const float r = 1.0f / l;
+      float finite = 0.f;
 #pragma unroll
-      for (int d = 0; d < DP / 64; ++d) write_out(seq, h0 + h, d * 64 + lane * 2, acc[d].x * r, acc[d].y * r);
+      for (int d = 0; d < DP / 64; ++d) {
+        const float a = acc[d].x * r, b = acc[d].y * r;
+        finite += a * 0.f + b * 0.f;
+        write_out(seq, h0 + h, d * 64 + lane * 2, a, b);
+      }
+      if (__any_sync(0xffffffffu, finite != 0.f)) {
+        __syncwarp();
+        redo(seq, h0 + h);
+      }
     }
   }
   stamp_end(p.stamps);
 }
 
-template <bool BF, int DP, int MG> cudaError_t setup_one() {
-  return cudaFuncSetAttribute(paged_token_kernel<BF, DP, MG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP, MG>::kSmem);
+template <bool BF, int DP, bool WIDE> cudaError_t setup_one() {
+  return cudaFuncSetAttribute(paged_token_kernel<BF, DP, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP, WIDE>::kSmem);
 }
-template <bool BF, int DP, int MG> cudaError_t run(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
-  using C = Cfg<DP, MG>;
+template <bool BF, int DP, bool WIDE> cudaError_t run(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
+  using C = Cfg<DP, WIDE>;
   // No more CTAs than there can be shares of.
-  const uint64_t per = p.heads / p.kv_heads, pairs = (uint64_t)p.kv_heads * ((per + 8 * MG - 1) / (8 * MG));
+  const uint64_t per = p.heads / p.kv_heads, pairs = (uint64_t)p.kv_heads * ((per + C::kHeads - 1) / C::kHeads);
   const uint64_t most = p.n * pairs * (((uint64_t)p.width * p.page.d + C::kTile - 1) / C::kTile + kPairCost), shares = (most + C::kShare - 1) / C::kShare;
-  return launch_following(paged_token_kernel<BF, DP, MG>, dim3((uint32_t)std::min<uint64_t>(sms, shares)), kThreads, C::kSmem, s, p);
+  return launch_following(paged_token_kernel<BF, DP, WIDE>, dim3((uint32_t)std::min<uint64_t>(sms, shares)), C::kThreads, C::kSmem, s, p);
 }
+bool wide(uint32_t heads, uint32_t kv_heads) { return heads / kv_heads > 8; }  // more query heads than the narrow form's rows
 template <bool BF> cudaError_t pick(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
-  // Sixteen query heads per warp where a group has more than eight and their outputs fit the registers: keys and values are read
-  // once for all of them. Wider heads take them eight at a time, the second time from L2.
-  const bool two = p.heads / p.kv_heads > 8;
-  if (p.dim <= 64) return two ? run<BF, 64, 2>(p, sms, s) : run<BF, 64, 1>(p, sms, s);
-  if (p.dim <= 128) return two ? run<BF, 128, 2>(p, sms, s) : run<BF, 128, 1>(p, sms, s);
-  return run<BF, 256, 1>(p, sms, s);
+  const bool w = wide(p.heads, p.kv_heads);
+  if (p.dim <= 64) return w ? run<BF, 64, true>(p, sms, s) : run<BF, 64, false>(p, sms, s);
+  if (p.dim <= 128) return w ? run<BF, 128, true>(p, sms, s) : run<BF, 128, false>(p, sms, s);
+  return w ? run<BF, 256, true>(p, sms, s) : run<BF, 256, false>(p, sms, s);
 }
 
 }  // namespace
 
 size_t paged_token_scratch(uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t sms) {
-  const uint32_t dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, most = heads / kv_heads > 8 && dim <= 128 ? 16 : 8;
+  const uint32_t dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256, most = wide(heads, kv_heads) ? 16 : 8;
   return (size_t)sms * 2 * most * (dp + 2) * 4;
 }
 cudaError_t setup_paged_token() {
-  for (cudaError_t e : {setup_one<false, 64, 1>(), setup_one<false, 64, 2>(), setup_one<false, 128, 1>(), setup_one<false, 128, 2>(), setup_one<false, 256, 1>(),
-                        setup_one<true, 64, 1>(), setup_one<true, 64, 2>(), setup_one<true, 128, 1>(), setup_one<true, 128, 2>(), setup_one<true, 256, 1>()})
+  for (cudaError_t e : {setup_one<false, 64, false>(), setup_one<false, 64, true>(), setup_one<false, 128, false>(), setup_one<false, 128, true>(),
+                        setup_one<false, 256, false>(), setup_one<false, 256, true>(), setup_one<true, 64, false>(), setup_one<true, 64, true>(),
+                        setup_one<true, 128, false>(), setup_one<true, 128, true>(), setup_one<true, 256, false>(), setup_one<true, 256, true>()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
