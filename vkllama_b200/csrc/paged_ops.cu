@@ -171,10 +171,10 @@ struct UpdatePagedOp : PagedOp {
     if (!good_dim(dim)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: head dim %d is no multiple of 8 up to 256", dim);
     if (theta != 0.f && !(theta >= 1.f && theta <= 1e30f)) return fail(VKL_INVALID_ARGUMENT, "UpdatePagedKVCache op: theta is %g", theta);
     if (theta != 0.f) {
-      std::vector<double> per(dim / 2);
+      double per[128];
       for (int k = 0; k < dim / 2; ++k) per[k] = std::pow((double)theta, -2.0 * k / dim) / (2.0 * std::acos(-1.0));
       VKL_OKAY(ensure_tensor(dev, &turns, 1, 1, dim, VKL_FP32));
-      VKL_CUDA(cudaMemcpyAsync(turns->data(), per.data(), per.size() * 8, cudaMemcpyHostToDevice, cmd->stream));
+      VKL_CUDA(cudaMemcpyAsync(turns->data(), per, dim / 2 * 8, cudaMemcpyHostToDevice, cmd->stream));
       VKL_CUDA(cudaStreamSynchronize(cmd->stream));
     }
     return paged_init();

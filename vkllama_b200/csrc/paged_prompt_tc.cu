@@ -7,9 +7,11 @@
 // products). Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
 //             that it grew by more than 2^8: until then the probabilities stay below 2^8 and O as it is; only then O is multiplied.
-//   8, 9      fetch K_j and V_j into a ring, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte swizzle of the matrix descriptors: K is K-major and
-//             V, as it lies in the cache, MN-major (64 dimensions of a position are a row of 128 bytes in both).
+//   8, 9      fetch K_j and V_j into a ring, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte
+//             swizzle of the matrix descriptors: K is K-major and V, as it lies in the cache, MN-major (64 dimensions of a position are a
+//             row of 128 bytes in both).
 //   10        issues the MMAs. They complete in order, so the commit behind S_i(j + 1) also says that P_i(j) V_j is in O_i.
+//   11        finds the tile, then idles.
 // Every wait is bounded; after one that ran out all warps leave, and the error word is raised.
 #include <algorithm>
 
@@ -19,7 +21,7 @@
 namespace vkl {
 namespace {
 
-constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // the twelfth idles: more than 12 warps would have 128 registers each
+constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // more than 12 warps would have 128 registers each
 constexpr uint32_t kRows = 128, kKeys = 128;
 constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20;
 
