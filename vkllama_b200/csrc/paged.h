@@ -110,6 +110,7 @@ struct PagedAttention {
   const uint32_t *starts;       // [n + 1], or null: row i is the last token of sequence i
   float *scratch;               // partial results, paged_token_scratch() bytes
   uint32_t *counters;           // [SMs + 1], 0 between launches
+  uint32_t *tickets;            // [2], 0 between launches
   unsigned long long *stamps;
   uint32_t *error;
   uint64_t q_ld;
@@ -125,10 +126,10 @@ size_t paged_token_scratch(uint32_t heads, uint32_t kv_heads, uint32_t dim, uint
 cudaError_t setup_paged_token();   // once per device
 // Any number of rows per sequence; in one launch or two.
 uint32_t paged_prompt_launches(const PagedAttention &p);
-cudaError_t launch_paged_prompt(const PagedAttention &p, cudaStream_t s);
+cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStream_t s);
 cudaError_t setup_paged_prompt();
 // The same on tcgen05, heads up to 128 wide.
-cudaError_t launch_paged_prompt_tc(const PagedAttention &p, cudaStream_t s);
+cudaError_t launch_paged_prompt_tc(const PagedAttention &p, uint32_t sms, cudaStream_t s);
 cudaError_t setup_paged_prompt_tc();
 
 }  // namespace vkl

@@ -252,7 +252,7 @@ struct PagedAttentionOp : PagedOp {
     VKL_CUDA(setup_paged_prompt());
     VKL_CUDA(setup_paged_prompt_tc());
     VKL_OKAY(ensure_tensor(dev, &scratch, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32));
-    VKL_OKAY(ensure_tensor(dev, &counters, 1, 1, sms + 1, VKL_UINT32));
+    VKL_OKAY(ensure_tensor(dev, &counters, 1, 1, sms + 3, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
     return paged_init();
   }
@@ -264,6 +264,7 @@ struct PagedAttentionOp : PagedOp {
     VKL_OKAY(check_cache(kcache, vcache, who, dtype, kv_heads, page, dim));
     VKL_OKAY(check_table(table, who, page));
     const size_t n = table->h, rows = q->h, per = heads / kv_heads;
+    const uint32_t sms = dev->prop.multiProcessorCount;
     VKL_OKAY(check_list(lengths, who, "lengths", n));
     if (starts) VKL_OKAY(check_list(starts, who, "starts", n + 1));
     if (!starts && rows != n) return fail(VKL_INVALID_ARGUMENT, "%s: %zu queries for %zu sequences of one new token each", who, rows, n);
@@ -284,6 +285,7 @@ struct PagedAttentionOp : PagedOp {
       p.starts = starts ? (const uint32_t *)starts->data() : nullptr;
       p.scratch = (float *)scratch->data();
       p.counters = (uint32_t *)counters->data();
+      p.tickets = p.counters + sms + 1;
       VKL_OKAY(command_error_word(cmd, &p.error));
       p.stamps = stamp();
       p.rows = (uint32_t)rows, p.n = (uint32_t)n, p.heads = heads, p.kv_heads = kv_heads, p.dim = dim;
@@ -292,7 +294,7 @@ struct PagedAttentionOp : PagedOp {
       p.group = divisor((uint32_t)per);
       p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
       p.bf = dtype == VKL_BF16;
-      VKL_LAUNCH(starts ? paged_prompt_launches(p) : 1, starts ? launch_paged_prompt(p, cmd->stream) : launch_paged_token(p, dev->prop.multiProcessorCount, cmd->stream));
+      VKL_LAUNCH(starts ? paged_prompt_launches(p) : 1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
     }
     *o = out;
     return VKL_OK;

@@ -40,7 +40,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256
   stamp_begin(p.stamps);
   if (warp == 0) {
     Place found = {};
-    const bool there = find_tile(p, per, kRows, tile, found);
+    Walk walk;
+    const bool there = find_tile(p, per, kRows, tile, found, walk);
     if (lane == 0) at_s = found, found_s = there;
   } else if (warp == 1 && blockIdx.x == 0) {
     check_rows(p);
@@ -229,15 +230,15 @@ uint32_t paged_prompt_launches(const PagedAttention &p) {
   const bool many = (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n;
   return p.dim > 128 || many || p.width * p.page.d < kTensorLength ? 1 : 2;
 }
-cudaError_t launch_paged_prompt(const PagedAttention &p, cudaStream_t s) {
+cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
   const bool many = (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n;
-  if (paged_prompt_launches(p) == 1) return p.dim <= 128 && many ? launch_paged_prompt_tc(p, s) : p.bf ? pick<true>(p, s) : pick<false>(p, s);
+  if (paged_prompt_launches(p) == 1) return p.dim <= 128 && many ? launch_paged_prompt_tc(p, sms, s) : p.bf ? pick<true>(p, s) : pick<false>(p, s);
   PagedAttention q = p;
   q.part = 1;
   const cudaError_t e = p.bf ? pick<true>(q, s) : pick<false>(q, s);
   if (e != cudaSuccess) return e;
   q.part = 2;
-  return launch_paged_prompt_tc(q, s);
+  return launch_paged_prompt_tc(q, sms, s);
 }
 
 }  // namespace vkl

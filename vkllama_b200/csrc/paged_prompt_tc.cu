@@ -4,14 +4,15 @@
 // 128. Per tile of rows i and positions j: S_i = Q_i K_j^T (tcgen05.mma, fp32 in TMEM), P_i = 2^(scale S_i - reference) as 16-bit numbers
 // written over S_i in TMEM, O_i += P_i V_j with P as the TMEM operand. The two tiles of rows take turns: while the tensor core works
 // for one, the exponentials of the other are computed, which take as long (16 per clock and SM: 1024 cycles for 128 x 128, like the two
-// products). Warps:
+// products). A CTA stays on its SM and takes one such item after the other by tickets, what takes longest first: a new CTA per item costs some
+// 10 us of start and end, in which nothing else runs (64 prompts of 256: 210 us, this way 149). Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
 //             that it grew by more than 2^8: until then the probabilities stay below 2^8 and O as it is; only then O is multiplied.
 //   8, 9      fetch K_j and V_j into a ring, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte
 //             swizzle of the matrix descriptors: K is K-major and V, as it lies in the cache, MN-major (64 dimensions of a position are a
 //             row of 128 bytes in both).
 //   10        issues the MMAs. They complete in order, so the commit behind S_i(j + 1) also says that P_i(j) V_j is in O_i.
-//   11        finds the tile, then idles.
+//   11        takes the tickets and fetches Q, so that queries, keys and values of the next item are there when this one's output is stored.
 // Every wait is bounded; after one that ran out all warps leave, and the error word is raised.
 #include <algorithm>
 
@@ -24,6 +25,14 @@ namespace {
 constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // more than 12 warps would have 128 registers each
 constexpr uint32_t kRows = 128, kKeys = 128;
 constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20;
+// Registers of a thread: a softmax thread has a row of scores in registers, the other warps give theirs. The sum has to be below what the launch has.
+constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80, kLaunchRegs = kSoftmaxWarps * 32 * kSoftmaxRegs + (kThreads - kSoftmaxWarps * 32) * kOtherRegs;
+
+// What a CTA works on: 256 packed rows of a sequence and key head, as one or two tiles, and the tiles of positions [b, e) that each of them sees.
+struct Item {
+  Place at;
+  uint32_t found, kvh, tiles, b[2], e[2];
+};
 
 template <int DP> struct Cfg {
   static constexpr uint32_t kTile = 128 * DP * 2;  // bytes of 128 rows
@@ -31,10 +40,10 @@ template <int DP> struct Cfg {
   // turns in one ring: with two places each (373 -> 238 us) the MMAs still waited 1000 of 4000 cycles a tile for keys.
   static constexpr uint32_t kStages = DP == 64 ? 8 : 5;
   struct Shared {  // behind the tiles
-    uint64_t q_full[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4], drained;
-    Place at;
-    uint32_t tmem, found;
-    volatile uint32_t failed;
+    uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4], item_full[2], item_empty[2], fetched, drained;
+    Item items[2];
+    uint32_t tmem;
+    volatile uint32_t failed, slow, slow_ended;  // slow: rows that are computed again at present, slow_ended: that have been
   };
   static constexpr uint32_t kSmem = (2 + kStages) * kTile + sizeof(Shared);
   static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA per SM");
@@ -111,6 +120,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
 // Sixteen columns times c.
 __device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
   uint32_t u[16];
@@ -125,209 +139,233 @@ __device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
 }
 
 template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
-    paged_prompt_tc_kernel(const PagedAttention p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t box) {
+    paged_prompt_tc_kernel(const PagedAttention p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const __grid_constant__ CUtensorMap map_q, const uint32_t box, const bool q_box) {
   using C = Cfg<DP>;
   extern __shared__ __align__(1024) unsigned char smem[];
   typename C::Shared &sh = *reinterpret_cast<typename C::Shared *>(smem + (2 + C::kStages) * C::kTile);
   auto &q_full = sh.q_full, &s_full = sh.s_full, &o_full = sh.o_full;
   auto &full = sh.full, &empty = sh.empty;
   auto &p_full = sh.p_full;
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = p.heads / p.kv_heads, tile = blockIdx.x / p.kv_heads, kvh = blockIdx.x - tile * p.kv_heads;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = p.heads / p.kv_heads;
   if (tid == 0) {
     auto init = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(bar)), "r"(n) : "memory"); };
     for (uint32_t s = 0; s < C::kStages; ++s) init(&full[s], 1), init(&empty[s], 1);
-    for (uint32_t i = 0; i < 2; ++i) init(&q_full[i], 4), init(&s_full[i], 1), init(&p_full[i][0], 4), init(&p_full[i][1], 4), init(&o_full[i], 1);
+    for (uint32_t i = 0; i < 2; ++i) init(&q_full[i], 1), init(&sh.q_empty[i], 1), init(&s_full[i], 1), init(&p_full[i][0], 4), init(&p_full[i][1], 4), init(&o_full[i], 1);
+    for (uint32_t i = 0; i < 2; ++i) init(&sh.item_full[i], 1), init(&sh.item_empty[i], kSoftmaxWarps + kFetchWarps + 1);
+    init(&sh.fetched, kFetchWarps);
     init(&sh.drained, 1);
-    sh.failed = 0;
     for (uint32_t i = 0; i < 8; ++i) init(&sh.turn[i >> 2][i & 3], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    sh.failed = sh.slow = sh.slow_ended = 0;
   }
   if (warp == kMmaWarp) tmem_alloc<512>(sa(&sh.tmem));
-  follow();
-  if (p.part != 2) stamp_begin(p.stamps);  // else the launch in front of this one did
-  if (warp == kMmaWarp + 1) {
-    Place found = {};
-    const bool there = find_tile(p, per, 2 * kRows, tile, found);
-    if (lane == 0) sh.at = found, sh.found = there;
-  } else if (warp == 0 && blockIdx.x == 0) {
-    check_rows(p);
-  }
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = sh.tmem;
-  if (!sh.found) {
-    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    return;
-  }
-  const Place &at = sh.at;
-  const uint32_t packed = at.fresh * per, past = at.len - at.fresh;
-  // per tile of rows: its rows that exist, and the tiles of positions [b, e) that they see
-  const bool both = at.first + kRows < packed;
-  uint32_t b[2], e[2];
-#pragma unroll
-  for (uint32_t i = 0; i < 2; ++i) {
-    const uint32_t r0 = at.first + (both ? i : 0) * kRows, r1 = min(r0 + kRows, packed), lo = past + r0 / per, hi = past + (r1 - 1) / per;
-    b[i] = (p.window && lo + 1 > p.window ? lo + 1 - p.window : 0) / kKeys;
-    e[i] = hi / kKeys + 1;
-  }
-  const uint32_t t0 = b[0], t1 = e[1], tiles = both ? 2 : 1;  // b and e grow with the rows
-  const uint32_t q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
-  // False when the wait ran out. The loop is one statement: its instructions are between every two steps of a tile.
-  auto wait = [&](uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
-        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
-        "there:\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(sa(bar)), "r"(parity), "n"(kPolls)
-        : "memory");
-    if (!ok) sh.failed = 1;
+  follow();
+  if (p.part != 2) stamp_begin(p.stamps);  // else the launch in front of this one did
+  const uint32_t tmem = sh.tmem, q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
+  // Waits, false when they ran out. A row that is computed again (below) may take longer than a wait's polls: as long as there is one, or was since
+  // the polls before, a wait goes on.
+  auto in_time = [&](auto poll) {
+    uint32_t ok = poll();
+    for (uint32_t seen = 0xffffffffu; !ok;) {
+      const uint32_t ended = sh.slow_ended;
+      if (!sh.slow && ended == seen) {
+        sh.failed = 1;
+        break;
+      }
+      seen = ended;
+      ok = poll();
+    }
     return ok != 0;
   };
+  // The loop is one statement: its instructions are between every two steps of a tile.
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    return in_time([&]() {
+      uint32_t ok;
+      asm volatile(
+          "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+          "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
+          "there:\n selp.u32 %0, 1, 0, p;\n}"
+          : "=r"(ok)
+          : "r"(sa(bar)), "r"(parity), "n"(kPolls)
+          : "memory");
+      return ok;
+    });
+  };
+  // For waits that are long by design: a warp that polls takes issue slots from the softmax warps of its scheduler (the ticket warp alone
+  // cost a third of the rate).
+  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns) {
+    const bool ok = in_time([&]() {
+      uint32_t ok = 0;
+      for (uint32_t n = 0; !ok && n < kPolls; ++n) {
+        asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(sa(bar)), "r"(parity) : "memory");
+        if (!ok) __nanosleep(ns);
+      }
+      return ok;
+    });
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
   auto wait_warp = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };  // the lanes agree
+
+  // Item k of this CTA; null when the wait ran out.
+  auto item = [&](uint32_t k) { return wait_warp(&sh.item_full[k & 1], k >> 1 & 1) ? &sh.items[k & 1] : nullptr; };
+  auto item_done = [&](uint32_t k) {
+    __syncwarp();
+    if (lane == 0) arrive(sa(&sh.item_empty[k & 1]));
+  };
+
+  if (warp < kSoftmaxWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
 
   if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------------------------------------------------- softmax
     const uint32_t i = warp >> 2, quad = warp & 3;
-    if (i < tiles) {
-      const uint32_t r = at.first + tid, w0 = min(at.first + warp * 32, packed - 1), w1 = min(w0 + 31, packed - 1);
-      const uint32_t pos = past + min(r, packed - 1) / per, w_lo = past + w0 / per, w_hi = past + w1 / per;
-      const uint32_t w_first = p.window && w_hi + 1 > p.window ? w_hi + 1 - p.window : 0;  // every row of the warp sees [w_first, w_lo]
-      const uint32_t first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
-      // the warp's 32 rows of Q, in the swizzle of the operand
-      {
-        constexpr uint32_t CH = DP / 8, RS = 32 / CH;  // pieces of a row; rows at a time
-        const uint32_t col = lane % CH, qr0 = at.first + warp * 32 + lane / CH, dst = q_a + i * C::kTile + (col >> 3) * (128 * 128);
-        const uint16_t *src = static_cast<const uint16_t *>(p.q), *mine = src + at.row0 * p.q_ld + kvh * per * p.dim + col * 8;
-#pragma unroll 8
-        for (uint32_t x = 0; x < 32 / RS; ++x) {
-          const uint32_t row = quad * 32 + x * RS + lane / CH, qr = qr0 + x * RS, rt = quotient(qr, p.group);
-          const bool there = qr < packed && col * 8 < p.dim;
-          copy16(dst + row * 128 + (((col & 7) ^ (row & 7)) << 4), there ? mine + rt * p.q_ld + (qr - rt * per) * p.dim : src, there);
-        }
-        copy_commit();
-        copy_wait<0>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive(sa(&q_full[i]));
-      }
-      const float scale = fabsf(p.scale) * kLog2e;  // a negative scale is the MMA's negated operand
-      const uint32_t lanes = (quad * 32u) << 16, s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * DP;
-      float top = -INFINITY, ref = 0.f, sum = 0.f;  // the reference, and what is subtracted from scaled scores (0 where it is -infinity)
-      bool ok = true;
-      uint32_t phase = 0;
-      const uint32_t bi = b[i], ei = e[i];
-      for (uint32_t t = bi; t < ei; ++t, phase ^= 1) {
-        if (!(ok = wait_warp(&s_full[i], phase))) break;
-        tc_after();
-        uint32_t u[128];
-        tmem_ld128(s_t, u);
-        if (t * kKeys + kKeys - 1 > w_lo) {  // positions that some row of the warp does not see yet
-          const int hi = (int)pos - (int)(t * kKeys);
+    uint32_t scores = 0, output = 0, turn = 0;  // parities of the barriers, over all items
+    bool ok = true;
+    for (uint32_t k = 0; ok; ++k) {
+      const Item *it = item(k);
+      if (!it || !it->found) break;
+      const Place at = it->at;
+      const uint32_t kvh = it->kvh, tiles = it->tiles, both_b = it->b[1], both_e = it->e[0];  // positions of both tiles, where there are two
+      if (i < tiles) {
+        const uint32_t packed = at.fresh * per, past = at.len - at.fresh, bi = it->b[i], ei = it->e[i];
+        const uint32_t r = at.first + tid, w0 = min(at.first + warp * 32, packed - 1), w1 = min(w0 + 31, packed - 1);
+        const uint32_t pos = past + quotient(min(r, packed - 1), p.group), w_lo = past + quotient(w0, p.group), w_hi = past + quotient(w1, p.group);
+        const uint32_t w_first = p.window && w_hi + 1 > p.window ? w_hi + 1 - p.window : 0;  // every row of the warp sees [w_first, w_lo]
+        const uint32_t first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
+        const float scale = fabsf(p.scale) * kLog2e;  // a negative scale is the MMA's negated operand
+        const uint32_t lanes = (quad * 32u) << 16, s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * DP;
+        float top = -INFINITY, ref = 0.f, sum = 0.f;  // the reference, and what is subtracted from scaled scores (0 where it is -infinity)
+        for (uint32_t t = bi; t < ei; ++t, scores ^= 1) {
+          if (!(ok = wait_warp(&s_full[i], scores))) break;
+          tc_after();
+          uint32_t u[128];
+          tmem_ld128(s_t, u);
+          if (t * kKeys + kKeys - 1 > w_lo) {  // positions that some row of the warp does not see yet
+            const int hi = (int)pos - (int)(t * kKeys);
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x > hi) u[x] = 0xff800000u;
-        }
-        if (t * kKeys < w_first) {  // and no more
-          const int lo = (int)first - (int)(t * kKeys);
+            for (int x = 0; x < 128; ++x)
+              if (x > hi) u[x] = 0xff800000u;
+          }
+          if (t * kKeys < w_first) {  // and no more
+            const int lo = (int)first - (int)(t * kKeys);
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x < lo) u[x] = 0xff800000u;
-        }
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int x = 0; x < 128; ++x)
+              if (x < lo) u[x] = 0xff800000u;
+          }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (uint32_t x = 0; x < 128; x += 8)
+          for (uint32_t x = 0; x < 128; x += 8)
 #pragma unroll
-          for (uint32_t y = 0; y < 4; ++y) m4[y] = max3(m4[y], __uint_as_float(u[x + y]), __uint_as_float(u[x + 4 + y]));
-        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        if (t == bi) {
-          top = m;
-          ref = m == -INFINITY ? 0.f : m * scale;
-        } else {
-          const bool grown = m * scale - ref > 8.0f || (top == -INFINITY && m != -INFINITY);
-          if (__any_sync(0xffffffffu, grown)) {
-            float c = 1.0f;
-            if (grown) {
-              c = exp2_fast((top - m) * scale);
-              top = m;
-              ref = m * scale;
-            }
-            sum *= c;
+            for (uint32_t y = 0; y < 4; ++y) m4[y] = max3(m4[y], __uint_as_float(u[x + y]), __uint_as_float(u[x + 4 + y]));
+          const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          if (t == bi) {
+            top = m;
+            ref = m == -INFINITY ? 0.f : m * scale;
+          } else {
+            const bool grown = m * scale - ref > 8.0f || (top == -INFINITY && m != -INFINITY);
+            if (__any_sync(0xffffffffu, grown)) {
+              float c = 1.0f;
+              if (grown) {
+                c = exp2_fast((top - m) * scale);
+                top = m;
+                ref = m * scale;
+              }
+              sum *= c;
 #pragma unroll 1
-            for (uint32_t d = 0; d < DP; d += 16) rescale16(o_t + d, c);
-            tmem_stored();
+              for (uint32_t d = 0; d < DP; d += 16) rescale16(o_t + d, c);
+              tmem_stored();
+            }
           }
-        }
-        // The special function unit of a scheduler belongs to one tile's warp at a time: the other's products run meanwhile.
-        const bool shared_tile = tiles == 2 && t >= b[1] && t < e[0];
-        if (shared_tile && (i || t > b[1])) {
-          if (!(ok = wait_warp(&sh.turn[i][quad], (t - b[1] - (i ^ 1)) & 1))) break;
-        }
-        const uint64_t scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
-        uint64_t sum2[2] = {0, 0};
+          // The special function unit of a scheduler belongs to one tile's warp at a time: the other's products run meanwhile.
+          const bool shared_tile = tiles == 2 && t >= both_b && t < both_e;
+          if (shared_tile && (i || t > both_b)) {
+            if (!(ok = wait_warp(&sh.turn[i][quad], turn))) break;
+            turn ^= 1;
+          }
+          const uint64_t scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
+          uint64_t sum2[2] = {0, 0};
 #pragma unroll
-        for (uint32_t c = 0; c < 4; ++c) {
-          uint32_t w[16];
+          for (uint32_t c = 0; c < 4; ++c) {
+            uint32_t w[16];
 #pragma unroll
-          for (uint32_t x = 0; x < 16; ++x) {
-            const uint64_t y = fma_pair(pair_of(__uint_as_float(u[c * 32 + 2 * x]), __uint_as_float(u[c * 32 + 2 * x + 1])), scale2, ref2);
-            const float2 v = of_pair(y);
-            const float a = exp2_fast(v.x), z = exp2_fast(v.y);
-            sum2[x & 1] = add_pair(sum2[x & 1], pair_of(a, z));
-            w[x] = pack2<BF>(a, z);
+            for (uint32_t x = 0; x < 16; ++x) {
+              const uint64_t y = fma_pair(pair_of(__uint_as_float(u[c * 32 + 2 * x]), __uint_as_float(u[c * 32 + 2 * x + 1])), scale2, ref2);
+              const float2 v = of_pair(y);
+              const float a = exp2_fast(v.x), z = exp2_fast(v.y);
+              sum2[x & 1] = add_pair(sum2[x & 1], pair_of(a, z));
+              w[x] = pack2<BF>(a, z);
+            }
+            tmem_st16(s_t + c * 16, w);
+            if (c == 1) {  // the product with the first 64 positions' values can begin
+              tmem_stored();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) arrive(sa(&p_full[i][0]));
+            }
           }
-          tmem_st16(s_t + c * 16, w);
-          if (c == 1) {  // the product with the first 64 positions' values can begin
-            tmem_stored();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) arrive(sa(&p_full[i][0]));
+          if (shared_tile && lane == 0) arrive(sa(&sh.turn[i ^ 1][quad]));
+          const float2 part = of_pair(add_pair(sum2[0], sum2[1]));
+          sum += part.x + part.y;
+          tmem_stored();
+          tc_before();
+          __syncwarp();
+          if (lane == 0) arrive(sa(&p_full[i][1]));
+        }
+        if (ok) ok = wait_warp(&o_full[i], output);
+        output ^= 1;
+        if (ok) {
+          tc_after();
+          const float inv = 1.0f / sum;
+          uint16_t *out = static_cast<uint16_t *>(p.out);
+          {
+            const uint32_t row = min(r, packed - 1), rt = quotient(row, p.group);
+            out += ((size_t)(at.row0 + rt) * p.heads + kvh * per + row - rt * per) * p.dim;
+          }
+          float finite = 0.f;
+#pragma unroll
+          for (uint32_t d = 0; d < DP; d += 32) {
+            uint32_t u[32], w[16];
+            tmem_ld32(o_t + d, u);
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) {
+              const float a = __uint_as_float(u[2 * x]) * inv, z = __uint_as_float(u[2 * x + 1]) * inv;
+              finite += a * 0.f + z * 0.f;
+              w[x] = pack2<BF>(a, z);
+            }
+            if (r < packed) {
+#pragma unroll
+              for (uint32_t x = 0; x < 32; x += 16) {  // whole sectors where rows begin at them
+                const uint32_t *v = w + x / 2;
+                if (p.dim % 16 == 0) {
+                  if (d + x < p.dim)
+                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + d + x), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                                 : "memory");
+                } else {
+                  if (d + x < p.dim) *reinterpret_cast<uint4 *>(out + d + x) = make_uint4(v[0], v[1], v[2], v[3]);
+                  if (d + x + 8 < p.dim) *reinterpret_cast<uint4 *>(out + d + x + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                }
+              }
+            }
+          }
+          uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f && r < packed);  // NaN
+          __syncwarp();
+          if (again) {
+            if (lane == 0) atomicAdd(const_cast<uint32_t *>(&sh.slow), 1u);
+            for (; again; again &= again - 1) {
+              row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
+              if (lane == 0) atomicAdd(const_cast<uint32_t *>(&sh.slow_ended), 1u);
+            }
+            if (lane == 0) atomicSub(const_cast<uint32_t *>(&sh.slow), 1u);
           }
         }
-        if (shared_tile && lane == 0) arrive(sa(&sh.turn[i ^ 1][quad]));
-        const float2 part = of_pair(add_pair(sum2[0], sum2[1]));
-        sum += part.x + part.y;
-        tmem_stored();
-        tc_before();
-        __syncwarp();
-        if (lane == 0) arrive(sa(&p_full[i][1]));
       }
-      if (ok && wait_warp(&o_full[i], 0)) {
-        tc_after();
-        const float inv = 1.0f / sum;
-        // through shared memory (the tile's queries are through), so that a row is stored by neighbouring lanes
-        constexpr uint32_t CH = DP / 8, RS = 32 / CH;
-        unsigned char *mine = smem + i * C::kTile + quad * 32 * DP * 2;
-        float finite = 0.f;
-#pragma unroll
-        for (uint32_t d = 0; d < DP; d += 32) {
-          uint32_t u[32];
-          tmem_ld32(o_t + d, u);
-#pragma unroll
-          for (uint32_t x = 0; x < 32; x += 8) {
-            float v[8];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) v[y] = __uint_as_float(u[x + y]) * inv;
-            finite += ((v[0] * 0.f + v[1] * 0.f) + (v[2] * 0.f + v[3] * 0.f)) + ((v[4] * 0.f + v[5] * 0.f) + (v[6] * 0.f + v[7] * 0.f));
-            *reinterpret_cast<uint4 *>(mine + lane * DP * 2 + ((((d + x) / 8) ^ (lane & 7)) << 4)) =
-                make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
-          }
-        }
-        __syncwarp();
-        const uint32_t col = lane % CH, qr0 = at.first + warp * 32 + lane / CH;
-        uint16_t *out = static_cast<uint16_t *>(p.out) + ((size_t)at.row0 * p.heads + kvh * per) * p.dim + col * 8;
-#pragma unroll 4
-        for (uint32_t x = 0; x < 32 / RS; ++x) {
-          const uint32_t row = x * RS + lane / CH, qr = qr0 + x * RS, rt = quotient(qr, p.group);
-          if (qr < packed && col * 8 < p.dim)
-            *reinterpret_cast<uint4 *>(out + ((size_t)rt * p.heads + qr - rt * per) * p.dim) = *reinterpret_cast<const uint4 *>(mine + row * DP * 2 + ((col ^ (row & 7)) << 4));
-        }
-        uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f && r < packed);  // NaN
-        __syncwarp();
-        for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
-      }
+      if (i == 0 && tiles == 2 && both_e > both_b) turn ^= 1;  // the other tile's last turn, which nobody waits for
+      item_done(k);
     }
   } else if (warp < kSoftmaxWarps + kFetchWarps) {
     // ------------------------------------------------------------------------------------- fetch: keys one warp, values the other
@@ -336,23 +374,9 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     const bool col_there = col * 8 < p.dim;
     const uint16_t *cache = static_cast<const uint16_t *>(values ? p.vcache : p.kcache);
     const CUtensorMap *map = values ? &map_v : &map_k;
-    const uint32_t j_first = p.window && past + at.first / per + 1 > p.window ? past + at.first / per + 1 - p.window : 0;
-    const uint32_t j_last = past + (min(at.first + 2 * kRows, packed) - 1) / per, len = at.len;
-    const uint32_t *pages = p.table + (size_t)at.seq * p.width;
-    auto cache_row = [&](uint32_t j) {  // of position j; behind the last one where there is none
-      const uint32_t n = quotient(j, p.page), page = __ldg(pages + n);
-      if (page < p.pages) return (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
-      raise(p.error, PAGED_BAD_PAGE);
-      return 0xffffffffu;
-    };
     // Of a tile, the boxes of rows that lie in one page and exist whole are tensor copies; what is left, and pages of which no eight rows
     // make a box, goes piece by piece. Positions that no row of the CTA sees count as zeros.
     const uint32_t boxes = box ? kKeys / box : 0, rows_all = p.pages * p.kv_heads * p.page.d;
-    uint32_t look_row = 0;
-    auto look_up = [&](uint32_t t) {  // lane x: box x of a tile
-      const uint32_t j = t * kKeys + lane * box;
-      if (lane < boxes && j + box > j_first && j + box <= len) look_row = cache_row(j);
-    };
     uint64_t *late = nullptr;  // pieces by cp.async are reported behind the next request
     auto landed = [&]() {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core may read them
@@ -360,51 +384,73 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) arrive(sa(late));
       late = nullptr;
     };
-    look_up(t0);
-    RingPos<(int)C::kStages> pos;  // tile t's keys are request 2 (t - t0), its values the one behind
+    RingPos<(int)C::kStages> pos;  // an item's tiles make requests in turn: keys, values, keys, ...
     if (values) pos.next();
     uint32_t x = values;
-    for (uint32_t t = t0; t < t1; ++t, x += 2, pos.next(), pos.next()) {
-      const uint32_t my_row = min(look_row, rows_all), j0 = t * kKeys;  // a row behind the cache reads as zeros
-      const uint32_t lo = box && j_first > j0 ? min((j_first - j0) / box, boxes) : 0, hi = max(box && len > j0 ? min((len - j0) / box, boxes) : 0, lo);
-      if (x >= C::kStages && !wait_warp(&empty[pos.s], pos.phase ^ 1)) break;
-      const uint32_t dst = ring_a + pos.s * C::kTile, bar = sa(&full[pos.s]);
-      const bool pieces = (hi - lo) * box < kKeys;
-      if (hi > lo) {
-        if (elect_one()) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((hi - lo) * box * DP * 2) : "memory");
-        for (uint32_t g = lo; g < hi; ++g) {
-          const uint32_t row = __shfl_sync(0xffffffffu, my_row, g);
-          if (elect_one()) {  // one lane, known to the compiler: copies from several lanes at once became a loop, 2000 cycles a tile
+    bool ok = true;
+    for (uint32_t k = 0; ok; ++k) {
+      const Item *it = item(k);
+      if (!it || !it->found) break;
+      const uint32_t packed = it->at.fresh * per, past = it->at.len - it->at.fresh, kvh = it->kvh, len = it->at.len, t0 = it->b[0], t1 = it->e[1];
+      const uint32_t lo_pos = past + quotient(it->at.first, p.group), j_first = p.window && lo_pos + 1 > p.window ? lo_pos + 1 - p.window : 0;
+      const uint32_t j_last = past + quotient(min(it->at.first + 2 * kRows, packed) - 1, p.group);
+      const uint32_t *pages = p.table + (size_t)it->at.seq * p.width;
+      auto cache_row = [&](uint32_t j) {  // of position j; behind the last one where there is none
+        const uint32_t n = quotient(j, p.page), page = __ldg(pages + n);
+        if (page < p.pages) return (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
+        raise(p.error, PAGED_BAD_PAGE);
+        return 0xffffffffu;
+      };
+      uint32_t look_row = 0;
+      auto look_up = [&](uint32_t t) {  // lane x: box x of a tile
+        const uint32_t j = t * kKeys + lane * box;
+        if (lane < boxes && j + box > j_first && j + box <= len) look_row = cache_row(j);
+      };
+      look_up(t0);
+      for (uint32_t t = t0; t < t1; ++t, x += 2, pos.next(), pos.next()) {
+        const uint32_t my_row = min(look_row, rows_all), j0 = t * kKeys;  // a row behind the cache reads as zeros
+        const uint32_t lo = box && j_first > j0 ? min((j_first - j0) / box, boxes) : 0, hi = max(box && len > j0 ? min((len - j0) / box, boxes) : 0, lo);
+        if (x >= C::kStages && !(ok = wait_idle(&empty[pos.s], pos.phase ^ 1, 64))) break;
+        const uint32_t dst = ring_a + pos.s * C::kTile, bar = sa(&full[pos.s]);
+        const bool pieces = (hi - lo) * box < kKeys;
+        if (hi > lo) {
+          if (elect_one()) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"((hi - lo) * box * DP * 2) : "memory");
+          for (uint32_t g = lo; g < hi; ++g) {
+            const uint32_t row = __shfl_sync(0xffffffffu, my_row, g);
+            if (elect_one()) {  // one lane, known to the compiler: copies from several lanes at once became a loop, 2000 cycles a tile
 #pragma unroll
-            for (uint32_t k = 0; k < BLOCKS; ++k) tma_load_2d(dst + k * (128 * 128) + g * box * 128, map, k * 64, row, bar);
+              for (uint32_t k = 0; k < BLOCKS; ++k) tma_load_2d(dst + k * (128 * 128) + g * box * 128, map, k * 64, row, bar);
+            }
           }
         }
-      }
-      if (pieces) {
+        if (pieces) {
 #pragma unroll 4
-        for (uint32_t i = 0; i < kKeys / RS; ++i) {
-          const uint32_t row = i * RS + frow, j = j0 + row;
-          if (row >= lo * box && row < hi * box) continue;
-          const uint32_t r = j >= j_first && j <= j_last ? cache_row(j) : 0xffffffffu;
-          const bool there = r != 0xffffffffu && col_there;
-          copy16(dst + (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), cache + (there ? (size_t)r * p.dim + col * 8 : 0), there);
+          for (uint32_t i = 0; i < kKeys / RS; ++i) {
+            const uint32_t row = i * RS + frow, j = j0 + row;
+            if (row >= lo * box && row < hi * box) continue;
+            const uint32_t r = j >= j_first && j <= j_last ? cache_row(j) : 0xffffffffu;
+            const bool there = r != 0xffffffffu && col_there;
+            copy16(dst + (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), cache + (there ? (size_t)r * p.dim + col * 8 : 0), there);
+          }
         }
+        copy_commit();
+        if (late) {
+          copy_wait<1>();
+          landed();
+        }
+        if (pieces) {
+          late = &full[pos.s];
+        } else {
+          __syncwarp();
+          if (lane == 0) arrive(bar);
+        }
+        if (t + 1 < t1) look_up(t + 1);
       }
-      copy_commit();
-      if (late) {
-        copy_wait<1>();
-        landed();
-      }
-      if (pieces) {
-        late = &full[pos.s];
-      } else {
-        __syncwarp();
-        if (lane == 0) arrive(bar);
-      }
-      if (t + 1 < t1) look_up(t + 1);
+      if (lane == 0) arrive(sa(&sh.fetched));
+      copy_wait<0>();
+      if (late) landed();
+      item_done(k);
     }
-    copy_wait<0>();
-    if (late) landed();
     if (sh.failed && lane == 0) {  // nothing may land when the CTA has gone
       for (uint32_t y = x > C::kStages ? x - C::kStages : 0; y < x; ++y)
         if ((y & 1) == values) mbar_wait_short(sa(&full[y % C::kStages]), y / C::kStages & 1);
@@ -417,53 +463,64 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q0 = desc_lo(q_a), k0 = desc_lo(ring_a);
       const uint32_t v0 = ((ring_a & 0x3FFFFu) >> 4) | (128u * 128 >> 4) << 16;  // 64 dimensions are 16 KB from the next 64
       bool ok = true;
-      uint32_t p_phase = 0;               // bit i
-      RingPos<(int)C::kStages> keys, vals;  // tile t's keys are request 2 t, its values 2 t + 1
+      uint32_t p_phase = 0, q_phase = 0;    // bit i, over all items
+      RingPos<(int)C::kStages> keys, vals;  // a tile's keys are an even request, its values the one behind
       vals.next();
-      // step n: output of tile t - 1, scores of tile t, for one tile of rows after the other
-      for (uint32_t n = 0; ok && n <= t1 - t0; ++n) {
-        const uint32_t t = t0 + n;
-        bool waited = false;
-        if (n > 0 && !(ok = wait(&full[vals.s], vals.phase))) break;
-        for (uint32_t i = 0; ok && i < tiles; ++i) {
-          if (n > 0 && t - 1 >= b[i] && t - 1 < e[i]) {
-            const uint32_t st = v0 + vals.s * (C::kTile >> 4), parity = p_phase >> i & 1;
-            p_phase ^= 1u << i;
+      for (uint32_t k = 0; ok; ++k) {
+        if (!(ok = wait(&sh.item_full[k & 1], k >> 1 & 1))) break;
+        const Item &it = sh.items[k & 1];
+        if (!it.found) break;
+        const uint32_t tiles = it.tiles, b[2] = {it.b[0], it.b[1]}, e[2] = {it.e[0], it.e[1]}, t0 = b[0], t1 = e[1];  // registers: the loops over i are unrolled
+        // step n: output of tile t - 1, scores of tile t, for one tile of rows after the other
+        for (uint32_t n = 0; ok && n <= t1 - t0; ++n) {
+          const uint32_t t = t0 + n;
+          bool waited = false;
+          if (n > 0 && !(ok = wait(&full[vals.s], vals.phase))) break;
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-              if (!(ok = wait(&p_full[i][half], parity))) break;
+          for (uint32_t i = 0; i < 2; ++i) {
+            if (!ok || i >= tiles) break;
+            if (n > 0 && t - 1 >= b[i] && t - 1 < e[i]) {
+              const uint32_t st = v0 + vals.s * (C::kTile >> 4), parity = p_phase >> i & 1;
+              p_phase ^= 1u << i;
+#pragma unroll
+              for (uint32_t half = 0; half < 2; ++half) {
+                if (!(ok = wait(&p_full[i][half], parity))) break;
+                tc_after();
+#pragma unroll
+                for (uint32_t k = half * 4; k < half * 4 + 4; ++k)
+                  mma_tmem(tmem + 256 + i * DP, tmem + i * 128 + k * 8, st + k * (2048 >> 4), idesc_o, k != 0 || t - 1 > b[i]);
+              }
+              if (!ok) break;
+              if (t == e[i]) mma_commit(sa(&o_full[i]));
+            }
+            if (n > 0 && i + 1 == tiles) mma_commit(sa(&empty[vals.s]));
+            if (t < t1 && t >= b[i] && t < e[i]) {
+              if (t == b[i]) {
+                if (!(ok = wait(&q_full[i], q_phase >> i & 1))) break;
+                q_phase ^= 1u << i;
+              }
+              if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;
+              waited = true;
               tc_after();
+              const uint32_t st = k0 + keys.s * (C::kTile >> 4), qi = q0 + i * (C::kTile >> 4);
 #pragma unroll
-              for (uint32_t k = half * 4; k < half * 4 + 4; ++k)
-                mma_tmem(tmem + 256 + i * DP, tmem + i * 128 + k * 8, st + k * (2048 >> 4), idesc_o, k != 0 || t - 1 > b[i]);
+              for (uint32_t k = 0; k < DP / 16; ++k) {
+                const uint32_t off = (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2;
+                mma_f16<1>(tmem + i * 128, qi + off, st + off, idesc_s, k != 0);
+              }
+              mma_commit(sa(&s_full[i]));
+              if (t + 1 == e[i]) mma_commit(sa(&sh.q_empty[i]));
             }
-            if (!ok) break;
-            if (t == e[i]) mma_commit(sa(&o_full[i]));
           }
-          if (n > 0 && i + 1 == tiles) mma_commit(sa(&empty[vals.s]));
-          if (t < t1 && t >= b[i] && t < e[i]) {
-            if (n == 0 || t == b[i]) {
-              if (!(ok = wait(&q_full[i], 0))) break;
-            }
-            if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;
-            waited = true;
-            tc_after();
-            const uint32_t st = k0 + keys.s * (C::kTile >> 4), qi = q0 + i * (C::kTile >> 4);
-#pragma unroll
-            for (uint32_t k = 0; k < DP / 16; ++k) {
-              const uint32_t off = (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2;
-              mma_f16<1>(tmem + i * 128, qi + off, st + off, idesc_s, k != 0);
-            }
-            mma_commit(sa(&s_full[i]));
+          if (!ok) break;
+          if (t < t1) {
+            if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;  // nobody sees it (between windows): still given back
+            mma_commit(sa(&empty[keys.s]));
+            keys.next(), keys.next();
           }
+          if (n > 0) vals.next(), vals.next();
         }
-        if (!ok) break;
-        if (t < t1) {
-          if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;  // nobody sees it (between windows): still given back
-          mma_commit(sa(&empty[keys.s]));
-          keys.next(), keys.next();
-        }
-        if (n > 0) vals.next(), vals.next();
+        arrive(sa(&sh.item_empty[k & 1]));
       }
       if (!ok) {  // nothing may be in work when the TMEM is given back
         mma_commit(sa(&sh.drained));
@@ -471,25 +528,107 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
+  } else {
+    // ------------------------------------------------------- what comes next, once all of this item is requested: a ticket taken earlier
+    // could have been another CTA's, which has nothing left to do (106 -> 158 us for a few long items)
+    if (blockIdx.x == 0) check_rows(p);
+    uint32_t used[2] = {};  // how often each tile's place for Q
+    Walk walk;
+    for (uint32_t k = 0;; ++k) {
+      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200)) break;
+      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200)) break;
+      uint32_t ticket = blockIdx.x;
+      if (k && lane == 0) ticket = gridDim.x + atomicAdd(p.tickets, 1u);
+      ticket = __shfl_sync(0xffffffffu, ticket, 0);
+      const uint32_t tile = ticket / p.kv_heads;  // all heads of a tile, then the next tile
+      Item it = {};
+      it.found = find_tile(p, per, 2 * kRows, tile, it.at, walk);
+      it.kvh = ticket - tile * p.kv_heads;
+      const uint32_t packed = it.at.fresh * per, past = it.at.len - it.at.fresh;
+      it.tiles = it.at.first + kRows < packed ? 2 : 1;
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {  // b and e grow with the rows; the second tile's stand for both where there is one
+        const uint32_t r0 = it.at.first + (it.tiles == 2 ? i : 0) * kRows, lo = past + quotient(r0, p.group), hi = past + quotient(min(r0 + kRows, packed) - 1, p.group);
+        it.b[i] = (p.window && lo + 1 > p.window ? lo + 1 - p.window : 0) / kKeys;
+        it.e[i] = hi / kKeys + 1;
+      }
+      if (lane == 0) sh.items[k & 1] = it;
+      __syncwarp();
+      if (lane == 0) arrive(sa(&sh.item_full[k & 1]));
+      if (!it.found) break;
+      // its queries: a tensor copy where a tile of packed rows is a box of rows and heads (what follows behind the sequence's rows comes along,
+      // and is not stored), else piece by piece
+      bool ok = true;
+      for (uint32_t i = 0; ok && i < it.tiles; ++i) {
+        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64))) break;
+        ++used[i];
+        const uint32_t dst = q_a + i * C::kTile, bar = sa(&q_full[i]), r0 = it.at.first + i * kRows;
+        if (q_box) {
+          if (elect_one()) {
+            asm volatile("mbarrier.arrive.expect_tx.relaxed.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::kTile) : "memory");
+#pragma unroll
+            for (uint32_t x = 0; x < DP / 64; ++x) tma_load_3d(dst + x * (128 * 128), &map_q, x * 64, it.kvh * per, it.at.row0 + quotient(r0, p.group), bar);
+          }
+          __syncwarp();
+        } else {
+          constexpr uint32_t CH = DP / 8, RS = 32 / CH;  // pieces of a row; rows at a time
+          const uint32_t col = lane % CH;
+          const uint16_t *src = static_cast<const uint16_t *>(p.q), *mine = src + it.at.row0 * p.q_ld + it.kvh * per * p.dim + col * 8;
+#pragma unroll 4
+          for (uint32_t row = lane / CH; row < kRows; row += RS) {
+            const uint32_t qr = r0 + row, rt = quotient(qr, p.group);
+            const bool there = qr < packed && col * 8 < p.dim;
+            copy16(dst + (col >> 3) * (128 * 128) + row * 128 + (((col & 7) ^ (row & 7)) << 4), there ? mine + rt * p.q_ld + (qr - rt * per) * p.dim : src, there);
+          }
+          copy_commit();
+          copy_wait<0>();
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive(bar);
+        }
+      }
+      if (!ok) break;
+    }
+    if (sh.failed && lane == 0) {  // nothing may land when the CTA has gone
+      for (uint32_t i = 0; i < 2; ++i)
+        if (used[i]) mbar_wait_short(sa(&q_full[i]), used[i] + 1 & 1);
+    }
   }
   tc_before();
   __syncthreads();
   tc_after();
   if (tid == 0 && sh.failed) raise(p.error, kWaitCode);
   stamp_end(p.stamps);
+  if (tid == 0) {
+    __threadfence();
+    if (atomicAdd(p.tickets + 1, 1u) + 1 == gridDim.x) p.tickets[0] = p.tickets[1] = 0;
+  }
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-template <bool BF, int DP> cudaError_t run(const PagedAttention &p, cudaStream_t s) {
+// Queries as [rows, heads, dim]: boxes of 64 dimensions, a group's heads and as many rows as make up a tile. False where they cannot be mapped.
+template <bool BF> bool make_q_map(CUtensorMap *map, const PagedAttention &p, uint32_t per) {
+  EncodeTiled enc = encode_tiled();
+  const cuuint64_t dims[3] = {p.dim, p.heads, p.rows}, strides[2] = {(cuuint64_t)p.dim * 2, (cuuint64_t)p.q_ld * 2};
+  const cuuint32_t boxes[3] = {64, per, kRows / per}, steps[3] = {1, 1, 1};
+  return enc && enc(map, BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(p.q), dims, strides, boxes, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+template <bool BF, int DP> cudaError_t run(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
   const uint64_t per = p.heads / p.kv_heads, tiles = p.rows * per / (2 * kRows) + std::min<uint64_t>(p.n, p.rows * per);
   const uint64_t cache_rows = (uint64_t)p.pages * p.kv_heads * p.page.d;
-  CUtensorMap map_k = {}, map_v = {};
+  CUtensorMap map_k = {}, map_v = {}, map_q = {};
   uint32_t box = kKeys;  // the most rows, a power of two, of which pages consist; coordinates are signed
   while (p.page.d % box) box /= 2;
   if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) || !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF)) box = 0;
-  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)(tiles * p.kv_heads)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, box);
+  const bool q_box = kRows % per == 0 && make_q_map<BF>(&map_q, p, (uint32_t)per);
+  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)std::min<uint64_t>(sms, tiles * p.kv_heads)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
+  cudaFuncAttributes a;
+  const cudaError_t e = cudaFuncGetAttributes(&a, paged_prompt_tc_kernel<BF, DP>);
+  if (e != cudaSuccess) return e;
+  if (a.numRegs * kThreads < kLaunchRegs) return cudaErrorInvalidConfiguration;  // the softmax warps would wait for registers that nobody has
   return cudaFuncSetAttribute(paged_prompt_tc_kernel<BF, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);
 }
 
@@ -500,9 +639,9 @@ cudaError_t setup_paged_prompt_tc() {
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
-cudaError_t launch_paged_prompt_tc(const PagedAttention &p, cudaStream_t s) {
-  if (p.dim <= 64) return p.bf ? run<true, 64>(p, s) : run<false, 64>(p, s);
-  return p.bf ? run<true, 128>(p, s) : run<false, 128>(p, s);
+cudaError_t launch_paged_prompt_tc(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
+  if (p.dim <= 64) return p.bf ? run<true, 64>(p, sms, s) : run<false, 64>(p, sms, s);
+  return p.bf ? run<true, 128>(p, sms, s) : run<false, 128>(p, sms, s);
 }
 
 }  // namespace vkl

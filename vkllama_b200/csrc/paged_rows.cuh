@@ -35,12 +35,17 @@ __device__ __forceinline__ uint32_t rows_here(const PagedAttention &p, uint32_t 
 }
 
 // The place of tile `index` when every sequence has ceil(new * per / rows) of them, by one warp; false beyond the last. What takes longest
-// comes first: a sequence's last tiles, which see most, and of up to 32 sequences the longest.
-__device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint32_t index, Place &at) {
+// comes first: a sequence's last tiles, which see most, and of up to 32 sequences the longest. A later search for a tile further on goes on where
+// this one ended.
+struct Walk {
+  uint32_t from = 0;    // sequences in front, a multiple of 32
+  uint64_t before = 0;  // their tiles
+};
+__device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint32_t index, Place &at, Walk &walk) {
   const uint32_t lane = threadIdx.x & 31;
   bool bad = false;
-  uint64_t before = 0;
-  for (uint32_t i0 = 0; i0 < p.n; i0 += 32) {
+  uint64_t &before = walk.before;
+  for (uint32_t &i0 = walk.from; i0 < p.n; i0 += 32) {
     const uint32_t i = i0 + lane, fresh = i < p.n ? rows_here(p, i, per, bad) : 0;
     const uint64_t mine = ((uint64_t)fresh * per + rows - 1) / rows;
     uint64_t up = mine;  // and all of the chunk's sequences that come before
