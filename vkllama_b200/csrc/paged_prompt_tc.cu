@@ -24,7 +24,7 @@ namespace {
 
 constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // more than 12 warps would have 128 registers each
 constexpr uint32_t kRows = 128, kKeys = 128;
-constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20;
+constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20, kRounds = 64;
 // Registers of a thread: a softmax thread has a row of scores in registers, the other warps give theirs. The sum has to be below what the launch has.
 constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80, kLaunchRegs = kSoftmaxWarps * 32 * kSoftmaxRegs + (kThreads - kSoftmaxWarps * 32) * kOtherRegs;
 
@@ -43,7 +43,7 @@ template <int DP> struct Cfg {
     uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4], item_full[2], item_empty[2], fetched, drained;
     Item items[2];
     uint32_t tmem;
-    volatile uint32_t failed, slow, slow_ended;  // slow: rows that are computed again at present, slow_ended: that have been
+    volatile uint32_t failed, slow;  // slow: rows have been computed again
   };
   static constexpr uint32_t kSmem = (2 + kStages) * kTile + sizeof(Shared);
   static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA per SM");
@@ -157,7 +157,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     init(&sh.drained, 1);
     for (uint32_t i = 0; i < 8; ++i) init(&sh.turn[i >> 2][i & 3], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    sh.failed = sh.slow = sh.slow_ended = 0;
+    sh.failed = sh.slow = 0;
   }
   if (warp == kMmaWarp) tmem_alloc<512>(sa(&sh.tmem));
   tc_before();
@@ -166,46 +166,31 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   follow();
   if (p.part != 2) stamp_begin(p.stamps);  // else the launch in front of this one did
   const uint32_t tmem = sh.tmem, q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
-  // Waits, false when they ran out. A row that is computed again (below) may take longer than a wait's polls: as long as there is one, or was since
-  // the polls before, a wait goes on.
-  auto in_time = [&](auto poll) {
-    uint32_t ok = poll();
-    for (uint32_t seen = 0xffffffffu; !ok;) {
-      const uint32_t ended = sh.slow_ended;
-      if (!sh.slow && ended == seen) {
-        sh.failed = 1;
-        break;
-      }
-      seen = ended;
-      ok = poll();
-    }
-    return ok != 0;
-  };
-  // The loop is one statement: its instructions are between every two steps of a tile.
+  // Waits, false when they ran out: after kPolls, or after kRounds times as many in a CTA that has computed rows again (below), which takes as long as it
+  // takes. The loop is one statement, with nothing behind a wait that is over: these instructions are between every two steps of a tile (checks in C++
+  // behind it: 108 us where 103 are possible).
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    return in_time([&]() {
-      uint32_t ok;
-      asm volatile(
-          "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
-          "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
-          "there:\n selp.u32 %0, 1, 0, p;\n}"
-          : "=r"(ok)
-          : "r"(sa(bar)), "r"(parity), "n"(kPolls)
-          : "memory");
-      return ok;
-    });
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p, q;\n .reg .u32 n, m;\n mov.u32 n, %3;\n"
+        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n and.b32 m, n, %4;\n setp.ne.u32 q, m, 0;\n @q bra again;\n"
+        " ld.volatile.shared.u32 m, [%5];\n setp.eq.u32 q, m, 0;\n @q bra there;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
+        "there:\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(sa(bar)), "r"(parity), "n"(kPolls * kRounds), "n"(kPolls - 1), "r"(sa(const_cast<uint32_t *>(&sh.slow)))
+        : "memory");
+    if (!ok) sh.failed = 1;
+    return ok != 0;
   };
   // For waits that are long by design: a warp that polls takes issue slots from the softmax warps of its scheduler (the ticket warp alone
   // cost a third of the rate).
   auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns) {
-    const bool ok = in_time([&]() {
-      uint32_t ok = 0;
-      for (uint32_t n = 0; !ok && n < kPolls; ++n) {
-        asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(sa(bar)), "r"(parity) : "memory");
-        if (!ok) __nanosleep(ns);
-      }
-      return ok;
-    });
+    uint32_t ok = 0;
+    for (uint32_t n = 0; !ok && n < (sh.slow ? kPolls * kRounds : kPolls); ++n) {
+      asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(sa(bar)), "r"(parity) : "memory");
+      if (!ok) __nanosleep(ns);
+    }
+    if (!ok) sh.failed = 1;
     return __all_sync(0xffffffffu, ok) != 0;
   };
   auto wait_warp = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };  // the lanes agree
@@ -354,14 +339,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
           }
           uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f && r < packed);  // NaN
           __syncwarp();
-          if (again) {
-            if (lane == 0) atomicAdd(const_cast<uint32_t *>(&sh.slow), 1u);
-            for (; again; again &= again - 1) {
-              row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
-              if (lane == 0) atomicAdd(const_cast<uint32_t *>(&sh.slow_ended), 1u);
-            }
-            if (lane == 0) atomicSub(const_cast<uint32_t *>(&sh.slow), 1u);
-          }
+          if (again) sh.slow = 1;
+          for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
         }
       }
       if (i == 0 && tiles == 2 && both_e > both_b) turn ^= 1;  // the other tile's last turn, which nobody waits for
