@@ -23,10 +23,11 @@ __device__ __forceinline__ uint32_t fresh_rows(const PagedAttention &p, uint32_t
   return 0;
 }
 
-// Which kernel takes a sequence: tcgen05 (part 2) where its tiles of 256 packed rows are filled far enough or there are many positions to see, the
-// tiles of 64 on mma.sync (part 1) else. us, 32 heads of 128, mma.sync / tcgen05: 8 prompts of 64 12.4 / 24.3, of 128 22.8 / 18.3; 4 times 64 rows behind
-// 2000 106 / 41; 32 drafts of 5 rows, 8 key heads, behind 1000 69 / 47.
-constexpr uint32_t kTensorRows = 96, kTensorLength = 512;
+// Which kernel takes a sequence: tcgen05 (part 2) where it has more packed rows than a tile of the other, or a tile of 128 positions to see; the tiles of
+// 64 rows on mma.sync (part 1), three CTAs to an SM, else. us, 32 heads of 128, mma.sync / tcgen05: 64 prompts of 32 52 / 65, of 64 67 / 65, of 96
+// 119 / 67; 8 prompts of 64 12.3 / 14.4, of 80 22.4 / 14.5; 64 drafts of 2 rows behind 100 63 / 72, behind 400 150 / 128; 8 drafts of 5, 8 key heads,
+// behind 100 10.9 / 9.3, behind 600 28.7 / 16.5.
+constexpr uint32_t kTensorRows = 65, kTensorLength = 128;
 __device__ __forceinline__ uint32_t rows_here(const PagedAttention &p, uint32_t i, uint32_t per, bool &bad) {
   const uint32_t fresh = fresh_rows(p, i, bad);
   if (p.part == 0) return fresh;
