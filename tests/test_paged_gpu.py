@@ -302,12 +302,39 @@ def test_whole_tiles_of_rows(dev, dtype, past, new, heads, kv, dim, page, window
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_call_with_sequences_for_either_kernel(dev, dtype):
-    """A few rows behind many positions and behind few, prompts short and long: two launches share the sequences."""
+    """A few rows behind many positions and behind few, prompts short and long: two launches share the sequences, and a third joins the parts of the
+    one whose positions are split."""
     before = vk.kernel_launches()
     prompt(dev, [2000, 0, 600, 0, 510, 511, 0, 30], [3, 40, 1, 130, 1, 1, 0, 66], 2, 2, 64, 16, dtype, behind=2)
-    assert vk.kernel_launches() - before == 4
+    assert vk.kernel_launches() - before == 6
     prompt(dev, [700, 3, 900], [2, 2, 7], 12, 2, 128, 8, dtype, window=600)
     prompt(dev, [700, 3, 900], [2, 2, 7], 4, 2, 200, 8, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("past,new,heads,kv,dim,page,window", [
+    ([5000], [5], 8, 2, 128, 16, 0), ([3000, 10, 700, 0], [3, 20, 1, 0], 4, 1, 64, 32, 0), ([2500], [200], 4, 2, 128, 16, 0), ([4000], [130], 2, 2, 80, 24, 1500),
+    ([2000], [300], 1, 1, 96, 5, 0), ([1100, 1100], [64, 2], 6, 2, 40, 64, 600), ([20000], [1], 5, 1, 128, 16, 0), ([1023], [1], 128, 1, 64, 128, 0), ([1022, 1024], [257, 255], 1, 1, 16, 8, 0)])
+def test_positions_are_split_where_there_are_few_rows(dev, dtype, past, new, heads, kv, dim, page, window):
+    """Slices of four tiles and more, sequences with one slice beside ones with many, windows that begin inside one."""
+    prompt(dev, past, new, heads, kv, dim, page, dtype, window, behind=3, wide=8)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_and_missing_numbers_in_a_slice(dev, dim):
+    for dtype in DTYPES:
+        inf, nan = (0x7c00, 0x7e00) if dtype == vk.FP16 else (0x7f80, 0x7fc0)
+        for window in (0, 1000):
+            c = Cache(np.random.default_rng(12), [4000, 60], 1, dim, 16, dtype)
+            c.seq_v[0][0, 700, 3], c.seq_v[0][0, 3500, 5], c.seq_v[0][0, 3998, 7], c.seq_k[1][0, 59] = nan, inf, nan, inf
+            for i in (0, 1):
+                c.put(c.v, i, c.seq_v[i])
+                c.put(c.k, i, c.seq_k[i])
+            got = prompt(dev, [3996, 56], [4, 4], 3, 1, dim, 16, dtype, window, cache=c, finite=False)
+            for r in range(4):  # positions 3996 ...
+                assert np.isnan(got[r, :, 3]).all() == (not window) and np.isposinf(got[r, :, 5]).all() and np.isnan(got[r, :, 7]).all() == (r >= 2)
+                assert np.isfinite(np.delete(got[r], [3, 5, 7], 1)).all()
+            assert np.isfinite(got[4:7]).all() and not np.isfinite(got[7]).any()
 
 
 def test_many_short_prompts_and_a_long_one(dev):

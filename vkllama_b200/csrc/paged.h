@@ -111,6 +111,8 @@ struct PagedAttention {
   float *scratch;               // partial results, paged_token_scratch() bytes
   uint32_t *counters;           // [SMs + 1], 0 between launches
   uint32_t *tickets;            // [2], 0 between launches
+  float *part_o;                // prompts whose positions are split: [splits][rows][heads][64 or 128] sums of parts
+  float2 *part_ml;              // and [splits][rows][heads] references and sums of probabilities, 0 between calls
   unsigned long long *stamps;
   uint32_t *error;
   uint64_t q_ld;
@@ -118,6 +120,7 @@ struct PagedAttention {
   Divisor page, group;          // query heads of a key head
   float scale;                  // on the scores
   bool bf;
+  uint32_t splits;              // parts of a sequence's positions at most
   uint32_t part;                // of a prompt call's sequences, those that the launch takes: 0 all, 1 or 2 by paged_rows.cuh's rule
 };
 // One new token per sequence.
@@ -129,7 +132,9 @@ uint32_t paged_prompt_launches(const PagedAttention &p);
 cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStream_t s);
 cudaError_t setup_paged_prompt();
 // The same on tcgen05, heads up to 128 wide.
+uint32_t paged_prompt_splits(const PagedAttention &p, uint32_t sms);
 cudaError_t launch_paged_prompt_tc(const PagedAttention &p, uint32_t sms, cudaStream_t s);
+cudaError_t launch_paged_prompt_join(const PagedAttention &p, cudaStream_t s);  // where splits > 1, behind it
 cudaError_t setup_paged_prompt_tc();
 
 }  // namespace vkl

@@ -231,11 +231,11 @@ struct UpdatePagedOp : PagedOp {
 struct PagedAttentionOp : PagedOp {
   int heads, kv_heads, dim, page, window, dtype;
   float scale;
-  vkl_tensor *out = nullptr, *scratch = nullptr, *counters = nullptr;
+  vkl_tensor *out = nullptr, *scratch = nullptr, *counters = nullptr, *part_o = nullptr, *part_ml = nullptr;
   PagedAttentionOp(vkl_device *d, vkl_command *c, int h, int kv, int dm, int pg, float s, int w, int dt)
       : PagedOp(d, c), heads(h), kv_heads(kv), dim(dm), page(pg), window(w), dtype(dt), scale(s) {}
   ~PagedAttentionOp() override {
-    for (vkl_tensor *t : {out, scratch, counters}) vkl_tensor_release(t);
+    for (vkl_tensor *t : {out, scratch, counters, part_o, part_ml}) vkl_tensor_release(t);
   }
   int init() override {
     if (inited) return VKL_OK;
@@ -294,6 +294,16 @@ struct PagedAttentionOp : PagedOp {
       p.group = divisor((uint32_t)per);
       p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
       p.bf = dtype == VKL_BF16;
+      p.splits = starts ? paged_prompt_splits(p, sms) : 1;
+      if (p.splits > 1) {
+        const size_t parts = p.splits * rows * heads;
+        if (!part_o || part_o->w < parts * (dim <= 64 ? 64 : 128)) VKL_OKAY(ensure_tensor(dev, &part_o, 1, 1, parts * (dim <= 64 ? 64 : 128), VKL_FP32));
+        if (!part_ml || part_ml->w < parts * 2) {
+          VKL_OKAY(ensure_tensor(dev, &part_ml, 1, 1, parts * 2, VKL_FP32));
+          VKL_CUDA(cudaMemsetAsync(part_ml->data(), 0, parts * 8, cmd->stream));
+        }
+        p.part_o = (float *)part_o->data(), p.part_ml = (float2 *)part_ml->data();
+      }
       VKL_LAUNCH(starts ? paged_prompt_launches(p) : 1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
     }
     *o = out;

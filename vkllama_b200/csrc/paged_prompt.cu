@@ -228,17 +228,20 @@ cudaError_t setup_paged_prompt() {
 // sequences that are its own (the second finds nothing to do in 2 to 3 us).
 uint32_t paged_prompt_launches(const PagedAttention &p) {
   const bool many = (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n;
-  return p.dim > 128 || many || p.width * p.page.d < kTensorLength ? 1 : 2;
+  return (p.dim > 128 || many || p.width * p.page.d < kTensorLength ? 1 : 2) + (p.splits > 1);
 }
 cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
   const bool many = (uint64_t)p.rows * (p.heads / p.kv_heads) >= (uint64_t)kTensorRows * p.n;
-  if (paged_prompt_launches(p) == 1) return p.dim <= 128 && many ? launch_paged_prompt_tc(p, sms, s) : p.bf ? pick<true>(p, s) : pick<false>(p, s);
+  const uint32_t launches = paged_prompt_launches(p) - (p.splits > 1);
+  const bool tensor = p.dim <= 128 && many;
   PagedAttention q = p;
-  q.part = 1;
-  const cudaError_t e = p.bf ? pick<true>(q, s) : pick<false>(q, s);
-  if (e != cudaSuccess) return e;
-  q.part = 2;
-  return launch_paged_prompt_tc(q, sms, s);
+  if (launches == 2) q.part = 1;
+  cudaError_t e = cudaSuccess;
+  if (launches == 2 || !tensor) e = p.bf ? pick<true>(q, s) : pick<false>(q, s);
+  if (launches == 2) q.part = 2;
+  if (e == cudaSuccess && (launches == 2 || tensor)) e = launch_paged_prompt_tc(q, sms, s);
+  if (e == cudaSuccess && p.splits > 1) e = launch_paged_prompt_join(p, s);
+  return e;
 }
 
 }  // namespace vkl

@@ -25,6 +25,9 @@ namespace {
 constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // more than 12 warps would have 128 registers each
 constexpr uint32_t kRows = 128, kKeys = 128;
 constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20, kRounds = 64;
+// Where there are fewer items than SMs, an item's positions are split, into slices of at least kSliceTiles tiles; the sums of a row's slices meet
+// in a kernel of their own.
+constexpr uint32_t kSliceTiles = 4, kMostSplits = 32;
 // Registers of a thread: a softmax thread has a row of scores in registers, the other warps give theirs. The sum has to be below what the launch has.
 constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80, kLaunchRegs = kSoftmaxWarps * 32 * kSoftmaxRegs + (kThreads - kSoftmaxWarps * 32) * kOtherRegs;
 
@@ -32,6 +35,7 @@ constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80, kLaunchRegs = kSoftmaxWa
 struct Item {
   Place at;
   uint32_t found, kvh, tiles, b[2], e[2];
+  uint32_t slice, slices;  // of the tiles of positions, this one's and how many
 };
 
 template <int DP> struct Cfg {
@@ -123,6 +127,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void store32(void *to, const uint32_t *v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
 // Sixteen columns times c.
@@ -304,13 +312,24 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
         output ^= 1;
         if (ok) {
           tc_after();
-          const float inv = 1.0f / sum;
-          uint16_t *out = static_cast<uint16_t *>(p.out);
-          {
-            const uint32_t row = min(r, packed - 1), rt = quotient(row, p.group);
-            out += ((size_t)(at.row0 + rt) * p.heads + kvh * per + row - rt * per) * p.dim;
-          }
+          const float inv = it->slices == 1 ? 1.0f / sum : 1.0f;
+          const uint32_t row = min(r, packed - 1), rt = quotient(row, p.group);
+          const size_t to = (size_t)(at.row0 + rt) * p.heads + kvh * per + row - rt * per;
+          uint16_t *out = static_cast<uint16_t *>(p.out) + to * p.dim;
           float finite = 0.f;
+          if (it->slices > 1) {  // a part of the row's positions
+            const size_t part = (size_t)it->slice * p.rows * p.heads + to;
+            if (r < packed) p.part_ml[part] = make_float2(ref, sum == 0.f ? -1.f : sum);  // 0 is a part that there is not
+#pragma unroll
+            for (uint32_t d = 0; d < DP; d += 32) {
+              uint32_t u[32];
+              tmem_ld32(o_t + d, u);
+              if (r < packed) {
+#pragma unroll
+                for (uint32_t x = 0; x < 32; x += 8) store32(p.part_o + part * DP + d + x, u + x);
+              }
+            }
+          } else
 #pragma unroll
           for (uint32_t d = 0; d < DP; d += 32) {
             uint32_t u[32], w[16];
@@ -326,10 +345,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
               for (uint32_t x = 0; x < 32; x += 16) {  // whole sectors where rows begin at them
                 const uint32_t *v = w + x / 2;
                 if (p.dim % 16 == 0) {
-                  if (d + x < p.dim)
-                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + d + x), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
-                                 "r"(v[5]), "r"(v[6]), "r"(v[7])
-                                 : "memory");
+                  if (d + x < p.dim) store32(out + d + x, v);
                 } else {
                   if (d + x < p.dim) *reinterpret_cast<uint4 *>(out + d + x) = make_uint4(v[0], v[1], v[2], v[3]);
                   if (d + x + 8 < p.dim) *reinterpret_cast<uint4 *>(out + d + x + 8) = make_uint4(v[4], v[5], v[6], v[7]);
@@ -520,24 +536,40 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     if (blockIdx.x == 0) check_rows(p);
     uint32_t used[2] = {};  // how often each tile's place for Q
     Walk walk;
+    uint32_t ticket = blockIdx.x;  // the first ones are dealt out
+    auto take = [&]() {
+      uint32_t next = 0;
+      if (lane == 0) next = gridDim.x + atomicAdd(p.tickets, 1u);
+      return __shfl_sync(0xffffffffu, next, 0);
+    };
     for (uint32_t k = 0;; ++k) {
       if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200)) break;
       if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200)) break;
-      uint32_t ticket = blockIdx.x;
-      if (k && lane == 0) ticket = gridDim.x + atomicAdd(p.tickets, 1u);
-      ticket = __shfl_sync(0xffffffffu, ticket, 0);
-      const uint32_t tile = ticket / p.kv_heads;  // all heads of a tile, then the next tile
+      if (k) ticket = take();
       Item it = {};
-      it.found = find_tile(p, per, 2 * kRows, tile, it.at, walk);
-      it.kvh = ticket - tile * p.kv_heads;
-      const uint32_t packed = it.at.fresh * per, past = it.at.len - it.at.fresh;
-      it.tiles = it.at.first + kRows < packed ? 2 : 1;
+      for (;; ticket = take()) {
+        const uint32_t head = ticket / p.splits, tile = head / p.kv_heads;  // all heads of a tile, then the next tile
+        it.found = find_tile(p, per, 2 * kRows, tile, it.at, walk);
+        it.kvh = head - tile * p.kv_heads;
+        it.slice = ticket - head * p.splits;
+        const uint32_t packed = it.at.fresh * per, past = it.at.len - it.at.fresh;
+        it.tiles = it.at.first + kRows < packed ? 2 : 1;
 #pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {  // b and e grow with the rows; the second tile's stand for both where there is one
-        const uint32_t r0 = it.at.first + (it.tiles == 2 ? i : 0) * kRows, lo = past + quotient(r0, p.group), hi = past + quotient(min(r0 + kRows, packed) - 1, p.group);
-        it.b[i] = (p.window && lo + 1 > p.window ? lo + 1 - p.window : 0) / kKeys;
-        it.e[i] = hi / kKeys + 1;
+        for (uint32_t i = 0; i < 2; ++i) {  // b and e grow with the rows, by one at most; the second tile's stand for both where there is one
+          const uint32_t r0 = it.at.first + (it.tiles == 2 ? i : 0) * kRows, lo = past + quotient(r0, p.group), hi = past + quotient(min(r0 + kRows, packed) - 1, p.group);
+          it.b[i] = (p.window && lo + 1 > p.window ? lo + 1 - p.window : 0) / kKeys;
+          it.e[i] = hi / kKeys + 1;
+        }
+        const uint32_t t0 = it.b[0], all = it.e[1] - t0;
+        it.slices = max(min(p.splits, all / kSliceTiles), 1u);
+        if (!it.found) break;
+        if (it.slice >= it.slices) continue;
+        const uint32_t s0 = t0 + it.slice * all / it.slices, s1 = t0 + (it.slice + 1) * all / it.slices;
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) it.b[i] = max(it.b[i], s0), it.e[i] = min(it.e[i], s1);
+        break;
       }
+      const uint32_t packed = it.at.fresh * per;
       if (lane == 0) sh.items[k & 1] = it;
       __syncwarp();
       if (lane == 0) arrive(sa(&sh.item_full[k & 1]));
@@ -592,6 +624,66 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// One row and head of a call whose positions were split, by a warp: lane s has slice s.
+template <bool BF, int DP> __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const PagedAttention p) {
+  const uint32_t lane = threadIdx.x & 31, per = p.heads / p.kv_heads;
+  const size_t to = (size_t)blockIdx.x * 8 + threadIdx.x / 32, all = (size_t)p.rows * p.heads;
+  follow();
+  if (to < all) {
+    float2 ml = {0.f, 0.f};
+    if (lane < p.splits) {
+      ml = p.part_ml[lane * all + to];
+      if (ml.y != 0.f) p.part_ml[lane * all + to] = make_float2(0.f, 0.f);
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    if (there) {  // else the row was not split, or belongs to no sequence
+      const bool seen = ml.y != 0.f && ml.y != -1.f;
+      const uint32_t use = __ballot_sync(0xffffffffu, seen);
+      const float top = warp_max(seen ? ml.x : -INFINITY), w = seen ? exp2f(ml.x - top) : 0.f, inv = 1.0f / warp_sum(seen ? w * ml.y : 0.f);
+      float v[DP / 32] = {};  // dimensions lane * DP / 32 ...
+#pragma unroll 4
+      for (uint32_t s = 0; s < p.splits; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        if (!(use >> s & 1)) continue;
+        const float *src = p.part_o + (s * all + to) * DP + lane * (DP / 32);
+#pragma unroll
+        for (int d = 0; d < DP / 32; d += 2) {
+          const float2 x = *reinterpret_cast<const float2 *>(src + d);
+          v[d] += ws * x.x, v[d + 1] += ws * x.y;
+        }
+      }
+      float finite = 0.f;
+      uint16_t *out = static_cast<uint16_t *>(p.out) + to * p.dim + lane * (DP / 32);
+#pragma unroll
+      for (int d = 0; d < DP / 32; d += 2) {
+        if (lane * (DP / 32) + d >= p.dim) continue;
+        const float a = v[d] * inv, b = v[d + 1] * inv;
+        finite += a * 0.f + b * 0.f;
+        *reinterpret_cast<uint32_t *>(out + d) = pack2<BF>(a, b);
+      }
+      if (__any_sync(0xffffffffu, finite != 0.f)) {  // NaN
+        const uint32_t row = (uint32_t)(to / p.heads), head = (uint32_t)(to - (size_t)row * p.heads), kvh = head / per;
+        uint32_t lo = 0, hi = p.n;  // the last sequence that begins at or in front of the row: the one that has it, for it was computed
+        while (hi - lo > 1) {
+          const uint32_t mid = (lo + hi) / 2;
+          if (p.starts[mid] <= row) lo = mid;
+          else hi = mid;
+        }
+        bool bad = false;
+        const Place at = {lo, p.starts[lo], fresh_rows(p, lo, bad), p.lengths[lo], 0};
+        __syncwarp();
+        if (row - at.row0 < at.fresh) row_again<BF>(p, at, kvh, (row - at.row0) * per + head - kvh * per, 0, DP);
+      }
+    }
+  }
+  stamp_end(p.stamps);
+}
+
+uint64_t most_items(const PagedAttention &p) {  // every sequence with rows may have a tile that is not full
+  const uint64_t packed = (uint64_t)p.rows * (p.heads / p.kv_heads);
+  return (packed + std::min<uint64_t>(p.n, packed) * (2 * kRows - 1)) / (2 * kRows) * p.kv_heads;
+}
+
 // Queries as [rows, heads, dim]: boxes of 64 dimensions, a group's heads and as many rows as make up a tile. False where they cannot be mapped.
 template <bool BF> bool make_q_map(CUtensorMap *map, const PagedAttention &p, uint32_t per) {
   EncodeTiled enc = encode_tiled();
@@ -601,14 +693,14 @@ template <bool BF> bool make_q_map(CUtensorMap *map, const PagedAttention &p, ui
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 template <bool BF, int DP> cudaError_t run(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
-  const uint64_t per = p.heads / p.kv_heads, tiles = p.rows * per / (2 * kRows) + std::min<uint64_t>(p.n, p.rows * per);
+  const uint64_t per = p.heads / p.kv_heads;
   const uint64_t cache_rows = (uint64_t)p.pages * p.kv_heads * p.page.d;
   CUtensorMap map_k = {}, map_v = {}, map_q = {};
   uint32_t box = kKeys;  // the most rows, a power of two, of which pages consist; coordinates are signed
   while (p.page.d % box) box /= 2;
   if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) || !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF)) box = 0;
   const bool q_box = kRows % per == 0 && make_q_map<BF>(&map_q, p, (uint32_t)per);
-  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)std::min<uint64_t>(sms, tiles * p.kv_heads)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
+  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)std::min<uint64_t>(sms, most_items(p) * p.splits)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
   cudaFuncAttributes a;
@@ -624,6 +716,16 @@ cudaError_t setup_paged_prompt_tc() {
   for (cudaError_t e : {setup_one<false, 64>(), setup_one<false, 128>(), setup_one<true, 64>(), setup_one<true, 128>()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
+}
+uint32_t paged_prompt_splits(const PagedAttention &p, uint32_t sms) {
+  if (p.dim > 128) return 1;
+  const uint64_t most = (uint64_t)p.width * p.page.d / (kKeys * kSliceTiles);
+  return (uint32_t)std::max<uint64_t>(std::min<uint64_t>({sms / most_items(p), most, kMostSplits}), 1);
+}
+cudaError_t launch_paged_prompt_join(const PagedAttention &p, cudaStream_t s) {
+  const dim3 grid((uint32_t)(((uint64_t)p.rows * p.heads + 7) / 8));
+  if (p.dim <= 64) return launch_following(p.bf ? paged_prompt_join_kernel<true, 64> : paged_prompt_join_kernel<false, 64>, grid, 256, 0, s, p);
+  return launch_following(p.bf ? paged_prompt_join_kernel<true, 128> : paged_prompt_join_kernel<false, 128>, grid, 256, 0, s, p);
 }
 cudaError_t launch_paged_prompt_tc(const PagedAttention &p, uint32_t sms, cudaStream_t s) {
   if (p.dim <= 64) return p.bf ? run<true, 64>(p, sms, s) : run<false, 64>(p, sms, s);
