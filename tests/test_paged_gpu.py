@@ -365,6 +365,21 @@ def test_numbers_that_a_row_does_not_see_do_not_reach_it(dev, dim):
             assert np.abs(got[60, 0]).max() < 10
 
 
+def test_a_cta_goes_on_behind_rows_that_are_computed_again(dev):
+    """More tiles than SMs; the other sequences' rows are the same bits as without infinities and NaN beside them."""
+    n, new = 60, 130
+    for bad in (0x7c00, 0x7e00):
+        c = Cache(np.random.default_rng(13), [new] * n, 4, 64, 16, vk.FP16)
+        clean = prompt(dev, [0] * n, [new] * n, 4, 4, 64, 16, vk.FP16, cache=c, finite=False)
+        for i in range(1, n, 2):
+            c.seq_v[i][:, 0, 5] = bad
+            c.put(c.v, i, c.seq_v[i])
+        got = prompt(dev, [0] * n, [new] * n, 4, 4, 64, 16, vk.FP16, cache=c, finite=False).reshape(n, new, 4, 64)
+        clean = clean.reshape(n, new, 4, 64)
+        assert np.array_equal(got[::2], clean[::2]) and np.isfinite(clean).all()
+        assert not np.isfinite(got[1::2, :, :, 5]).any() and np.isfinite(np.delete(got[1::2], 5, 3)).all()
+
+
 # ---- what is refused ---------------------------------------------------------------------------------------------------
 def test_bad_pages_and_lengths_are_reported(dev):
     """The kernels check pages against the cache, lengths against the table, starts against both, and read nothing outside."""

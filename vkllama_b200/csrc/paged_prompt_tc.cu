@@ -191,10 +191,10 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     return ok != 0;
   };
   // For waits that are long by design: a warp that polls takes issue slots from the softmax warps of its scheduler (the ticket warp alone
-  // cost a third of the rate).
-  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns) {
+  // cost a third of the rate). That one waits for whole items, which may have millions of positions.
+  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns, bool item = false) {
     uint32_t ok = 0;
-    for (uint32_t n = 0; !ok && n < (sh.slow ? kPolls * kRounds : kPolls); ++n) {
+    for (uint32_t n = 0; !ok && n < (item || sh.slow ? kPolls * kRounds : kPolls); ++n) {
       asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(sa(bar)), "r"(parity) : "memory");
       if (!ok) __nanosleep(ns);
     }
@@ -543,8 +543,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       return __shfl_sync(0xffffffffu, next, 0);
     };
     for (uint32_t k = 0;; ++k) {
-      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200)) break;
-      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200)) break;
+      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200, true)) break;
+      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200, true)) break;
       if (k) ticket = take();
       Item it = {};
       for (;; ticket = take()) {
@@ -578,7 +578,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       // and is not stored), else piece by piece
       bool ok = true;
       for (uint32_t i = 0; ok && i < it.tiles; ++i) {
-        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64))) break;
+        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64, true))) break;
         ++used[i];
         const uint32_t dst = q_a + i * C::kTile, bar = sa(&q_full[i]), r0 = it.at.first + i * kRows;
         if (q_box) {
