@@ -211,8 +211,13 @@ class Device:
             self.h = None
 
 
+_Shape = u32 * 6
+
+
 class Tensor:
     """Tensor (src/core/tensor.h): a reference-counted handle."""
+
+    _ptr = None  # its memory's address, which it keeps as long as it lives
 
     def __init__(self, c=0, h=0, w=0, dev=None, dtype=FP32, _handle=None, _borrowed=False):
         self.L = load_library()
@@ -229,7 +234,7 @@ class Tensor:
         return self
 
     def shape_constant(self):
-        o = (u32 * 6)()
+        o = _Shape()
         _ck(self.L.vkl_tensor_shape(self.h, o))
         return tuple(o)
 
@@ -265,9 +270,11 @@ class Tensor:
         return self
 
     def device_ptr(self):
-        p = vp()
-        _ck(self.L.vkl_tensor_device_ptr(self.h, C.byref(p)))
-        return p.value
+        if self._ptr is None:
+            p = vp()
+            _ck(self.L.vkl_tensor_device_ptr(self.h, C.byref(p)))
+            self._ptr = p.value
+        return self._ptr
 
     def __del__(self):
         try:
