@@ -146,7 +146,8 @@ __device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
   tmem_st16(taddr, u);
 }
 
-template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
+// SPLIT: p.splits > 1. (One kernel for both costs 0.4 us an item.)
+template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThreads, 1)
     paged_prompt_tc_kernel(const PagedAttention p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const __grid_constant__ CUtensorMap map_q, const uint32_t box, const bool q_box) {
   using C = Cfg<DP>;
@@ -312,12 +313,12 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
         output ^= 1;
         if (ok) {
           tc_after();
-          const float inv = it->slices == 1 ? 1.0f / sum : 1.0f;
+          const float inv = 1.0f / sum;
           const uint32_t row = min(r, packed - 1), rt = quotient(row, p.group);
           const size_t to = (size_t)(at.row0 + rt) * p.heads + kvh * per + row - rt * per;
           uint16_t *out = static_cast<uint16_t *>(p.out) + to * p.dim;
           float finite = 0.f;
-          if (it->slices > 1) {  // a part of the row's positions
+          if (SPLIT && it->slices > 1) {  // a part of the row's positions
             const size_t part = (size_t)it->slice * p.rows * p.heads + to;
             if (r < packed) p.part_ml[part] = make_float2(ref, sum == 0.f ? -1.f : sum);  // 0 is a part that there is not
 #pragma unroll
@@ -413,6 +414,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t first = values ? 0 : lo, last = values ? boxes : hi;
         const uint32_t r0 = values ? whole * box : 0, r1 = !box ? kKeys : values ? hi * box : 0;
         const uint32_t copied = last > first ? last - first - (r1 > r0 && box ? 1 : 0) : 0;
+        if (t1 - t == min(t1 - t0, 2u) && lane == 0) arrive(sa(&sh.fetched));  // the next ticket may be taken
         if (x >= C::kStages && !(ok = wait_idle(&empty[pos.s], pos.phase ^ 1, 64))) break;
         const uint32_t dst = ring_a + pos.s * C::kTile, bar = sa(&full[pos.s]);
         const bool pieces = r1 > r0;
@@ -448,7 +450,6 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
         }
         if (t + 1 < t1) look_up(t + 1);
       }
-      if (lane == 0) arrive(sa(&sh.fetched));
       copy_wait<0>();
       if (late) landed();
       item_done(k);
@@ -531,7 +532,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------- what comes next, once all of this item is requested: a ticket taken earlier
+    // ------------------------------------------------- what comes next, once two tiles of this item are left to request: a ticket taken much earlier
     // could have been another CTA's, which has nothing left to do (106 -> 158 us for a few long items)
     if (blockIdx.x == 0) check_rows(p);
     uint32_t used[2] = {};  // how often each tile's place for Q
@@ -548,10 +549,9 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
       if (k) ticket = take();
       Item it = {};
       for (;; ticket = take()) {
-        const uint32_t head = ticket / p.splits, tile = head / p.kv_heads;  // all heads of a tile, then the next tile
+        const uint32_t head = SPLIT ? ticket / p.splits : ticket, tile = head / p.kv_heads;  // all heads of a tile, then the next tile
         it.found = find_tile(p, per, 2 * kRows, tile, it.at, walk);
         it.kvh = head - tile * p.kv_heads;
-        it.slice = ticket - head * p.splits;
         const uint32_t packed = it.at.fresh * per, past = it.at.len - it.at.fresh;
         it.tiles = it.at.first + kRows < packed ? 2 : 1;
 #pragma unroll
@@ -560,9 +560,10 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, 1)
           it.b[i] = (p.window && lo + 1 > p.window ? lo + 1 - p.window : 0) / kKeys;
           it.e[i] = hi / kKeys + 1;
         }
+        if (!SPLIT || !it.found) break;
         const uint32_t t0 = it.b[0], all = it.e[1] - t0;
+        it.slice = ticket - head * p.splits;
         it.slices = max(min(p.splits, all / kSliceTiles), 1u);
-        if (!it.found) break;
         if (it.slice >= it.slices) continue;
         const uint32_t s0 = t0 + it.slice * all / it.slices, s1 = t0 + (it.slice + 1) * all / it.slices;
 #pragma unroll
@@ -700,14 +701,18 @@ template <bool BF, int DP> cudaError_t run(const PagedAttention &p, uint32_t sms
   while (p.page.d % box) box /= 2;
   if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) || !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF)) box = 0;
   const bool q_box = kRows % per == 0 && make_q_map<BF>(&map_q, p, (uint32_t)per);
-  return launch_following(paged_prompt_tc_kernel<BF, DP>, dim3((uint32_t)std::min<uint64_t>(sms, most_items(p) * p.splits)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
+  return launch_following(p.splits > 1 ? paged_prompt_tc_kernel<BF, DP, true> : paged_prompt_tc_kernel<BF, DP, false>, dim3((uint32_t)std::min<uint64_t>(sms, most_items(p) * p.splits)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
-  cudaFuncAttributes a;
-  const cudaError_t e = cudaFuncGetAttributes(&a, paged_prompt_tc_kernel<BF, DP>);
-  if (e != cudaSuccess) return e;
-  if (a.numRegs * kThreads < kLaunchRegs) return cudaErrorInvalidConfiguration;  // the softmax warps would wait for registers that nobody has
-  return cudaFuncSetAttribute(paged_prompt_tc_kernel<BF, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);
+  for (auto kernel : {paged_prompt_tc_kernel<BF, DP, false>, paged_prompt_tc_kernel<BF, DP, true>}) {
+    cudaFuncAttributes a;
+    cudaError_t e = cudaFuncGetAttributes(&a, kernel);
+    if (e != cudaSuccess) return e;
+    if (a.numRegs * kThreads < kLaunchRegs) return cudaErrorInvalidConfiguration;  // the softmax warps would wait for registers that nobody has
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
