@@ -320,6 +320,15 @@ def test_positions_are_split_where_there_are_few_rows(dev, dtype, past, new, hea
     prompt(dev, past, new, heads, kv, dim, page, dtype, window, behind=3, wide=8)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,dim,page,window,least", [(8, 128, 16, 0, 0), (2, 64, 24, 0, 0), (6, 96, 5, 300, 0), (8, 40, 128, 129, 200)])
+def test_drafts_of_many_sequences(dev, dtype, heads, dim, page, window, least):
+    """A few rows behind none, one and more tiles of positions, more sequences than SMs."""
+    rng = np.random.default_rng(14)
+    past = [0, 127, 128, 255, 256, 383, 384, 1000] + [int(x) for x in rng.integers(least, 1200, 72)]
+    prompt(dev, [max(x, least) for x in past], [int(x) for x in rng.integers(0 if least else 1, 8, 80)], heads, 2, dim, page, dtype, window, behind=1)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_infinite_and_missing_numbers_in_a_slice(dev, dim):
     for dtype in DTYPES:
@@ -335,6 +344,14 @@ def test_infinite_and_missing_numbers_in_a_slice(dev, dim):
                 assert np.isnan(got[r, :, 3]).all() == (not window) and np.isposinf(got[r, :, 5]).all() and np.isnan(got[r, :, 7]).all() == (r >= 2)
                 assert np.isfinite(np.delete(got[r], [3, 5, 7], 1)).all()
             assert np.isfinite(got[4:7]).all() and not np.isfinite(got[7]).any()
+            n = 80  # and in many sequences
+            c = Cache(np.random.default_rng(13), [500] * n, 2, dim, 16, dtype)
+            for i in range(1, n, 2):
+                c.seq_v[i][:, 100, 3], c.seq_v[i][:, 200, dim - 1] = nan, inf
+                c.put(c.v, i, c.seq_v[i])
+            got = prompt(dev, [496] * n, [4] * n, 4, 2, dim, 16, dtype, cache=c, finite=False).reshape(n, 4, 4, dim)
+            assert np.isfinite(got[::2]).all() and np.isnan(got[1::2, :, :, 3]).all() and np.isposinf(got[1::2, :, :, dim - 1]).all()
+            assert np.isfinite(np.delete(got[1::2], [3, dim - 1], 3)).all()
 
 
 def test_many_short_prompts_and_a_long_one(dev):
