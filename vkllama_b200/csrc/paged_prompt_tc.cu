@@ -5,7 +5,7 @@
 // written over S_i in TMEM, O_i += P_i V_j with P as the TMEM operand. The two tiles of rows take turns: while the tensor core works
 // for one, the exponentials of the other are computed, which take as long (16 per clock and SM: 1024 cycles for 128 x 128, like the two
 // products). A CTA stays on its SM and takes one such item after the other by tickets, what takes longest first: a new CTA per item costs some
-// 10 us of start and end, in which nothing else runs (64 prompts of 256: 210 us, this way 149). Warps:
+// 10 us of start and end, in which nothing else runs (64 prompts of 256: 210 us, this way 107). Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
 //             that it grew by more than 2^8: until then the probabilities stay below 2^8 and O as it is; only then O is multiplied.
 //   8, 9      fetch K_j and V_j into a ring, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte
