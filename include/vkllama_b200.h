@@ -215,7 +215,8 @@ int vkl_cast_run(vkl_op *op, vkl_tensor *in, vkl_tensor **out);
  * What only the device can see (a page number beyond the cache, lengths beyond the table, an empty pool) is checked there; nothing outside
  * the tensors is touched, and the next vkl_command_wait returns the error. The calls of ONE op share its outputs and workspace: they must not
  * overlap on the GPU, also not as replays of captured graphs. After a first call of the same shape a call allocates nothing and
- * can be captured (vkl_command_stream); the error word is then read by the wait of the next directly recorded call.
+ * can be captured (vkl_command_stream); the error word is then read by the wait of the next directly recorded call. A captured call
+ * keeps the op and goes on writing the outputs that it had, which the op gives up at the next call of another shape: retain them as long as the graph lives.
  *
  * PagedTables: gives and takes pages so that every sequence has pages for target[i] tokens, and names the slots of its new ones. Sequences may
  * grow, shrink (to 0: finished; by some: tokens taken back) or stay in one call; lengths becomes target.

@@ -575,6 +575,44 @@ def test_a_captured_step_follows_what_is_in_its_tensors(dev):
     del graph
 
 
+def test_captured_calls_of_several_shapes(dev):
+    """Each shape's graph keeps its outputs and workspace when the op goes on to others, whose workspace is larger."""
+    torch = pytest.importorskip("torch")
+    rng, cmd = np.random.default_rng(15), vk.Command(dev)
+    heads, kv, dim, page = 4, 1, 64, 16
+    op, kept = vk.PagedAttention(dev, cmd, heads, kv, dim, page).init(), []
+    stream = torch.cuda.ExternalStream(cmd.stream())
+    for past, new in (([3000], [2]), ([2500, 3000, 40], [3, 300, 1]), ([3000, 3000], [500, 400])):
+        c = Cache(rng, [a + b for a, b in zip(past, new)], kv, dim, page, vk.FP16)
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.uint32)
+        with cmd:
+            k, v, table, lens = c.up(cmd, dev)
+            args = (tensor(cmd, dev, draw(rng, (int(starts[-1]), heads * dim), vk.FP16), vk.FP16), k, v, table, lens, tensor(cmd, dev, starts))
+            out = op(*args)
+            want = cmd.download(out)
+        graph = torch.cuda.CUDAGraph()
+        cmd.begin()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            assert op(*args) is out
+        cmd.end()
+        kept.append((graph, out, want, args))
+    held = [vk.Tensor(1, 1, 1 << x, dev, vk.FP32) for x in range(4, 22)]  # takes what has been given up
+    with cmd:
+        for t in held:
+            cmd.upload(np.full(t.shape(), 7, np.float32), t)
+    for graph, out, want, _ in kept + kept[::-1]:
+        with cmd:
+            cmd.upload(np.zeros_like(want), out)
+        with torch.cuda.stream(stream):
+            graph.replay()
+        stream.synchronize()
+        with cmd:
+            assert (cmd.download(out) == want).all()
+    with cmd:
+        assert all((cmd.download(t) == 7).all() for t in held)
+    kept.clear()
+
+
 def test_two_commands_at_once(dev):
     """Ops of their own on streams of their own do not share workspace."""
     rng = np.random.default_rng(13)

@@ -232,10 +232,13 @@ struct PagedAttentionOp : PagedOp {
   int heads, kv_heads, dim, page, window, dtype;
   float scale;
   vkl_tensor *out = nullptr, *scratch = nullptr, *counters = nullptr, *part_o = nullptr, *part_ml = nullptr;
+  vkl_tensor *older[64];  // smaller part_o and part_ml, which captured calls go on using
+  int n_older = 0;
   PagedAttentionOp(vkl_device *d, vkl_command *c, int h, int kv, int dm, int pg, float s, int w, int dt)
       : PagedOp(d, c), heads(h), kv_heads(kv), dim(dm), page(pg), window(w), dtype(dt), scale(s) {}
   ~PagedAttentionOp() override {
     for (vkl_tensor *t : {out, scratch, counters, part_o, part_ml}) vkl_tensor_release(t);
+    while (n_older) vkl_tensor_release(older[--n_older]);
   }
   int init() override {
     if (inited) return VKL_OK;
@@ -255,6 +258,20 @@ struct PagedAttentionOp : PagedOp {
     VKL_OKAY(ensure_tensor(dev, &counters, 1, 1, sms + 3, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
     return paged_init();
+  }
+  // Room for n numbers, all 0 if it is new. It grows by powers of two.
+  int room(vkl_tensor **t, size_t n) {
+    if (*t && (*t)->w >= n) return VKL_OK;
+    size_t more = 1 << 16;
+    while (more < n) more *= 2;
+    if (*t) {
+      if (n_older == 64) return fail(VKL_RESOURCE_EXHAUSTED, "paged_attention: too many workspaces");
+      older[n_older++] = *t;
+      *t = nullptr;
+    }
+    VKL_OKAY(ensure_tensor(dev, t, 1, 1, more, VKL_FP32));
+    VKL_CUDA(cudaMemsetAsync((*t)->data(), 0, more * 4, cmd->stream));
+    return VKL_OK;
   }
   int run(vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths, vkl_tensor *starts, vkl_tensor **o) {
     const char *who = "paged_attention";
@@ -297,11 +314,8 @@ struct PagedAttentionOp : PagedOp {
       p.splits = starts ? paged_prompt_splits(p, sms) : 1;
       if (p.splits > 1) {
         const size_t parts = p.splits * rows * heads;
-        if (!part_o || part_o->w < parts * (dim <= 64 ? 64 : 128)) VKL_OKAY(ensure_tensor(dev, &part_o, 1, 1, parts * (dim <= 64 ? 64 : 128), VKL_FP32));
-        if (!part_ml || part_ml->w < parts * 2) {
-          VKL_OKAY(ensure_tensor(dev, &part_ml, 1, 1, parts * 2, VKL_FP32));
-          VKL_CUDA(cudaMemsetAsync(part_ml->data(), 0, parts * 8, cmd->stream));
-        }
+        VKL_OKAY(room(&part_o, parts * (dim <= 64 ? 64 : 128)));
+        VKL_OKAY(room(&part_ml, parts * 2));
         p.part_o = (float *)part_o->data(), p.part_ml = (float2 *)part_ml->data();
       }
       VKL_LAUNCH(starts ? paged_prompt_launches(p) : 1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
