@@ -272,14 +272,16 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
       const uint32_t h0 = first_head(at.grp), nh = heads_of(at.grp);
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        const uint16_t *src = static_cast<const uint16_t *>(p.q) + at.seq * p.q_ld + (h0 + r * 8 + g) * p.dim;
+        // every load first, whether its number exists or not: under conditions they waited for one another (sixteen heads of 192: 5.5 us)
+        const uint16_t *src = static_cast<const uint16_t *>(p.q) + at.seq * p.q_ld + (h0 + min(r * 8 + g, nh - 1)) * p.dim;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t d = k * 16 + e * 8 + t4 * 2;
-            q[k][e * NR + r] = r * 8 + g < nh && d < p.dim ? *reinterpret_cast<const uint32_t *>(src + d) ^ flip : 0u;
-          }
+          for (int e = 0; e < 2; ++e) q[k][e * NR + r] = __ldg(reinterpret_cast<const uint32_t *>(src + min(k * 16 + e * 8 + t4 * 2, p.dim - 2)));
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) q[k][e * NR + r] = r * 8 + g < nh && k * 16 + e * 8 + t4 * 2 < p.dim ? q[k][e * NR + r] ^ flip : 0u;
         mx[r] = -INFINITY;
         sum[r] = 0.f;
       }
@@ -427,10 +429,14 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
               write_out(at.seq, h0 + r * 8 + g, n * 8 + t4 * 2, a, b);
             }
           }
-          const uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f);  // NaN
+          uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f);  // NaN
           __syncwarp();
-          for (uint32_t x = 0; x < 8; ++x)
-            if (again >> (x * 4) & 15u) redo(at.seq, h0 + r * 8 + x);
+#pragma unroll 1
+          while (again) {
+            const uint32_t x = (__ffs(again) - 1) / 4;
+            redo(at.seq, h0 + r * 8 + x);
+            again &= ~(15u << (x * 4));
+          }
         }
       } else {
         if (lane == 0) part_s[warp][over] = {at.seq, at.grp, 1, begins, ends};
@@ -478,9 +484,9 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
       l = warp_sum(l * c);
       m = top;
       float2 acc[DP / 64] = {};
-#pragma unroll
-      for (uint32_t x = 0; x < 2 * kWarps; ++x) {
-        if (!(in_run >> x & 1)) continue;
+#pragma unroll 1
+      for (uint32_t more = in_run; more; more &= more - 1) {
+        const uint32_t x = __ffs(more) - 1;
         const float cx = __shfl_sync(0xffffffffu, c, x);
         const float *src = part_o(x) + h * DP;
 #pragma unroll
