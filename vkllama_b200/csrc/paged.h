@@ -109,7 +109,7 @@ struct PagedAttention {
   const uint32_t *table, *lengths;
   const uint32_t *starts;       // [n + 1], or null: row i is the last token of sequence i
   float *scratch;               // partial results, paged_token_scratch() bytes
-  uint32_t *counters;           // [SMs + 1], 0 between launches
+  uint32_t *counters;           // [2 (SMs + 1)], 0 between launches
   uint32_t *tickets;            // [2], 0 between launches
   float *part_o;                // prompts whose positions are split: [splits][rows][heads][64 or 128] sums of parts
   float2 *part_ml;              // and [splits][rows][heads] references and sums of probabilities, 0 between calls

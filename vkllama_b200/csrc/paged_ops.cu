@@ -255,7 +255,7 @@ struct PagedAttentionOp : PagedOp {
     VKL_CUDA(setup_paged_prompt());
     VKL_CUDA(setup_paged_prompt_tc());
     VKL_OKAY(ensure_tensor(dev, &scratch, 1, 1, paged_token_scratch(heads, kv_heads, dim, sms) / 4, VKL_FP32));
-    VKL_OKAY(ensure_tensor(dev, &counters, 1, 1, sms + 3, VKL_UINT32));
+    VKL_OKAY(ensure_tensor(dev, &counters, 1, 1, 2 * (sms + 1) + 2, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
     return paged_init();
   }
@@ -302,7 +302,7 @@ struct PagedAttentionOp : PagedOp {
       p.starts = starts ? (const uint32_t *)starts->data() : nullptr;
       p.scratch = (float *)scratch->data();
       p.counters = (uint32_t *)counters->data();
-      p.tickets = p.counters + sms + 1;
+      p.tickets = p.counters + 2 * (sms + 1);
       VKL_OKAY(command_error_word(cmd, &p.error));
       p.stamps = stamp();
       p.rows = (uint32_t)rows, p.n = (uint32_t)n, p.heads = heads, p.kv_heads = kv_heads, p.dim = dim;

@@ -34,6 +34,9 @@ constexpr uint32_t kShareRows = 256;          // a CTA's share is at least this 
 // A cut this near to a pair's border moves there. A cut costs some 5 us at the end (the parts of several CTAs meet in L2); a tile of 32 more
 // for one CTA costs 0.4 us where HBM is the limit, and an eighth of 1 us where the whole call is short.
 constexpr uint32_t kSnapRows = 256, kSnapRowsShort = 512, kShortRows = 1024;
+// Parts of a pair that one CTA adds up, and how many it does at a time; of more, every kGroup are added up first (one sequence of 60,000 positions, 16 heads of 128
+// on one key head, 148 parts: 55 us by one CTA, this way 29).
+constexpr uint32_t kJoin = 32, kGroup = 16, kAtOnce = 8;
 constexpr uint32_t kPairCost = 1;             // what a pair costs beside its tiles (queries, output, short rows in the ring), in tiles
 
 // DP: padded head width. WIDE: sixteen query heads in the rows of A; else eight, and the low parts of their probabilities in the others.
@@ -525,43 +528,39 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
     return;
   }
 
-  // ---- pairs of several CTAs ----
-  __threadfence();
-  __syncthreads();
-  if (tid < 2) {
-    last_s[tid] = 0;
-    if (open_there >> tid & 1) {
-      const uint32_t c0 = cut_s[tid][0], parts = cut_s[tid][1] - c0 + 2;
-      __threadfence();
-      if (atomicAdd(p.counters + c0, 1u) + 1 == parts) {
-        p.counters[c0] = 0;
-        last_s[tid] = 1;
-      }
-    }
-  }
-  __syncthreads();
+  // ---- pairs of several CTAs: the last of its CTAs adds up the parts, of more than kJoin the last one of every kGroup does and the last of those ----
+  auto rec = [&](uint32_t c, uint32_t c0, uint32_t h) { return ((size_t)c * 2 + (c + 1 == c0 ? 1 : 0)) * C::kHeads + h; };  // the first part ends its CTA's range
+  auto add_up = [&](uint32_t side, uint32_t first, uint32_t step, uint32_t parts, bool whole) {  // at most 32 parts: lane x has part x's maximum and sum
+    const uint32_t seq = open_seq[side], grp = open_grp[side], h0 = first_head(grp), nh = heads_of(grp), c0 = cut_s[side][0];
 #pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    if (!last_s[side]) continue;
-    __threadfence();
-    const uint32_t seq = open_seq[side], grp = open_grp[side], h0 = first_head(grp), nh = heads_of(grp), c0 = cut_s[side][0], c1 = cut_s[side][1];
-    auto rec = [&](uint32_t c, uint32_t h) { return ((size_t)c * 2 + (c + 1 == c0 ? 1 : 0)) * C::kHeads + h; };  // the first part ends its CTA's range
     for (uint32_t h = warp; h < nh; h += kWarps) {
-      float m = -INFINITY, l = 0.f;
-      for (uint32_t c = c0 - 1 + lane; c <= c1; c += 32) m = fmaxf(m, __ldcg(scratch_ml + rec(c, h) * 2));
-      m = warp_max(m);
-      const float ref = m == -INFINITY ? 0.f : m * scale;
+      float2 own = {-INFINITY, 0.f};
+      if (lane < parts) own = __ldcg(reinterpret_cast<const float2 *>(scratch_ml + rec(first + lane * step, c0, h) * 2));
+      const float m = warp_max(own.x), ref = m == -INFINITY ? 0.f : m * scale, w = exp2_fast(own.x * scale - ref), l = warp_sum(lane < parts ? w * own.y : 0.f);
       float2 acc[DP / 64] = {};
-#pragma unroll 4
-      for (uint32_t c = c0 - 1; c <= c1; ++c) {
-        const float2 x = __ldcg(reinterpret_cast<const float2 *>(scratch_ml + rec(c, h) * 2));
-        const float w = exp2_fast(x.x * scale - ref);
-        l += w * x.y;
+#pragma unroll 1
+      for (uint32_t x = 0; x < parts; x += kAtOnce) {
+        float2 v[kAtOnce][DP / 64];
 #pragma unroll
-        for (int d = 0; d < DP / 64; ++d) {
-          const float2 v = __ldcg(reinterpret_cast<const float2 *>(scratch_o + rec(c, h) * DP + d * 64 + lane * 2));
-          acc[d].x += w * v.x, acc[d].y += w * v.y;
+        for (uint32_t y = 0; y < kAtOnce; ++y)
+#pragma unroll
+          for (int d = 0; d < DP / 64; ++d)
+            v[y][d] = __ldcg(reinterpret_cast<const float2 *>(scratch_o + rec(first + min(x + y, parts - 1) * step, c0, h) * DP + d * 64 + lane * 2));
+#pragma unroll
+        for (uint32_t y = 0; y < kAtOnce; ++y) {
+          const float wy = __shfl_sync(0xffffffffu, w, (x + y) & 31);
+          if (x + y >= parts) continue;
+#pragma unroll
+          for (int d = 0; d < DP / 64; ++d) acc[d].x += wy * v[y][d].x, acc[d].y += wy * v[y][d].y;
         }
+      }
+      if (!whole) {
+        const size_t to = rec(first, c0, h);
+        __syncwarp();
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d) *reinterpret_cast<float2 *>(scratch_o + to * DP + d * 64 + lane * 2) = acc[d];
+        if (lane == 0) *reinterpret_cast<float2 *>(scratch_ml + to * 2) = make_float2(m, l);
+        continue;
       }
       const float r = 1.0f / l;
       float finite = 0.f;
@@ -575,6 +574,48 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
         __syncwarp();
         redo(seq, h0 + h);
       }
+    }
+  };
+  __threadfence();
+  __syncthreads();
+  if (tid < 2) {
+    last_s[tid] = 0;
+    if (open_there >> tid & 1) {
+      const uint32_t c0 = cut_s[tid][0], parts = cut_s[tid][1] - c0 + 2, g = (blockIdx.x + 1 - c0) / kGroup;
+      uint32_t *counter = parts <= kJoin ? p.counters + c0 : p.counters + gridDim.x + 1 + c0 + g;  // a pair has fewer groups than cuts
+      __threadfence();
+      if (atomicAdd(counter, 1u) + 1 == (parts <= kJoin ? parts : min(kGroup, parts - g * kGroup))) {
+        *counter = 0;
+        last_s[tid] = 1;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t side = 0; side < 2; ++side) {
+    if (!last_s[side]) continue;
+    __threadfence();
+    const uint32_t c0 = cut_s[side][0], parts = cut_s[side][1] - c0 + 2;
+    if (parts <= kJoin) {
+      add_up(side, c0 - 1, 1, parts, true);
+      continue;
+    }
+    const uint32_t g = (blockIdx.x + 1 - c0) / kGroup, groups = (parts + kGroup - 1) / kGroup;
+    add_up(side, c0 - 1 + g * kGroup, 1, min(kGroup, parts - g * kGroup), false);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      last_s[side] = 1;
+      if (atomicAdd(p.counters + c0, 1u) + 1 == groups) {
+        p.counters[c0] = 0;
+        last_s[side] = 2;
+      }
+    }
+    __syncthreads();
+    if (last_s[side] == 2) {
+      __threadfence();
+      add_up(side, c0 - 1, kGroup, groups, true);
     }
   }
   stamp_end(p.stamps);
