@@ -34,6 +34,9 @@ constexpr uint32_t kShareRows = 256;          // a CTA's share is at least this 
 // A cut this near to a pair's border moves there. A cut costs some 5 us at the end (the parts of several CTAs meet in L2); a tile of 32 more
 // for one CTA costs 0.4 us where HBM is the limit, and an eighth of 1 us where the whole call is short.
 constexpr uint32_t kSnapRows = 256, kSnapRowsShort = 512, kShortRows = 1024;
+// Where a tile has more products (sixteen heads, or heads above 128), shorter pieces are worth their cut. us, these three as above and as below: one sequence of 1151
+// positions, 32 heads of 128 on 2 key heads, 21.8 and 14.9; three of 2500, 16 heads of 256 on one, 35 and 26; four of 2000, 16 of 256 on 2, 26 and 19.
+constexpr uint32_t kWideRows = 128, kSnapRowsShort256 = 256;
 // Parts of a pair that one CTA adds up, and how many it does at a time; of more, every kGroup are added up first (one sequence of 60,000 positions, 16 heads of 128
 // on one key head, 148 parts: 55 us by one CTA, this way 29).
 constexpr uint32_t kJoin = 32, kGroup = 16, kAtOnce = 8;
@@ -48,7 +51,8 @@ template <int DP, bool WIDE> struct Cfg {
   static constexpr uint32_t kHeads = WIDE ? 16 : 8;
   static constexpr uint32_t kStash = kHeads * DP * 4;  // a warp's first part, where its range goes on behind it
   static constexpr uint32_t kSmem = kWarps * (kRing * kHalf + kStash + 2 * kHeads * 2 * 4);
-  static constexpr uint32_t kShare = kShareRows / kTile, kSnap = kSnapRows / kTile, kSnapShort = kSnapRowsShort / kTile, kShort = kShortRows / kTile;
+  static constexpr uint32_t kShare = (WIDE ? kWideRows : kShareRows) / kTile, kSnap = (WIDE ? kWideRows : kSnapRows) / kTile;
+  static constexpr uint32_t kSnapShort = (WIDE ? kWideRows : DP == 256 ? kSnapRowsShort256 : kSnapRowsShort) / kTile, kShort = kShortRows / kTile;
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory of an SM");
   static_assert(kRing * kHalf >= kStash, "a warp's last part lies in its ring");
 };
