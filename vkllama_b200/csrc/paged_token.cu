@@ -10,16 +10,16 @@
 // Work is cut into equal shares, not by sequence: the tiles (of 16 or 32 positions) of all (sequence, head group) pairs stand in one row, with
 // a place more for each pair's own cost; every CTA takes a range of it and every warp of the CTA a range of that, however the lengths are spread. Ranges cut pairs: a warp keeps
 // running maximum, sum and output of its part; parts meet in shared memory, and those of several CTAs in scratch, where the CTA that
-// arrives last adds them up in their order (the result does not depend on who that is). Cuts that would leave a small piece of a pair are
+// arrives last adds them up in their order, many of them in two steps (the result does not depend on who that is). Cuts that would leave a small piece of a pair are
 // moved to its border.
 //
 // A warp streams its range through a ring of its own (cp.async, tiles of keys and of values alternating, swizzled for ldmatrix):
 // no barrier inside the stream, the next pages are looked up a tile ahead. Rows that are not visible are not read and count as zeros.
 //
-// Measured on sequences that hold 0.37 GB together (57 us at the rate of a copy): 71 ... 76 us, 4.9 ... 5.2 TB/s, with up to eight heads to a
-// key head whatever the width, the page and the lengths; 87 us with 12 or 16 heads of 128, 103 us with 16 of 256 (shared memory and the
-// products are the limit there), 122 us with 32 on one key head, which reads everything twice. What is left up to eight heads is the
-// machine's: under full load 24 of the 148 SMs take 12 % longer for the same bytes, and shares are fixed before anyone knows which.
+// Measured on sequences that hold 0.37 GB together (57 us at the rate of a copy): 70 ... 78 us, 4.9 ... 5.3 TB/s, with up to eight heads to a
+// key head whatever the width, the page and the lengths; 76 us with 12 or 16 heads of 128, 93 us with 16 of 256 (shared memory and the
+// products are the limit there), 117 us with 32 on one key head, which reads everything twice. What is left up to eight heads is the
+// machine's: under full load groups of SMs take 12 % longer for the same bytes, and shares are fixed before anyone knows which.
 #include <algorithm>
 
 #include "common.cuh"
