@@ -699,9 +699,13 @@ template <bool BF, int DP> cudaError_t run(const PagedAttention &p, uint32_t sms
   CUtensorMap map_k = {}, map_v = {}, map_q = {};
   uint32_t box = kKeys;  // the most rows, a power of two, of which pages consist; coordinates are signed
   while (p.page.d % box) box /= 2;
-  if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) || !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF)) box = 0;
+  if (box < 8 || cache_rows > 0x7fffffffu || !make_map(&map_k, p.kcache, (uint32_t)cache_rows, p.dim, box, BF) ||
+      !make_map(&map_v, p.vcache, (uint32_t)cache_rows, p.dim, box, BF))
+    box = 0;
   const bool q_box = kRows % per == 0 && make_q_map<BF>(&map_q, p, (uint32_t)per);
-  return launch_following(p.splits > 1 ? paged_prompt_tc_kernel<BF, DP, true> : paged_prompt_tc_kernel<BF, DP, false>, dim3((uint32_t)std::min<uint64_t>(sms, most_items(p) * p.splits)), kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
+  const dim3 grid((uint32_t)std::min<uint64_t>(sms, most_items(p) * p.splits));
+  return launch_following(p.splits > 1 ? paged_prompt_tc_kernel<BF, DP, true> : paged_prompt_tc_kernel<BF, DP, false>, grid, kThreads, Cfg<DP>::kSmem, s, p, map_k,
+                          map_v, map_q, box, q_box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
   for (auto kernel : {paged_prompt_tc_kernel<BF, DP, false>, paged_prompt_tc_kernel<BF, DP, true>}) {
