@@ -59,3 +59,16 @@ def attention(q, pos, keys, values, window=0, scale=None):
                 out[r, h], mass[r, h] = p @ v, p @ np.abs(v)
             size[r, h] = abs(scale) * (np.abs(k) @ np.abs(q[r, h])).max()
     return out, mass, size
+
+
+def weights_sum(q, pos, keys, window=0, scale=None):
+    """Of attention's rows: the sum of exp(score - largest score)."""
+    rows, heads, dim = q.shape
+    per, scale = heads // keys.shape[0], dim ** -0.5 if scale is None else scale
+    den = np.ones((rows, heads, 1))
+    for r in range(rows):
+        lo = max(0, pos[r] + 1 - window) if window else 0
+        for h in range(heads if pos[r] >= 0 else 0):
+            s = scale * (keys[h // per, lo:pos[r] + 1] @ q[r, h])
+            den[r, h] = np.exp(s - s.max()).sum()
+    return den

@@ -1,0 +1,56 @@
+"""Attention over a paged cache where one position outweighs thousands of others that make up the output, and where a lost tile would show."""
+import numpy as np
+import pytest
+
+import vkllama_b200 as vk
+from paged_weights import LONG_STEPS, Cache, Sink, draw, near, tensor, to_values
+
+pytestmark = pytest.mark.gpu
+GAPS = [14.0, 17.0, 18.0, 20.0]
+
+
+def attention(dev, c, q, heads, scale=0.0, window=0, starts=None):
+    """Rows q, by one call."""
+    cmd = vk.Command(dev)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        op = vk.PagedAttention(dev, cmd, heads, c.kv, c.dim, c.page, scale, window, c.dtype).init()
+        args = () if starts is None else (tensor(cmd, dev, np.array(starts, np.uint32)),)
+        got = cmd.download(op(tensor(cmd, dev, q, c.dtype), k, v, table, lens, *args))
+    return to_values(got, c.dtype).reshape(-1, heads, c.dim)
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("lengths,heads,kv,dim,at,value", [
+    ([4000], 2, 1, 64, 0, 0.0), ([4000], 16, 1, 128, 3999, 0.0), ([300, 20, 150], 8, 1, 128, 0, 0.05), ([2000, 1], 24, 1, 256, 1000, 0.0), ([700] * 150, 4, 4, 64, 5, 0.0),
+    ([3000, 900], 8, 8, 192, 0, 0.0)])
+def test_one_token_that_a_position_outweighs(dev, gap, lengths, heads, kv, dim, at, value):
+    """Pairs that a warp has whole, and parts that warps and CTAs join."""
+    for spread in (0.0, 0.5):
+        c = Sink(np.random.default_rng(len(lengths) + dim), lengths, kv, dim, 16, vk.FP16, gap, value, at, spread)
+        q = c.queries(len(lengths), heads, dim, vk.FP16)
+        got, q = attention(dev, c, q, heads, 1.0), to_values(q, vk.FP16).reshape(-1, heads, dim)
+        for i in sorted({0, len(lengths) // 2, len(lengths) - 1}):
+            near(got[i:i + 1], c, i, q[i:i + 1], [lengths[i] - 1], "token", scale=1.0, what="sequence %d" % i)
+
+
+def rows(dev, c, past, new, heads, kernel, scale=1.0, window=0, q=None):
+    starts = np.concatenate([[0], np.cumsum(new)])
+    bits = c.queries(starts[-1], heads, c.dim, c.dtype) if q is None else q
+    got = attention(dev, c, bits, heads, scale, window, starts)
+    q = to_values(bits, c.dtype).reshape(-1, heads, c.dim)
+    for i in sorted({0, len(new) // 2, len(new) - 1}):
+        mine = sorted({int(starts[i]), int(starts[i]) + new[i] // 2, int(starts[i + 1]) - 1})
+        near(got[mine], c, i, q[mine], [past[i] + r - int(starts[i]) for r in mine], kernel, window, scale or None, "sequence %d" % i)
+
+
+@pytest.mark.parametrize("dtype", [vk.FP16, vk.BF16])
+def test_long_sequences_lack_no_tile(dev, dtype):
+    """The sequences of test_paged_weights_cpu.py, whose bounds sixteen positions do not fit into."""
+    for n, dim in ((300, 128), (4000, 64), (70001, 64)):
+        c = Cache(np.random.default_rng(n + dim), [n], 1, dim, 16, dtype)
+        q = draw(np.random.default_rng(1), (1, 2 * dim), dtype)
+        near(attention(dev, c, q, 2), c, 0, to_values(q, dtype).reshape(1, 2, dim), [n - 1], "token", steps=LONG_STEPS if n > 4000 else None)
+    for past, new, heads, dim, kernel in ((2999, 1, 3, 128, "tensor"), (2700, 300, 2, 128, "tensor"), (898, 2, 2, 200, "rows")):
+        c = Cache(np.random.default_rng(dim), [past + new], 1, dim, 16, dtype)
+        rows(dev, c, [past], [new], heads, kernel, 0.0, q=draw(np.random.default_rng(2), (new, heads * dim), dtype))

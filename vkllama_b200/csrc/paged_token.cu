@@ -4,8 +4,11 @@
 // Every visible key and value is read once for all query heads of its group (sixteen of them at a time), so HBM bounds it: 4 dim bytes a
 // position and key head. The products run on mma.sync (m16n8k16, fp32 sums) because a group's queries share the fragments: its query
 // heads are the rows of A, cached rows the columns. Probabilities go into the second product as two 16-bit numbers, p = hi + lo, both
-// products exact, so the result has their 32 bits. Up to eight heads lo has the upper eight rows of A, which would be empty, and costs nothing;
-// beyond, a second product with the same fragment of V.
+// products exact: relative 2^-16 in bfloat16, 2^-22 in fp16 (half steps of two numbers). fp16 ends at steps of 2^-24, so its probabilities
+// are 2^14 times as large, in sums and outputs alike: they keep 2^-22 down to 2^-17 of the row's largest, an output's 2^-11 down to 2^-28, and below each is off by
+// 2^-39 of the largest. (As they are, thousands of positions below 2^-25 counted in the sum and not in the output: with one position that outweighs
+// 4000 others by 20 nats and has the value 0, nothing was left.) Up to eight heads lo has the upper eight rows of A, which would be empty, and costs
+// nothing; beyond, a second product with the same fragment of V.
 //
 // Work is cut into equal shares, not by sequence: the tiles (of 16 or 32 positions) of all (sequence, head group) pairs stand in one row, with
 // a place more for each pair's own cost; every CTA takes a range of it and every warp of the CTA a range of that, however the lengths are spread. Ranges cut pairs: a warp keeps
@@ -41,6 +44,7 @@ constexpr uint32_t kWideRows = 128, kSnapRowsShort256 = 256;
 // on one key head, 148 parts: 55 us by one CTA, this way 29).
 constexpr uint32_t kJoin = 32, kGroup = 16, kAtOnce = 8;
 constexpr uint32_t kPairCost = 1;             // what a pair costs beside its tiles (queries, output, short rows in the ring), in tiles
+constexpr float kRaise = 14.f;                // fp16 probabilities are 2^14 times as large; 2^16 is left for one that its exponent's rounding takes above 1
 
 // DP: padded head width. WIDE: sixteen query heads in the rows of A; else eight, and the low parts of their probabilities in the others.
 template <int DP, bool WIDE> struct Cfg {
@@ -376,15 +380,17 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
         }
       }
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
+      for (int r = 0; r < NR; ++r) {
+        const float raise = BF ? -ref[r] : kRaise - ref[r];
 #pragma unroll
         for (int n = 0; n < SN; ++n) {
-          const float a = exp2_fast(fmaf(s[n][2 * r], scale, -ref[r])), b = exp2_fast(fmaf(s[n][2 * r + 1], scale, -ref[r]));
+          const float a = exp2_fast(fmaf(s[n][2 * r], scale, raise)), b = exp2_fast(fmaf(s[n][2 * r + 1], scale, raise));
           sum[r] += a + b;
           hi[n][r] = pack2<BF>(a, b);
           const float2 h = unpack2<BF>(hi[n][r]);
           lo[n][r] = pack2<BF>(a - h.x, b - h.y);
         }
+      }
       copy_wait<C::kRing - 1>();
       __syncwarp();
       {
