@@ -44,6 +44,15 @@ def rows(dev, c, past, new, heads, kernel, scale=1.0, window=0, q=None):
         near(got[mine], c, i, q[mine], [past[i] + r - int(starts[i]) for r in mine], kernel, window, scale or None, "sequence %d" % i)
 
 
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("past,new,heads,kv,dim,page", [
+    ([4000], [3], 4, 1, 200, 16), ([100, 50, 0], [9, 20, 60], 1, 1, 64, 16), ([60] * 40, [6] * 40, 4, 2, 128, 24), ([0, 1000], [300, 2], 2, 2, 136, 5)])
+def test_rows_that_a_position_outweighs(dev, gap, past, new, heads, kv, dim, page):
+    for at in (0, 20):
+        c = Sink(np.random.default_rng(dim), [a + b for a, b in zip(past, new)], kv, dim, page, vk.FP16, gap, 0.0, at)
+        rows(dev, c, past, new, heads, "rows")
+
+
 @pytest.mark.parametrize("dtype", [vk.FP16, vk.BF16])
 def test_long_sequences_lack_no_tile(dev, dtype):
     """The sequences of test_paged_weights_cpu.py, whose bounds sixteen positions do not fit into."""

@@ -6,7 +6,9 @@
 // grouped heads a tile has fewer rows of the sequence and the same use of every key that is fetched. One CTA of four warps has a tile;
 // keys and values come through shared memory by cp.async, two tiles ahead, and both products run on mma.sync (m16n8k16, fp32 sums) with
 // a running maximum and sum per row. Probabilities are rounded to 16 bits for the second product, as its operand has to be (relative
-// 2^-12 or 2^-9 each, as much as the rounding of the output); their sum is taken before. Positions that a row does not see are masked
+// 2^-11 or 2^-8 each, as much as the rounding of the output); their sum is taken before. In fp16 they are 2^14 times as large, in sum and output
+// alike, because the format ends at steps of 2^-24: so 2^-11 holds down to 2^-28 of the row's largest, and below each is off by 2^-39 of
+// the largest at most. Positions that a row does not see are masked
 // only in the tiles that some row of the warp does not see whole; a row whose result is not finite is computed again from its own
 // positions (paged_rows.cuh).
 //
@@ -24,6 +26,7 @@ namespace vkl {
 namespace {
 
 constexpr uint32_t kThreads = 128, kRows = 64;
+constexpr float kRaise = 14.f;  // of fp16 probabilities' exponents
 
 template <int DP> struct Cfg {
   static constexpr uint32_t kKeys = DP == 256 ? 32 : 64;  // positions of a tile
@@ -150,13 +153,14 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256
         }
         top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
       }
-    float ref[2];
+    float ref[2], from[2];  // what exponents are taken against, of sums so far and of probabilities
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
       const float now = fmaxf(mx[i], top[i]);
       ref[i] = now == -INFINITY ? 0.f : now;
+      from[i] = BF ? ref[i] : ref[i] - kRaise;
       const float c = exp2f(mx[i] - ref[i]);
       mx[i] = now;
       sum[i] *= c;
@@ -167,7 +171,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256
     for (int n = 0; n < SN; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = exp2f(s[n][e] - ref[e >> 1]);
+        s[n][e] = exp2f(s[n][e] - from[e >> 1]);
         sum[e >> 1] += s[n][e];
       }
 #pragma unroll
