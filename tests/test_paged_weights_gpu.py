@@ -53,6 +53,16 @@ def test_rows_that_a_position_outweighs(dev, gap, past, new, heads, kv, dim, pag
         rows(dev, c, past, new, heads, "rows")
 
 
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("past,new,heads,kv,dim,page", [
+    ([4000], [3], 4, 1, 128, 16), ([200], [600], 1, 1, 64, 16), ([700] * 20, [40] * 20, 8, 8, 64, 16), ([1000, 0], [130, 140], 6, 2, 96, 5)])
+def test_rows_on_the_tensor_cores_that_a_position_outweighs(dev, gap, past, new, heads, kv, dim, page):
+    """Positions in slices and whole, the position that outweighs the others in the first tile and in a later one."""
+    for at in (0, 130):
+        c = Sink(np.random.default_rng(dim), [a + b for a, b in zip(past, new)], kv, dim, page, vk.FP16, gap, 0.0, at)
+        rows(dev, c, past, new, heads, "tensor")
+
+
 @pytest.mark.parametrize("dtype", [vk.FP16, vk.BF16])
 def test_long_sequences_lack_no_tile(dev, dtype):
     """The sequences of test_paged_weights_cpu.py, whose bounds sixteen positions do not fit into."""
