@@ -35,7 +35,8 @@ inline Divisor divisor(uint32_t d) {
 __device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor &v) { return (__umulhi(n, v.mul) + n) >> v.shift; }
 __device__ __forceinline__ void raise(uint32_t *error, uint32_t code) { atomicCAS(error, 0u, code); }
 // Launches may begin before the one in front of them in the stream has ended (launch_following): nothing is read or written before
-// follow() returns, when everything in front has ended and is visible, and the launch behind may be prepared from then on.
+// follow() returns, when everything in front has ended and is visible, and the launch behind may be prepared from then on. What the launch in
+// front may have written is not read-only for the whole of this one, so these kernels have no ld.global.nc (__ldg).
 __device__ __forceinline__ void follow() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");

@@ -68,7 +68,7 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256
       const uint32_t j = t * KT + tid;
       uint32_t r = 0xffffffffu;
       if (t < t1 && j >= j_begin && j <= hi_pos) {
-        const uint32_t n = quotient(j, p.page), page = __ldg(p.table + (size_t)at.seq * p.width + n);
+        const uint32_t n = quotient(j, p.page), page = p.table[(size_t)at.seq * p.width + n];
         if (page < p.pages) r = (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
         else raise(p.error, PAGED_BAD_PAGE);
       }

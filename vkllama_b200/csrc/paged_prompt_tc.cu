@@ -401,7 +401,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       const uint32_t j_last = past + quotient(min(it->at.first + 2 * kRows, packed) - 1, p.group);
       const uint32_t *pages = p.table + (size_t)it->at.seq * p.width;
       auto cache_row = [&](uint32_t j) {  // of position j; behind the last one where there is none
-        const uint32_t n = quotient(j, p.page), page = __ldg(pages + n);
+        const uint32_t n = quotient(j, p.page), page = pages[n];
         if (page < p.pages) return (page * p.kv_heads + kvh) * p.page.d + j - n * p.page.d;
         raise(p.error, PAGED_BAD_PAGE);
         return 0xffffffffu;

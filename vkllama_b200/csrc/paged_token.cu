@@ -225,7 +225,7 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
       entry = kNoSlot;
       if (j >= in.first && j < in.len) {
         const uint32_t n = quotient(j, p.page);
-        entry = __ldg(p.table + (size_t)in.seq * p.width + n);
+        entry = p.table[(size_t)in.seq * p.width + n];
         in_page = j - n * p.page.d;
       }
     };
@@ -288,7 +288,7 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) q[k][e * NR + r] = __ldg(reinterpret_cast<const uint32_t *>(src + min(k * 16 + e * 8 + t4 * 2, p.dim - 2)));
+          for (int e = 0; e < 2; ++e) q[k][e * NR + r] = *reinterpret_cast<const uint32_t *>(src + min(k * 16 + e * 8 + t4 * 2, p.dim - 2));
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll

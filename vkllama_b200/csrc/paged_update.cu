@@ -33,7 +33,7 @@ template <bool BF> __global__ void __launch_bounds__(kThreads) paged_update_kern
     const uint16_t *src = c < nq        ? static_cast<const uint16_t *>(p.q) + row * p.q_ld + c * 8
                           : c < nq + nk ? static_cast<const uint16_t *>(p.k) + row * p.k_ld + (c - nq) * 8
                                         : static_cast<const uint16_t *>(p.v) + row * p.v_ld + (c - nq - nk) * 8;
-    x[i] = ldg_stream(src);
+    x[i] = load_once(src);
   }
   const uint32_t slot = p.map[row], pos = p.map[p.rows + row];
   if (p.turns) {

@@ -40,6 +40,12 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
+// 16 bytes that are read once.
+__device__ __forceinline__ uint4 load_once(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 // 16 bytes from global to shared memory, zeros where `there` is false (nothing is read then).
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
