@@ -8,7 +8,7 @@ from paged_util import HALF_STEP, TINY, Cache, draw, tensor, to_bits, to_values
 
 # The kernels hold a probability relative to a reference that is at most the row's largest, times a power of two, in 16 bits: in fp16 steps
 # end at 2^-24, so that each is off by up to 2^-25 over that power, however small it is.
-FLOOR = {"token": 2.0 ** -39, "rows": 2.0 ** -39, "tensor": 2.0 ** -37}
+FLOOR = {"token": 2.0 ** -39, "rows": 2.0 ** -39, "tensor": 2.0 ** -36}
 # One pair alone is cut over all CTAs and their warps: 70,001 positions into 1,184 parts of four products, which meet eight, sixteen and ten at a time.
 LONG_STEPS = 40
 

@@ -7,9 +7,9 @@
 // products). A CTA stays on its SM and takes one such item after the other by tickets, what takes longest first: a new CTA per item costs some
 // 10 us of start and end, in which nothing else runs (64 prompts of 256: 210 us, this way 107). Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
-//             that it grew by more than 2^8 (fp16: 2^3): until then the probabilities stay below that and O as it is; only then O is multiplied. In fp16,
-//             which ends at steps of 2^-24, they are 2^12 times as large, in sum and O alike: their rounding is relative (2^-11) down to 2^-26
-//             of the row's largest, and below each is off by 2^-37 of the largest at most.
+//             that it grew by more than 2^8 (fp16: 2^4): until then the probabilities stay below that and O as it is; only then O is multiplied. In fp16,
+//             which ends at steps of 2^-24, they are 2^11 times as large, in sum and O alike: their rounding is relative (2^-11) down to 2^-25
+//             of the row's largest, and below each is off by 2^-36 of the largest at most.
 //   8, 9      fetch K_j and V_j into a ring, by tensor copies of boxes of rows and, where pages have none, by cp.async; in the 128-byte
 //             swizzle of the matrix descriptors: K is K-major and V, as it lies in the cache, MN-major (64 dimensions of a position are a
 //             row of 128 bytes in both).
@@ -30,10 +30,10 @@ constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20, kRounds = 64;
 // Where there are fewer items than SMs, an item's positions are split, into slices of at least kSliceTiles tiles; the sums of a row's slices meet
 // in a kernel of their own.
 constexpr uint32_t kSliceTiles = 4, kMostSplits = 32;
-// Octaves that a maximum grows by before the reference follows, and that probabilities are raised by: together 2^15, of 2^16 that fp16 has. (Scores of
-// random numbers hardly ever grow by 2^3 after their first tile; at 2^1 O would be multiplied in most tiles.)
-template <bool BF> constexpr float kGrown = BF ? 8.0f : 3.0f;
-template <bool BF> constexpr float kRaise = BF ? 0.0f : 12.0f;
+// Octaves that a maximum grows by before the reference follows, and that probabilities are raised by: together 2^15, of 2^16 that fp16 has. (Of normally
+// distributed scores, 32 rows of 4096 positions, 0.1 % of the tiles let O be multiplied; with 2^3 2.4 %, and 4096 rows take 165 us instead of 163.)
+template <bool BF> constexpr float kGrown = BF ? 8.0f : 4.0f;
+template <bool BF> constexpr float kRaise = BF ? 0.0f : 11.0f;
 // Registers of a thread: a softmax thread has a row of scores in registers, the other warps give theirs. The sum has to be below what the launch has.
 constexpr uint32_t kSoftmaxRegs = 208, kOtherRegs = 80, kLaunchRegs = kSoftmaxWarps * 32 * kSoftmaxRegs + (kThreads - kSoftmaxWarps * 32) * kOtherRegs;
 
