@@ -1,0 +1,34 @@
+"""Calls on the operators of a paged cache as programs make them: times while other work is queued, captures, tables for long contexts, refusals."""
+import numpy as np
+import pytest
+
+import vkllama_b200 as vk
+from paged_util import Cache, attend, check, draw, tensor, to_values
+
+pytestmark = pytest.mark.gpu
+
+
+def code_of(call):
+    with pytest.raises(vk.VklError) as e:
+        call()
+    return e.value.code
+
+
+def test_items_of_millions_of_positions(dev):
+    """Two rows each behind four million positions, which are one page again and again: half of a CTA's softmax warps have nothing to do as long as that takes. More
+    items than SMs, so that none is split."""
+    n, heads, dim, page, width = 19, 8, 64, 128, 1 << 15
+    rng, cmd = np.random.default_rng(23), vk.Command(dev)
+    c = Cache(rng, [page], heads, dim, page, vk.FP16)
+    bits = draw(rng, (2 * n, heads * dim), vk.FP16)
+    with cmd:
+        k, v, _, _ = c.up(cmd, dev)
+        table = tensor(cmd, dev, np.full((n, width), c.table[0, 0], np.uint32))
+        lens, starts = tensor(cmd, dev, np.full(n, width * page, np.uint32)), tensor(cmd, dev, np.arange(n + 1, dtype=np.uint32) * 2)
+        op = vk.PagedAttention(dev, cmd, heads, heads, dim, page).init()
+        got = to_values(cmd.download(op(tensor(cmd, dev, bits, vk.FP16), k, v, table, lens, starts)), vk.FP16).reshape(2 * n, heads, dim)
+    q = to_values(bits, vk.FP16).reshape(2 * n, heads, dim)
+    want, mass, size = attend(c, 0, q, [page - 1] * (2 * n))  # the one position of four million that the first row does not see counts 2^-22
+    # as tests/paged_weights.py: 2^18 products one after the other, each cut off at 2^-23 of their sum
+    tol = 2.0 ** -11 * np.abs(want) + (4 * (dim + 4) * 2.0 ** -24 * size + 2.0 ** -11 + 2.0 ** -17 + 2.0 ** -5 + 2.0 ** -14) * mass
+    assert (np.abs(got - want) <= tol).all()

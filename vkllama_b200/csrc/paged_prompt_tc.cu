@@ -15,7 +15,8 @@
 //             row of 128 bytes in both).
 //   10        issues the MMAs. They complete in order, so the commit behind S_i(j + 1) also says that P_i(j) V_j is in O_i.
 //   11        takes the tickets and fetches Q, so that queries, keys and values of the next item are there when this one's output is stored.
-// Every wait is bounded; after one that ran out all warps leave, and the error word is raised.
+// Every wait gives up when the CTA has not got on for kPolls polls (items take as long as they have positions, rows that are computed again longer
+// still, so there is no fixed bound); after one that did all warps leave, and the error word is raised.
 #include <algorithm>
 
 #include "paged_rows.cuh"
@@ -26,7 +27,7 @@ namespace {
 
 constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // more than 12 warps would have 128 registers each
 constexpr uint32_t kRows = 128, kKeys = 128;
-constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20, kRounds = 64;
+constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20;
 // Where there are fewer items than SMs, an item's positions are split, into slices of at least kSliceTiles tiles; the sums of a row's slices meet
 // in a kernel of their own.
 constexpr uint32_t kSliceTiles = 4, kMostSplits = 32;
@@ -52,8 +53,8 @@ template <int DP> struct Cfg {
   struct Shared {  // behind the tiles
     uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4], item_full[2], item_empty[2], fetched, drained;
     Item items[2];
-    uint32_t tmem;
-    volatile uint32_t failed, slow;  // slow: rows have been computed again
+    uint32_t tmem, beat;  // beat: counted up by tiles requested, sequences looked at, positions of rows computed again
+    volatile uint32_t failed;
   };
   static constexpr uint32_t kSmem = (2 + kStages) * kTile + sizeof(Shared);
   static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA per SM");
@@ -172,7 +173,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
     init(&sh.drained, 1);
     for (uint32_t i = 0; i < 8; ++i) init(&sh.turn[i >> 2][i & 3], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    sh.failed = sh.slow = 0;
+    sh.failed = sh.beat = 0;
   }
   if (warp == kMmaWarp) tmem_alloc<512>(sa(&sh.tmem));
   tc_before();
@@ -181,29 +182,34 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
   follow();
   if (p.part != 2) stamp_begin(p.stamps);  // else the launch in front of this one did
   const uint32_t tmem = sh.tmem, q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
-  // Waits, false when they ran out: after kPolls, or after kRounds times as many in a CTA that has computed rows again (below), which takes as long as it
-  // takes. The loop is one statement, with nothing behind a wait that is over: these instructions are between every two steps of a tile (checks in C++
-  // behind it: 108 us where 103 are possible).
+  // Waits, false when they ran out. The loop is one statement, with nothing behind a wait that is over: these instructions are between every two steps of a
+  // tile (checks in C++ behind it: 108 us where 103 are possible).
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p, q;\n .reg .u32 n, m;\n mov.u32 n, %3;\n"
-        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n and.b32 m, n, %4;\n setp.ne.u32 q, m, 0;\n @q bra again;\n"
-        " ld.volatile.shared.u32 m, [%5];\n setp.eq.u32 q, m, 0;\n @q bra there;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
+        "{\n .reg .pred p, q;\n .reg .u32 n, m, seen;\n mov.u32 n, 0;\n"
+        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n and.b32 m, n, %3;\n setp.ne.u32 q, m, 0;\n @q bra again;\n"
+        " ld.volatile.shared.u32 m, [%4];\n setp.eq.u32 q, n, %5;\n @q mov.u32 seen, 0;\n setp.ne.u32 q, m, seen;\n mov.u32 seen, m;\n @q bra again;\n"
         "there:\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
-        : "r"(sa(bar)), "r"(parity), "n"(kPolls * kRounds), "n"(kPolls - 1), "r"(sa(const_cast<uint32_t *>(&sh.slow)))
+        : "r"(sa(bar)), "r"(parity), "n"(kPolls - 1), "r"(sa(&sh.beat)), "n"(0u - kPolls)
         : "memory");
     if (!ok) sh.failed = 1;
     return ok != 0;
   };
   // For waits that are long by design: a warp that polls takes issue slots from the softmax warps of its scheduler (the ticket warp alone
-  // cost a third of the rate). That one waits for whole items, which may have millions of positions.
-  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns, bool item = false) {
-    uint32_t ok = 0;
-    for (uint32_t n = 0; !ok && n < (item || sh.slow ? kPolls * kRounds : kPolls); ++n) {
+  // cost a third of the rate).
+  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns) {
+    uint32_t ok = 0, seen = 0;
+    for (uint32_t n = 1;; ++n) {
       asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(sa(bar)), "r"(parity) : "memory");
-      if (!ok) __nanosleep(ns);
+      if (ok) break;
+      __nanosleep(ns);
+      if (n % kPolls == 0) {
+        const uint32_t now = *const_cast<volatile uint32_t *>(&sh.beat);
+        if (now == seen) break;
+        seen = now;
+      }
     }
     if (!ok) sh.failed = 1;
     return __all_sync(0xffffffffu, ok) != 0;
@@ -362,8 +368,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
           }
           uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f && r < packed);  // NaN
           __syncwarp();
-          if (again) sh.slow = 1;
-          for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
+          for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP, &sh.beat);
         }
       }
       if (i == 0 && tiles == 2 && both_e > both_b) turn ^= 1;  // the other tile's last turn, which nobody waits for
@@ -422,6 +427,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
         const uint32_t copied = last > first ? last - first - (r1 > r0 && box ? 1 : 0) : 0;
         if (t1 - t == min(t1 - t0, 2u) && lane == 0) arrive(sa(&sh.fetched));  // the next ticket may be taken
         if (x >= C::kStages && !(ok = wait_idle(&empty[pos.s], pos.phase ^ 1, 64))) break;
+        get_on(&sh.beat);
         const uint32_t dst = ring_a + pos.s * C::kTile, bar = sa(&full[pos.s]);
         const bool pieces = r1 > r0;
         if (copied) {
@@ -540,9 +546,10 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
   } else {
     // ------------------------------------------------- what comes next, once two tiles of this item are left to request: a ticket taken much earlier
     // could have been another CTA's, which has nothing left to do (106 -> 158 us for a few long items)
-    if (blockIdx.x == 0) check_rows(p);
+    if (blockIdx.x == 0) check_rows(p, &sh.beat);
     uint32_t used[2] = {};  // how often each tile's place for Q
     Walk walk;
+    walk.beat = &sh.beat;
     uint32_t ticket = blockIdx.x;  // the first ones are dealt out
     auto take = [&]() {
       uint32_t next = 0;
@@ -550,8 +557,8 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       return __shfl_sync(0xffffffffu, next, 0);
     };
     for (uint32_t k = 0;; ++k) {
-      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200, true)) break;
-      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200, true)) break;
+      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200)) break;
+      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200)) break;
       if (k) ticket = take();
       Item it = {};
       for (;; ticket = take()) {
@@ -585,7 +592,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       // and is not stored), else piece by piece
       bool ok = true;
       for (uint32_t i = 0; ok && i < it.tiles; ++i) {
-        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64, true))) break;
+        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64))) break;
         ++used[i];
         const uint32_t dst = q_a + i * C::kTile, bar = sa(&q_full[i]), r0 = it.at.first + i * kRows;
         if (q_box) {
