@@ -32,3 +32,26 @@ def test_items_of_millions_of_positions(dev):
     # as tests/paged_weights.py: 2^18 products one after the other, each cut off at 2^-23 of their sum
     tol = 2.0 ** -11 * np.abs(want) + (4 * (dim + 4) * 2.0 ** -24 * size + 2.0 ** -11 + 2.0 ** -17 + 2.0 ** -5 + 2.0 ** -14) * mass
     assert (np.abs(got - want) <= tol).all()
+
+
+def test_time_of_a_run_that_is_over_while_others_are_queued(dev):
+    """As of the other ops: what counts is the op's own last run."""
+    rng, cmd = np.random.default_rng(20), vk.Command(dev)
+    c = Cache(rng, [60000], 2, 128, 16, vk.FP16)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        q = tensor(cmd, dev, draw(rng, (1, 256), vk.FP16), vk.FP16)
+        op, other = (vk.PagedAttention(dev, cmd, 2, 2, 128, 16).init() for _ in range(2))
+        op(q, k, v, table, lens)
+    took = op.time()
+    assert 2 <= took < 1000
+    cmd.begin()
+    for _ in range(2000):
+        other(q, k, v, table, lens)
+    assert op.time() == took
+    assert code_of(other.time) == 9  # its own has not finished
+    op(q, k, v, table, lens)
+    assert code_of(op.time) == 9
+    cmd.end()
+    cmd.submit_and_wait()
+    assert 2 <= op.time() < 1000 and 2 <= other.time() < 1000

@@ -24,8 +24,18 @@ struct OnDevice {
   }
 };
 
+// A stream for what has to be done at once, beside the command's.
+struct OwnStream {
+  cudaStream_t s = nullptr;
+  cudaError_t open() { return cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking); }
+  ~OwnStream() {
+    if (s) cudaStreamDestroy(s);
+  }
+};
+
 struct PagedOp : vkl_op {
   vkl_tensor *stamps = nullptr;  // of the last launch (paged.h), in the place of the other ops' events
+  uint64_t run_in = 0;           // the command's waits before the last launch
   using vkl_op::vkl_op;
   ~PagedOp() override { vkl_tensor_release(stamps); }
   int paged_init() {
@@ -43,18 +53,25 @@ struct PagedOp : vkl_op {
   }
   unsigned long long *stamp() {
     timed = true;
+    run_in = cmd->waits;
     return (unsigned long long *)stamps->data();
   }
   int elapsed(uint64_t *usec) override {
     *usec = 0;
     if (!timed) return VKL_OK;
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;  // a query would end a capture
-    if (cudaStreamIsCapturing(cmd->stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone || cudaStreamQuery(cmd->stream) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return fail(VKL_FAILED_PRECONDITION, "op_time: the op's last run has not finished (wait on its command first)");
+    OnDevice here(dev->ordinal);
+    if (cmd->waits == run_in) {  // not waited for since: over where the stream has nothing left
+      cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;  // a query would end a capture
+      if (cudaStreamIsCapturing(cmd->stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone || cudaStreamQuery(cmd->stream) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return fail(VKL_FAILED_PRECONDITION, "op_time: the op's last run has not finished (wait on its command first)");
+      }
     }
     unsigned long long t[2];
-    VKL_CUDA(cudaMemcpy(t, stamps->data(), 16, cudaMemcpyDeviceToHost));
+    OwnStream own;  // not behind what the command's has, nor in the way of other streams
+    VKL_CUDA(own.open());
+    VKL_CUDA(cudaMemcpyAsync(t, stamps->data(), 16, cudaMemcpyDeviceToHost, own.s));
+    VKL_CUDA(cudaStreamSynchronize(own.s));
     *usec = t[1] > t[0] ? (t[1] - t[0] + 500) / 1000 : 0;
     return VKL_OK;
   }

@@ -425,6 +425,7 @@ int vkl_command_wait(vkl_command *cmd) {
   cmd->deferred.clear();
   for (auto &f : tasks) f();
   if (e != cudaSuccess) return fail(VKL_INTERNAL, "command_wait: %s", cudaGetErrorString(e));
+  ++cmd->waits;
   if (watched && *cmd->err_host) {
     cudaMemsetAsync(cmd->err_word, 0, 4, cmd->stream);
     switch (*cmd->err_host) {

@@ -117,6 +117,7 @@ struct vkl_command {
   uint32_t *err_word = nullptr;  // device word raised by a kernel whose bounded wait ran out; read by wait()
   uint32_t *err_host = nullptr;  // pinned: where it is read to
   bool err_used = false;
+  uint64_t waits = 0;            // how often wait() has found everything over
 };
 
 namespace vkl {
