@@ -55,3 +55,37 @@ def test_time_of_a_run_that_is_over_while_others_are_queued(dev):
     cmd.end()
     cmd.submit_and_wait()
     assert 2 <= op.time() < 1000 and 2 <= other.time() < 1000
+
+
+def test_a_shape_that_is_captured_first(dev):
+    """Its workspace is zero for the first direct call too, which comes before any replay."""
+    torch = pytest.importorskip("torch")
+    rng, cmd = np.random.default_rng(21), vk.Command(dev)
+    heads, kv, dim, page, past, new = 8, 1, 64, 16, (6000, 100), 40  # the second one's positions are not split
+    c = Cache(rng, [a + new for a in past], kv, dim, page, vk.FP16)
+    bits = draw(rng, (2 * new, heads * dim), vk.FP16)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        args = (tensor(cmd, dev, bits, vk.FP16), k, v, table, lens, tensor(cmd, dev, np.array([0, new, 2 * new], np.uint32)))
+        used = [vk.Tensor(1, 1, 1 << x, dev, vk.FP32) for x in range(14, 24)]  # memory that the workspace may get
+        for t in used:
+            cmd.upload(np.full(t.shape(), 7, np.float32), t)
+        op = vk.PagedAttention(dev, cmd, heads, kv, dim, page).init()
+    del used, t
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.ExternalStream(cmd.stream())
+    cmd.begin()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+        out = op(*args)
+    cmd.end()
+    with cmd:
+        direct = cmd.download(op(*args))
+    with torch.cuda.stream(stream):
+        graph.replay()
+    stream.synchronize()
+    with cmd:
+        assert (cmd.download(out) == direct).all()
+    q, got = (to_values(a, vk.FP16).reshape(2, new, heads, dim) for a in (bits, direct))
+    for i in range(2):
+        want, mass, size = attend(c, i, q[i], list(range(past[i], past[i] + new)))
+        check(got[i], want, mass, size, vk.FP16, dim, past[i] + new, 5.0, True, str(i))
+    del graph

@@ -276,7 +276,7 @@ struct PagedAttentionOp : PagedOp {
     VKL_CUDA(cudaMemsetAsync(counters->data(), 0, counters->device_bytes(), cmd->stream));
     return paged_init();
   }
-  // Room for n numbers, all 0 if it is new. It grows by powers of two.
+  // Room for n numbers, all 0 if it is new: at once, for a call that is being captured would only put that into its graph. It grows by powers of two.
   int room(vkl_tensor **t, size_t n) {
     if (*t && (*t)->w >= n) return VKL_OK;
     size_t more = 1 << 16;
@@ -287,7 +287,10 @@ struct PagedAttentionOp : PagedOp {
       *t = nullptr;
     }
     VKL_OKAY(ensure_tensor(dev, t, 1, 1, more, VKL_FP32));
-    VKL_CUDA(cudaMemsetAsync((*t)->data(), 0, more * 4, cmd->stream));
+    OwnStream own;
+    VKL_CUDA(own.open());
+    VKL_CUDA(cudaMemsetAsync((*t)->data(), 0, more * 4, own.s));
+    VKL_CUDA(cudaStreamSynchronize(own.s));
     return VKL_OK;
   }
   int run(vkl_tensor *q, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *table, vkl_tensor *lengths, vkl_tensor *starts, vkl_tensor **o) {
