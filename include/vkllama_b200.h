@@ -240,7 +240,8 @@ int vkl_update_paged_kvcache_run(vkl_op *op, vkl_tensor *kcache, vkl_tensor *vca
  * kv_heads, query head h reads key head h / (heads / kv_heads). scale 0: 1 / sqrt(dim). window > 0: a token sees the last `window`
  * positions up to its own. fp32 sums and softmax, one rounding of the output (with `starts` also of the probabilities, to dtype).
  *   starts NULL: one new token per sequence, q [1, n, heads * dim], row i the last token of sequence i (position lengths[i] - 1); a sequence
- *   of no tokens gives zeros.
+ *   of no tokens gives zeros. Up to 2^35 tokens of all sequences times key heads (times eights of query heads, where one has more than eight); the
+ *   device refuses a call of more than it can count (OUT_OF_RANGE), by lengths, not by what the table could hold.
  *   else q [1, rows, heads * dim]: sequence i's new tokens are the last starts[i + 1] - starts[i] of its lengths[i]; each sees the
  *   positions up to its own. Sequences without new rows are skipped; output rows that belong to no sequence are left as they were.
  * q may be a view of wider rows (16-byte row starts). Values at positions that a row does not see never reach it, whatever they are;

@@ -89,3 +89,30 @@ def test_a_shape_that_is_captured_first(dev):
         want, mass, size = attend(c, i, q[i], list(range(past[i], past[i] + new)))
         check(got[i], want, mass, size, vk.FP16, dim, past[i] + new, 5.0, True, str(i))
     del graph
+
+@pytest.mark.parametrize("heads", [32, 300])
+def test_tables_that_could_hold_more_than_is_counted(dev, heads):
+    """2300 sequences with room for a million tokens each: lengths decide. Beyond 2^31 tiles the call is refused on the device and writes nothing."""
+    n, page, width, dim, kv = 2300, 64, 16384, 8, 32 if heads == 32 else 30
+    rng, cmd = np.random.default_rng(22), vk.Command(dev)
+    c = Cache(rng, [int(x) for x in rng.integers(0, 40, n)], kv, dim, page, vk.FP16, spare=1)
+    c.table = np.pad(c.table, ((0, 0), (0, width - c.table.shape[1])))
+    bits = draw(rng, (n, heads * dim), vk.FP16)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        q = tensor(cmd, dev, bits, vk.FP16)
+        op = vk.PagedAttention(dev, cmd, heads, kv, dim, page).init()
+        got = cmd.download(op(q, k, v, table, lens))
+    q_ = to_values(bits, vk.FP16).reshape(n, heads, dim)
+    for i in range(0, n, 17):
+        l = c.lengths[i]
+        want, mass, size = attend(c, i, q_[i:i + 1], [l - 1])
+        check(to_values(got, vk.FP16).reshape(n, heads, dim)[i:i + 1], want, mass, size, vk.FP16, dim, l, 5.0, False, str(i))
+    cmd.begin()
+    assert n * kv * width * page // 32 > 2 ** 31
+    out = op(q, k, v, table, tensor(cmd, dev, np.full(n, width * page, np.uint32)))
+    cmd.end()
+    assert code_of(cmd.submit_and_wait) == 11
+    with cmd:
+        assert (cmd.download(out) == got).all()
+        assert (cmd.download(op(q, k, v, table, lens)) == got).all()

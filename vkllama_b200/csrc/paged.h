@@ -20,6 +20,7 @@ enum PagedError : uint32_t {
   PAGED_POOL_BAD,            // tables: the pool's count and what comes back do not fit it
   PAGED_BAD_PAGE,            // a page that the cache does not have
   PAGED_BAD_ROWS,            // attention: starts and lengths do not belong together
+  PAGED_TOO_MUCH,            // attention of one token: tiles of positions beyond 31 bits
 };
 
 // n / d for n < 2^31 by a multiplication.
@@ -122,6 +123,7 @@ struct PagedAttention {
   float scale;                  // on the scores
   bool bf;
   uint32_t splits;              // parts of a sequence's positions at most
+  bool count;                   // one token: the tables could hold more tiles than are counted in 31 bits, so the lengths have to be added up first
   uint32_t part;                // of a prompt call's sequences, those that the launch takes: 0 all, 1 or 2 by paged_rows.cuh's rule
 };
 // One new token per sequence.

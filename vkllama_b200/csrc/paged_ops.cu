@@ -306,8 +306,7 @@ struct PagedAttentionOp : PagedOp {
     if (starts) VKL_OKAY(check_list(starts, who, "starts", n + 1));
     if (!starts && rows != n) return fail(VKL_INVALID_ARGUMENT, "%s: %zu queries for %zu sequences of one new token each", who, rows, n);
     VKL_OKAY(check_apart(q, who, "queries"));
-    // the one-token form counts tiles of 16 positions of all sequences and head groups in 31 bits
-    if (rows * per > kMaxTokens || n > kMaxTokens || (rows * per / 64 + n) * kv_heads > kMaxTokens || (!starts && n * (table->w * page / 16 + 2) * (kv_heads * ((per + 7) / 8)) > kMaxTokens))
+    if (rows * per > kMaxTokens || n > kMaxTokens || (rows * per / 64 + n) * kv_heads > kMaxTokens)
       return fail(VKL_OUT_OF_RANGE, "%s: %zu rows, %zu sequences of up to %zu tokens", who, rows, n, table->w * page);
     VKL_OKAY(begin(who));
     if (out && q->data() == out->data()) return fail(VKL_INVALID_ARGUMENT, "%s: the queries are this op's own output", who);
@@ -331,6 +330,8 @@ struct PagedAttentionOp : PagedOp {
       p.group = divisor((uint32_t)per);
       p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)dim);
       p.bf = dtype == VKL_BF16;
+      // the one-token form counts tiles of 16 or 32 positions of all sequences and head groups in 31 bits
+      p.count = !starts && table->w * page / 16 + 2 > kMaxTokens / (n * kv_heads * ((per + 7) / 8));
       p.splits = starts ? paged_prompt_splits(p, sms) : 1;
       if (p.splits > 1) {
         const size_t parts = p.splits * rows * heads;

@@ -88,7 +88,7 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
   constexpr uint32_t T = C::kTile, NC = T * CH / 32;  // pieces of a half and lane
   constexpr int KS = DP / 16, NT = DP / 8, SN = T / 8;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ uint32_t before_s[kThreads + 1];  // tiles of one head group's sequences; the host has checked that they fit 32 bits
+  __shared__ uint32_t before_s[kThreads + 1];  // tiles of one head group's sequences, which fit 31 bits over all groups (the host knows, or p.count)
   __shared__ uint32_t warp_sum_s[kWarps];
   __shared__ uint32_t border_s[2], cut_s[2][2];  // the range's ends, and the first and last cut of the pairs that they cut
   __shared__ Part part_s[kWarps][2];
@@ -110,6 +110,19 @@ template <bool BF, int DP, bool WIDE> __global__ void __launch_bounds__(Cfg<DP, 
   // A pair's tiles, and the places that it takes up in the row of all work.
   auto tiles = [&](uint32_t len) { return max((len + T - 1) / T, 1u) - first_of(len) / T; };
   auto places = [&](uint32_t len) { return tiles(len) + kPairCost; };
+  if (p.count) {
+    __shared__ unsigned long long all_s;
+    if (tid == 0) all_s = 0;
+    __syncthreads();
+    unsigned long long all = 0;
+    for (uint32_t i = tid; i < p.n; i += kThreads) all += places(length(i));
+    atomicAdd(&all_s, all);
+    __syncthreads();
+    if (all_s > 0x7fffffffu / pairs) {
+      if (blockIdx.x == 0 && tid == 0) raise(p.error, PAGED_TOO_MUCH);
+      return;
+    }
+  }
   const uint32_t each = (p.n + kThreads - 1) / kThreads;
   {
     const uint32_t i0 = min(tid * each, p.n), i1 = min(i0 + each, p.n);
@@ -638,8 +651,8 @@ template <bool BF, int DP, bool WIDE> cudaError_t run(const PagedAttention &p, u
   using C = Cfg<DP, WIDE>;
   // No more CTAs than there can be shares of.
   const uint64_t per = p.heads / p.kv_heads, pairs = (uint64_t)p.kv_heads * ((per + C::kHeads - 1) / C::kHeads);
-  const uint64_t most = p.n * pairs * (((uint64_t)p.width * p.page.d + C::kTile - 1) / C::kTile + kPairCost), shares = (most + C::kShare - 1) / C::kShare;
-  return launch_following(paged_token_kernel<BF, DP, WIDE>, dim3((uint32_t)std::min<uint64_t>(sms, shares)), C::kThreads, C::kSmem, s, p);
+  const double most = (double)p.n * pairs * (((uint64_t)p.width * p.page.d + C::kTile - 1) / C::kTile + kPairCost), shares = (most + C::kShare - 1) / C::kShare;
+  return launch_following(paged_token_kernel<BF, DP, WIDE>, dim3((uint32_t)std::min<double>(sms, shares)), C::kThreads, C::kSmem, s, p);
 }
 bool wide(uint32_t heads, uint32_t kv_heads) { return heads / kv_heads > 8; }  // more query heads than the narrow form's rows
 template <bool BF> cudaError_t pick(const PagedAttention &p, uint32_t sms, cudaStream_t s) {

@@ -434,6 +434,7 @@ int vkl_command_wait(vkl_command *cmd) {
       case PAGED_ROWS: return fail(VKL_OUT_OF_RANGE, "command_wait: paged_tables: more new tokens than rows; nothing was changed");
       case PAGED_POOL_BAD: return fail(VKL_FAILED_PRECONDITION, "command_wait: paged_tables: the pool holds more pages than it has room for; nothing was changed");
       case PAGED_BAD_PAGE: return fail(VKL_OUT_OF_RANGE, "command_wait: a page that the cache does not have was named");
+      case PAGED_TOO_MUCH: return fail(VKL_OUT_OF_RANGE, "command_wait: paged_attention: the sequences' tiles of 16 or 32 positions, of every key head, are more than 2^31 - 1");
       case PAGED_BAD_ROWS: return fail(VKL_INVALID_ARGUMENT, "command_wait: paged_attention: starts, lengths and rows do not belong together");
     }
     return fail(VKL_INTERNAL, "command_wait: a bounded wait inside a kernel ran out (code %u)", *cmd->err_host);
