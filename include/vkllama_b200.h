@@ -231,7 +231,7 @@ int vkl_paged_tables_run(vkl_op *op, vkl_tensor *lengths, vkl_tensor *target, vk
 /* UpdatePagedKVCache: writes the rows k, v [1, rows, kv_heads * dim] to their slots, the keys rotated by their positions as Rope rotates
  * (neighbouring pairs, angle position * theta^(-2k/dim), angles in 64 bits); theta 0: not rotated. Rows without a slot are not written.
  * q [1, rows, heads * dim], or NULL: rotated into the op's output (rows without a slot by their map's position as well). k, v and q may be views of wider
- * rows whose rows start at multiples of 16 bytes. Slots of one call must differ: of two rows with one slot either may be
+ * rows whose rows start at multiples of 16 bytes; q may be the op's output (turned in its place), k and v not. Slots of one call must differ: of two rows with one slot either may be
  * stored, piece by piece. dim: a multiple of 8 up to 256. */
 int vkl_update_paged_kvcache_create(vkl_device *dev, vkl_command *cmd, int dim, int page_size, float theta, int dtype, vkl_op **out);
 int vkl_update_paged_kvcache_run(vkl_op *op, vkl_tensor *kcache, vkl_tensor *vcache, vkl_tensor *k, vkl_tensor *v, vkl_tensor *map,

@@ -116,3 +116,25 @@ def test_tables_that_could_hold_more_than_is_counted(dev, heads):
     with cmd:
         assert (cmd.download(out) == got).all()
         assert (cmd.download(op(q, k, v, table, lens)) == got).all()
+
+
+def test_an_update_on_its_own_output(dev):
+    """Queries are turned in their place; keys and values that other threads would store over meanwhile are refused."""
+    rng, cmd = np.random.default_rng(24), vk.Command(dev)
+    rows, dim, page = 40, 64, 16
+    x, m = draw(rng, (rows, 4 * dim), vk.FP16), np.stack([np.arange(rows), np.arange(rows)]).astype(np.uint32)
+    with cmd:
+        kc, vc = (tensor(cmd, dev, np.zeros((3, 4 * page, dim), np.uint16), vk.FP16) for _ in range(2))
+        q, k, mt = tensor(cmd, dev, x, vk.FP16), tensor(cmd, dev, x, vk.FP16), tensor(cmd, dev, m)
+        op, other = (vk.UpdatePagedKVCache(dev, cmd, dim, page).init() for _ in range(2))
+        out = op(kc, vc, k, k, mt, q)
+        once = cmd.download(out)
+        want = cmd.download(other(kc, vc, k, k, mt, tensor(cmd, dev, once[0], vk.FP16)))
+        assert op(kc, vc, k, k, mt, out) is out and (cmd.download(out) == want).all()
+        assert code_of(lambda: op(kc, vc, out, k, mt, q)) == 3
+        assert code_of(lambda: op(kc, vc, k, out, mt, q)) == 3
+        assert code_of(lambda: op(kc, vc, out.view(1, rows, 4 * dim), k, mt, out)) == 3
+        assert op(kc, vc, out, out, mt) is None  # nothing is stored there
+        got = cmd.download(vc).reshape(3, 4, page, dim)
+    at = np.arange(rows)
+    assert (got[at // page, :, at % page].reshape(rows, -1) == want[0]).all()

@@ -219,6 +219,8 @@ struct UpdatePagedOp : PagedOp {
     if (kcache->data() == vcache->data()) return fail(VKL_INVALID_ARGUMENT, "%s: keys and values have one cache", who);
     if ((q ? q->w : 0) + 2 * k->w > 1u << 24) return fail(VKL_OUT_OF_RANGE, "%s: rows of %zu values", who, (q ? q->w : 0) + 2 * k->w);
     VKL_OKAY(begin(who));
+    // queries may be turned in their place; keys and values would be read while other threads store there
+    if (q && out && (k->data() == out->data() || v->data() == out->data())) return fail(VKL_INVALID_ARGUMENT, "%s: keys or values are this op's own output", who);
     if (q) VKL_OKAY(ensure_tensor(dev, &out, 1, rows, q->w, dtype));
     if (rows) {
       PagedUpdate p = {};
