@@ -138,3 +138,77 @@ def test_an_update_on_its_own_output(dev):
         got = cmd.download(vc).reshape(3, 4, page, dim)
     at = np.arange(rows)
     assert (got[at // page, :, at % page].reshape(rows, -1) == want[0]).all()
+
+
+@pytest.mark.parametrize("bad", ["page", "length", "short", "order"])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("lengths,new,launches", [([300, 200, 260], [100, 80, 90], 1), ([300, 140, 260, 40], [2, 3, 1, 5], 2), ([3000, 2500, 40], [5, 4, 2], 3)])
+def test_bad_rows_of_several_kernels(dev, bad, page, lengths, new, launches):
+    """The tcgen05 kernel alone, both kernels, split positions: what is wrong with the second sequence is reported, the others' rows are right, and so is the
+    next call."""
+    heads, kv, dim, dtype = 4, 2, 64, vk.BF16
+    rng, cmd = np.random.default_rng(25), vk.Command(dev)
+    c = Cache(rng, lengths, kv, dim, page, dtype)
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.uint32)
+    bits = draw(rng, (starts[-1], heads * dim), dtype)
+    q_ = to_values(bits, dtype).reshape(-1, heads, dim)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        q, good = tensor(cmd, dev, bits, dtype), tensor(cmd, dev, starts)
+        op = vk.PagedAttention(dev, cmd, heads, kv, dim, page, dtype=dtype).init()
+    wrong_table, wrong_lengths, wrong_starts = c.table.copy(), np.array(lengths, np.uint32), starts.copy()
+    if bad == "page":
+        wrong_table[1, 3], wrong_table[1, 7] = c.pages, 0xffffffff
+    elif bad == "length":
+        wrong_lengths[1] = c.table.shape[1] * page + 1
+    elif bad == "short":
+        wrong_lengths[1] = new[1] - 1
+    else:
+        wrong_starts[2] = 0
+    for first in (True, False):
+        before = vk.kernel_launches()
+        cmd.begin()
+        if first:
+            wrong = [tensor(cmd, dev, a) for a in (wrong_table, wrong_lengths, wrong_starts)]
+            got = cmd.download(op(q, k, v, *wrong))
+        else:
+            got = cmd.download(op(q, k, v, table, lens, good))
+        cmd.end()
+        assert vk.kernel_launches() - before == launches
+        if first:
+            assert code_of(cmd.submit_and_wait) == (11 if bad == "page" else 3)
+        else:
+            cmd.submit_and_wait()
+        got = to_values(got, dtype).reshape(-1, heads, dim)
+        for i, l in enumerate(lengths):
+            if first and (i == 1 or bad == "order"):  # rows of the others are the second's too there
+                continue
+            mine = slice(starts[i], starts[i + 1])
+            want, mass, size = attend(c, i, q_[mine], list(range(l - new[i], l)))
+            check(got[mine], want, mass, size, dtype, dim, l, 5.0, True, str(i))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(12, 1, 128), (4, 2, 64), (16, 1, 200)])
+def test_bad_pages_of_single_tokens(dev, heads, kv, dim):
+    """In a sequence that several CTAs share, up to eight heads a key head and beyond."""
+    rng, cmd, page = np.random.default_rng(26), vk.Command(dev), 16
+    c = Cache(rng, [3000, 50, 4000], kv, dim, page, vk.FP16)
+    bits = draw(rng, (3, heads * dim), vk.FP16)
+    q_ = to_values(bits, vk.FP16).reshape(3, heads, dim)
+    wrong = c.table.copy()
+    wrong[0, 11], wrong[0, 150] = 0xffffffff, c.pages
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        q, bad = tensor(cmd, dev, bits, vk.FP16), tensor(cmd, dev, wrong)
+        op = vk.PagedAttention(dev, cmd, heads, kv, dim, page).init()
+    for t, which in ((bad, (1, 2)), (table, (0, 1, 2))):
+        cmd.begin()
+        got = to_values(cmd.download(op(q, k, v, t, lens)), vk.FP16).reshape(3, heads, dim)
+        cmd.end()
+        if t is bad:
+            assert code_of(cmd.submit_and_wait) == 11
+        else:
+            cmd.submit_and_wait()
+        for i in which:
+            want, mass, size = attend(c, i, q_[i:i + 1], [c.lengths[i] - 1])
+            check(got[i:i + 1], want, mass, size, vk.FP16, dim, c.lengths[i], 5.0, False, str(i))
