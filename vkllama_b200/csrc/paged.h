@@ -121,9 +121,8 @@ struct PagedAttention {
   uint32_t rows, n, heads, kv_heads, dim, width, pages, window;
   Divisor page, group;          // query heads of a key head
   float scale;                  // on the scores
-  bool bf;
+  bool bf, count;               // count (one token): the tables could hold more tiles than 31 bits count, so the lengths have to be added up first
   uint32_t splits;              // parts of a sequence's positions at most
-  bool count;                   // one token: the tables could hold more tiles than are counted in 31 bits, so the lengths have to be added up first
   uint32_t part;                // of a prompt call's sequences, those that the launch takes: 0 all, 1 or 2 by paged_rows.cuh's rule
 };
 // One new token per sequence.

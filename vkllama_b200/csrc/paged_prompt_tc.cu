@@ -15,8 +15,8 @@
 //             row of 128 bytes in both).
 //   10        issues the MMAs. They complete in order, so the commit behind S_i(j + 1) also says that P_i(j) V_j is in O_i.
 //   11        takes the tickets and fetches Q, so that queries, keys and values of the next item are there when this one's output is stored.
-// Every wait gives up when the CTA has not got on for kPolls polls (items take as long as they have positions, rows that are computed again longer
-// still, so there is no fixed bound); after one that did all warps leave, and the error word is raised.
+// Every wait is bounded: a step's after some seconds, an item's, and all of a CTA that computes rows again, after minutes (for items of up to 2^31
+// positions, and rows of some ten million), or when another one has run out. Then all warps leave, and the error word is raised.
 #include <algorithm>
 
 #include "paged_rows.cuh"
@@ -27,7 +27,7 @@ namespace {
 
 constexpr uint32_t kSoftmaxWarps = 8, kFetchWarps = 2, kMmaWarp = 10, kThreads = 12 * 32;  // more than 12 warps would have 128 registers each
 constexpr uint32_t kRows = 128, kKeys = 128;
-constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20;
+constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20, kRounds = 64, kLongPolls = 1u << 30;
 // Where there are fewer items than SMs, an item's positions are split, into slices of at least kSliceTiles tiles; the sums of a row's slices meet
 // in a kernel of their own.
 constexpr uint32_t kSliceTiles = 4, kMostSplits = 32;
@@ -53,8 +53,9 @@ template <int DP> struct Cfg {
   struct Shared {  // behind the tiles
     uint64_t q_full[2], q_empty[2], full[kStages], empty[kStages], s_full[2], p_full[2][2], o_full[2], turn[2][4], item_full[2], item_empty[2], fetched, drained;
     Item items[2];
-    uint32_t tmem, beat;  // beat: counted up by tiles requested, sequences looked at, positions of rows computed again
-    volatile uint32_t failed;
+    uint32_t tmem;
+    // going: 0 once a wait has run out; slow: rows have been computed again. Words that, where they are not 0, make waits long.
+    volatile uint32_t going, slow;
   };
   static constexpr uint32_t kSmem = (2 + kStages) * kTile + sizeof(Shared);
   static_assert(kSmem > 114 * 1024 && kSmem <= 227 * 1024, "one CTA per SM");
@@ -173,7 +174,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
     init(&sh.drained, 1);
     for (uint32_t i = 0; i < 8; ++i) init(&sh.turn[i >> 2][i & 3], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    sh.failed = sh.beat = 0;
+    sh.going = 1, sh.slow = 0;
   }
   if (warp == kMmaWarp) tmem_alloc<512>(sa(&sh.tmem));
   tc_before();
@@ -182,42 +183,37 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
   follow();
   if (p.part != 2) stamp_begin(p.stamps);  // else the launch in front of this one did
   const uint32_t tmem = sh.tmem, q_a = sa(smem), ring_a = q_a + 2 * C::kTile;
-  // Waits, false when they ran out. The loop is one statement, with nothing behind a wait that is over: these instructions are between every two steps of a
-  // tile (checks in C++ behind it: 108 us where 103 are possible).
-  auto wait = [&](uint64_t *bar, uint32_t parity) {
+  // Waits, false when they ran out: after kPolls (4 us each: try_wait sleeps), or after kRounds times as many as long as the word `longer` is not 0.
+  // The loop is one statement, with nothing behind a wait that is over: these instructions are between every two steps of a tile (checks in C++
+  // behind it: 108 us where 103 are possible).
+  auto wait = [&](uint64_t *bar, uint32_t parity, const volatile uint32_t &longer) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p, q;\n .reg .u32 n, m, seen;\n mov.u32 n, 0;\n"
-        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n and.b32 m, n, %3;\n setp.ne.u32 q, m, 0;\n @q bra again;\n"
-        " ld.volatile.shared.u32 m, [%4];\n setp.eq.u32 q, n, %5;\n @q mov.u32 seen, 0;\n setp.ne.u32 q, m, seen;\n mov.u32 seen, m;\n @q bra again;\n"
+        "{\n .reg .pred p, q;\n .reg .u32 n, m;\n mov.u32 n, %3;\n"
+        "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra there;\n sub.u32 n, n, 1;\n and.b32 m, n, %4;\n setp.ne.u32 q, m, 0;\n @q bra again;\n"
+        " ld.volatile.shared.u32 m, [%5];\n setp.eq.u32 q, m, 0;\n @q bra there;\n setp.ne.u32 q, n, 0;\n @q bra again;\n"
         "there:\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
-        : "r"(sa(bar)), "r"(parity), "n"(kPolls - 1), "r"(sa(&sh.beat)), "n"(0u - kPolls)
+        : "r"(sa(bar)), "r"(parity), "n"(kPolls * kRounds), "n"(kPolls - 1), "r"(sa(const_cast<uint32_t *>(&longer)))
         : "memory");
-    if (!ok) sh.failed = 1;
+    if (!ok) sh.going = 0;
     return ok != 0;
   };
   // For waits that are long by design: a warp that polls takes issue slots from the softmax warps of its scheduler (the ticket warp alone
-  // cost a third of the rate).
-  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns) {
-    uint32_t ok = 0, seen = 0;
-    for (uint32_t n = 1;; ++n) {
+  // cost a third of the rate). That one waits for whole items, which may have millions of positions.
+  auto wait_idle = [&](uint64_t *bar, uint32_t parity, uint32_t ns, bool item = false) {
+    uint32_t ok = 0;
+    for (uint32_t n = 0; !ok && n < ((item ? sh.going : sh.slow) ? kLongPolls : item ? 0 : kPolls); ++n) {
       asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(sa(bar)), "r"(parity) : "memory");
-      if (ok) break;
-      __nanosleep(ns);
-      if (n % kPolls == 0) {
-        const uint32_t now = *const_cast<volatile uint32_t *>(&sh.beat);
-        if (now == seen) break;
-        seen = now;
-      }
+      if (!ok) __nanosleep(ns);
     }
-    if (!ok) sh.failed = 1;
+    if (!ok) sh.going = 0;
     return __all_sync(0xffffffffu, ok) != 0;
   };
-  auto wait_warp = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };  // the lanes agree
+  auto wait_warp = [&](uint64_t *bar, uint32_t parity, const volatile uint32_t &longer) { return __all_sync(0xffffffffu, wait(bar, parity, longer)) != 0; };  // the lanes agree
 
   // Item k of this CTA; null when the wait ran out.
-  auto item = [&](uint32_t k) { return wait_warp(&sh.item_full[k & 1], k >> 1 & 1) ? &sh.items[k & 1] : nullptr; };
+  auto item = [&](uint32_t k) { return wait_warp(&sh.item_full[k & 1], k >> 1 & 1, sh.going) ? &sh.items[k & 1] : nullptr; };
   auto item_done = [&](uint32_t k) {
     __syncwarp();
     if (lane == 0) arrive(sa(&sh.item_empty[k & 1]));
@@ -246,7 +242,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
         const uint32_t lanes = (quad * 32u) << 16, s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * DP;
         float top = -INFINITY, ref = 0.f, sum = 0.f;  // the reference, and what is subtracted from scaled scores (0 where it is -infinity)
         for (uint32_t t = bi; t < ei; ++t, scores ^= 1) {
-          if (!(ok = wait_warp(&s_full[i], scores))) break;
+          if (!(ok = wait_warp(&s_full[i], scores, sh.slow))) break;
           tc_after();
           uint32_t u[128];
           tmem_ld128(s_t, u);
@@ -289,7 +285,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
           // The special function unit of a scheduler belongs to one tile's warp at a time: the other's products run meanwhile.
           const bool shared_tile = tiles == 2 && t >= both_b && t < both_e;
           if (shared_tile && (i || t > both_b)) {
-            if (!(ok = wait_warp(&sh.turn[i][quad], turn))) break;
+            if (!(ok = wait_warp(&sh.turn[i][quad], turn, sh.slow))) break;
             turn ^= 1;
           }
           const uint64_t scale2 = pair_of(scale, scale), ref2 = pair_of(kRaise<BF> - ref, kRaise<BF> - ref);
@@ -321,7 +317,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
           __syncwarp();
           if (lane == 0) arrive(sa(&p_full[i][1]));
         }
-        if (ok) ok = wait_warp(&o_full[i], output);
+        if (ok) ok = wait_warp(&o_full[i], output, sh.slow);
         output ^= 1;
         if (ok) {
           tc_after();
@@ -368,7 +364,8 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
           }
           uint32_t again = __ballot_sync(0xffffffffu, finite != 0.f && r < packed);  // NaN
           __syncwarp();
-          for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP, &sh.beat);
+          if (again) sh.slow = 1;
+          for (; again; again &= again - 1) row_again<BF>(p, at, kvh, at.first + warp * 32 + __ffs(again) - 1, 0, DP);
         }
       }
       if (i == 0 && tiles == 2 && both_e > both_b) turn ^= 1;  // the other tile's last turn, which nobody waits for
@@ -427,7 +424,6 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
         const uint32_t copied = last > first ? last - first - (r1 > r0 && box ? 1 : 0) : 0;
         if (t1 - t == min(t1 - t0, 2u) && lane == 0) arrive(sa(&sh.fetched));  // the next ticket may be taken
         if (x >= C::kStages && !(ok = wait_idle(&empty[pos.s], pos.phase ^ 1, 64))) break;
-        get_on(&sh.beat);
         const uint32_t dst = ring_a + pos.s * C::kTile, bar = sa(&full[pos.s]);
         const bool pieces = r1 > r0;
         if (copied) {
@@ -466,7 +462,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       if (late) landed();
       item_done(k);
     }
-    if (sh.failed && lane == 0) {  // nothing may land when the CTA has gone
+    if (!sh.going && lane == 0) {  // nothing may land when the CTA has gone
       for (uint32_t y = x > C::kStages ? x - C::kStages : 0; y < x; ++y)
         if ((y & 1) == values) mbar_wait_short(sa(&full[y % C::kStages]), y / C::kStages & 1);
     }
@@ -482,7 +478,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       RingPos<(int)C::kStages> keys, vals;  // a tile's keys are an even request, its values the one behind
       vals.next();
       for (uint32_t k = 0; ok; ++k) {
-        if (!(ok = wait(&sh.item_full[k & 1], k >> 1 & 1))) break;
+        if (!(ok = wait(&sh.item_full[k & 1], k >> 1 & 1, sh.going))) break;
         const Item &it = sh.items[k & 1];
         if (!it.found) break;
         const uint32_t tiles = it.tiles, b[2] = {it.b[0], it.b[1]}, e[2] = {it.e[0], it.e[1]}, t0 = b[0], t1 = e[1];  // registers: the loops over i are unrolled
@@ -490,7 +486,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
         for (uint32_t n = 0; ok && n <= t1 - t0; ++n) {
           const uint32_t t = t0 + n;
           bool waited = false;
-          if (n > 0 && !(ok = wait(&full[vals.s], vals.phase))) break;
+          if (n > 0 && !(ok = wait(&full[vals.s], vals.phase, sh.slow))) break;
 #pragma unroll
           for (uint32_t i = 0; i < 2; ++i) {
             if (!ok || i >= tiles) break;
@@ -499,7 +495,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
               p_phase ^= 1u << i;
 #pragma unroll
               for (uint32_t half = 0; half < 2; ++half) {
-                if (!(ok = wait(&p_full[i][half], parity))) break;
+                if (!(ok = wait(&p_full[i][half], parity, sh.slow))) break;
                 tc_after();
 #pragma unroll
                 for (uint32_t k = half * 4; k < half * 4 + 4; ++k)
@@ -511,10 +507,10 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
             if (n > 0 && i + 1 == tiles) mma_commit(sa(&empty[vals.s]));
             if (t < t1 && t >= b[i] && t < e[i]) {
               if (t == b[i]) {
-                if (!(ok = wait(&q_full[i], q_phase >> i & 1))) break;
+                if (!(ok = wait(&q_full[i], q_phase >> i & 1, sh.slow))) break;
                 q_phase ^= 1u << i;
               }
-              if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;
+              if (!waited && !(ok = wait(&full[keys.s], keys.phase, sh.slow))) break;
               waited = true;
               tc_after();
               const uint32_t st = k0 + keys.s * (C::kTile >> 4), qi = q0 + i * (C::kTile >> 4);
@@ -529,7 +525,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
           }
           if (!ok) break;
           if (t < t1) {
-            if (!waited && !(ok = wait(&full[keys.s], keys.phase))) break;  // nobody sees it (between windows): still given back
+            if (!waited && !(ok = wait(&full[keys.s], keys.phase, sh.slow))) break;  // nobody sees it (between windows): still given back
             mma_commit(sa(&empty[keys.s]));
             keys.next(), keys.next();
           }
@@ -546,10 +542,9 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
   } else {
     // ------------------------------------------------- what comes next, once two tiles of this item are left to request: a ticket taken much earlier
     // could have been another CTA's, which has nothing left to do (106 -> 158 us for a few long items)
-    if (blockIdx.x == 0) check_rows(p, &sh.beat);
+    if (blockIdx.x == 0) check_rows(p);
     uint32_t used[2] = {};  // how often each tile's place for Q
     Walk walk;
-    walk.beat = &sh.beat;
     uint32_t ticket = blockIdx.x;  // the first ones are dealt out
     auto take = [&]() {
       uint32_t next = 0;
@@ -557,8 +552,8 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       return __shfl_sync(0xffffffffu, next, 0);
     };
     for (uint32_t k = 0;; ++k) {
-      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200)) break;
-      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200)) break;
+      if (k >= 1 && !wait_idle(&sh.fetched, k + 1 & 1, 200, true)) break;
+      if (k >= 2 && !wait_idle(&sh.item_empty[k & 1], (k >> 1) + 1 & 1, 200, true)) break;
       if (k) ticket = take();
       Item it = {};
       for (;; ticket = take()) {
@@ -592,7 +587,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       // and is not stored), else piece by piece
       bool ok = true;
       for (uint32_t i = 0; ok && i < it.tiles; ++i) {
-        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64))) break;
+        if (used[i] && !(ok = wait_idle(&sh.q_empty[i], used[i] + 1 & 1, 64, true))) break;
         ++used[i];
         const uint32_t dst = q_a + i * C::kTile, bar = sa(&q_full[i]), r0 = it.at.first + i * kRows;
         if (q_box) {
@@ -621,7 +616,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
       }
       if (!ok) break;
     }
-    if (sh.failed && lane == 0) {  // nothing may land when the CTA has gone
+    if (!sh.going && lane == 0) {  // nothing may land when the CTA has gone
       for (uint32_t i = 0; i < 2; ++i)
         if (used[i]) mbar_wait_short(sa(&q_full[i]), used[i] + 1 & 1);
     }
@@ -629,7 +624,7 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
   tc_before();
   __syncthreads();
   tc_after();
-  if (tid == 0 && sh.failed) raise(p.error, kWaitCode);
+  if (tid == 0 && !sh.going) raise(p.error, kWaitCode);
   stamp_end(p.stamps);
   if (tid == 0) {
     __threadfence();

@@ -41,12 +41,7 @@ __device__ __forceinline__ uint32_t rows_here(const PagedAttention &p, uint32_t 
 struct Walk {
   uint32_t from = 0;    // sequences in front, a multiple of 32
   uint64_t before = 0;  // their tiles
-  uint32_t *beat = nullptr;
 };
-// One lane of a warp that is getting on with work of any length counts it up in shared memory, for waits that give up where nothing moves.
-__device__ __forceinline__ void get_on(uint32_t *beat) {
-  if (beat && (threadIdx.x & 31) == 0) atomicAdd(beat, 1u);
-}
 __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per, uint32_t rows, uint32_t index, Place &at, Walk &walk) {
   const uint32_t lane = threadIdx.x & 31;
   bool bad = false;
@@ -79,26 +74,21 @@ __device__ __forceinline__ bool find_tile(const PagedAttention &p, uint32_t per,
       at.len = p.lengths[at.seq];
       return true;
     }
-    if (p.n > 32) before += __shfl_sync(0xffffffffu, up, 31), get_on(walk.beat);
+    if (p.n > 32) before += __shfl_sync(0xffffffffu, up, 31);
   }
   return false;
 }
 // Starts and lengths that do not belong together are reported by the first CTA's first warp.
-__device__ __forceinline__ void check_rows(const PagedAttention &p, uint32_t *beat = nullptr) {
+__device__ __forceinline__ void check_rows(const PagedAttention &p) {
   bool bad = false;
-  for (uint32_t i0 = 0; i0 < p.n; i0 += 32) {
-    const uint32_t i = i0 + (threadIdx.x & 31);
-    if (i < p.n) fresh_rows(p, i, bad);
-    if (i0) get_on(beat);
-  }
+  for (uint32_t i = threadIdx.x & 31; i < p.n; i += 32) fresh_rows(p, i, bad);
   if (bad) raise(p.error, PAGED_BAD_ROWS);
 }
 
 // Dimensions [d0, d1) of one packed row by a warp, from the definition in fp32. In the tiles' second product a position that a row does not see has the
 // probability 0, and 0 times an infinity or a NaN in that position's value is NaN: rows that come out of it not finite are computed
 // again here, from the positions that they see. (So a value that is not finite costs time, and reaches only the rows that see it.)
-template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &p, const Place &at, uint32_t kvh, uint32_t packed, uint32_t d0, uint32_t d1,
-                                                                uint32_t *beat = nullptr) {
+template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &p, const Place &at, uint32_t kvh, uint32_t packed, uint32_t d0, uint32_t d1) {
   const uint32_t lane = threadIdx.x & 31, per = p.heads / p.kv_heads, t = packed / per, h = kvh * per + packed - t * per;
   const uint32_t pos = at.len - at.fresh + t, first = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0;
   const uint16_t *q = static_cast<const uint16_t *>(p.q) + (at.row0 + t) * p.q_ld + h * p.dim;
@@ -106,7 +96,6 @@ template <bool BF> __device__ __noinline__ void row_again(const PagedAttention &
   float m = -INFINITY, l = 0.f;
   float2 o[4] = {};  // dimensions lane * 2 + 64 i
   for (uint32_t j0 = first; j0 <= pos; j0 += 32) {
-    get_on(beat);
     const uint32_t j = j0 + lane;
     bool there = j <= pos;
     size_t row = 0;
