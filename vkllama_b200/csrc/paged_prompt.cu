@@ -5,7 +5,7 @@
 // The query heads of a key head share its keys and values, so a tile's rows are (row, head of the group) pairs, 64 of them: with
 // grouped heads a tile has fewer rows of the sequence and the same use of every key that is fetched. One CTA of four warps has a tile;
 // keys and values come through shared memory by cp.async, two tiles ahead, and both products run on mma.sync (m16n8k16, fp32 sums) with
-// a running maximum and sum per row. Probabilities are rounded to 16 bits for the second product, as its operand has to be (relative
+// a running maximum and sum per row (Milakov and Gimelshein, 2018). Probabilities are rounded to 16 bits for the second product, as its operand has to be (relative
 // 2^-11 or 2^-8 each, as much as the rounding of the output); their sum is taken before. In fp16 they are 2^14 times as large, in sum and output
 // alike, because the format ends at steps of 2^-24: so 2^-11 holds down to 2^-28 of the row's largest, and below each is off by 2^-39 of
 // the largest at most. Positions that a row does not see are masked
@@ -14,7 +14,8 @@
 //
 // It has what the tcgen05 kernel (paged_prompt_tc.cu) would leave mostly empty, and heads above 128: sequences of few rows that see few positions, where
 // the start and end of a CTA are what there is, so three of them share an SM. 64 prompts of 64 rows, 32 heads of 128: 67 us, 2.0 TB/s; four of
-// 64 rows 9 us. On long prompts its products run at 210 TFLOP/s (fp32 sums of mma.sync; 4096 rows 658 us, tcgen05 137).
+// 64 rows 10 us. On long prompts its products run at 210 TFLOP/s (fp32 sums of mma.sync; 4096 rows, 32 heads of 128, 658 us, tcgen05 137 on a cool GPU and
+// 163 under full load; 16 heads of 200 or 256, which have no other kernel, 570 and 565).
 #include <algorithm>
 
 #include "common.cuh"

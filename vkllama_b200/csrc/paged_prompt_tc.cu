@@ -5,7 +5,8 @@
 // written over S_i in TMEM, O_i += P_i V_j with P as the TMEM operand. The two tiles of rows take turns: while the tensor core works
 // for one, the exponentials of the other are computed, which take as long (16 per clock and SM: 1024 cycles for 128 x 128, like the two
 // products). A CTA stays on its SM and takes one such item after the other by tickets, what takes longest first: a new CTA per item costs some
-// 10 us of start and end, in which nothing else runs (64 prompts of 256: 210 us, this way 107). Warps:
+// 10 us of start and end, in which nothing else runs (64 prompts of 256: 210 us, this way 106; both on a cool GPU, under full load 123). That a reference
+// follows its maximum only after some growth, and that two tiles of rows take turns, are published ways of attention on tensor cores. Warps:
 //   0-3, 4-7  softmax of tile 0, 1: one thread per row, so no exchange between threads. The reference is the row's maximum as of the last time
 //             that it grew by more than 2^8 (fp16: 2^4): until then the probabilities stay below that and O as it is; only then O is multiplied. In fp16,
 //             which ends at steps of 2^-24, they are 2^11 times as large, in sum and O alike: their rounding is relative (2^-11) down to 2^-25

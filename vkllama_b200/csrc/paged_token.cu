@@ -17,7 +17,8 @@
 // moved to its border.
 //
 // A warp streams its range through a ring of its own (cp.async, tiles of keys and of values alternating, swizzled for ldmatrix):
-// no barrier inside the stream, the next pages are looked up a tile ahead. Rows that are not visible are not read and count as zeros.
+// no barrier inside the stream, the next pages are looked up a tile ahead. Maximum and sum run along in one pass (Milakov and Gimelshein, Online normalizer
+// calculation for softmax, 2018). Rows that are not visible are not read and count as zeros.
 //
 // Measured on sequences that hold 0.37 GB together (57 us at the rate of a copy): 70 ... 78 us, 4.9 ... 5.3 TB/s, with up to eight heads to a
 // key head whatever the width, the page and the lengths; 76 us with 12 or 16 heads of 128, 93 us with 16 of 256 (shared memory and the
@@ -41,7 +42,7 @@ constexpr uint32_t kSnapRows = 256, kSnapRowsShort = 512, kShortRows = 1024;
 // positions, 32 heads of 128 on 2 key heads, 21.8 and 14.9; three of 2500, 16 heads of 256 on one, 35 and 26; four of 2000, 16 of 256 on 2, 26 and 19.
 constexpr uint32_t kWideRows = 128, kSnapRowsShort256 = 256;
 // Parts of a pair that one CTA adds up, and how many it does at a time; of more, every kGroup are added up first (one sequence of 60,000 positions, 16 heads of 128
-// on one key head, 148 parts: 55 us by one CTA, this way 29).
+// on one key head, 148 parts: 55 us by one CTA, this way 26).
 constexpr uint32_t kJoin = 32, kGroup = 16, kAtOnce = 8;
 constexpr uint32_t kPairCost = 1;             // what a pair costs beside its tiles (queries, output, short rows in the ring), in tiles
 constexpr float kRaise = 14.f;                // fp16 probabilities are 2^14 times as large; 2^16 is left for one that its exponent's rounding takes above 1
