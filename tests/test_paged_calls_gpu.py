@@ -57,6 +57,20 @@ def test_time_of_a_run_that_is_over_while_others_are_queued(dev):
     assert 2 <= op.time() < 1000 and 2 <= other.time() < 1000
 
 
+def test_time_when_the_command_is_gone(dev):
+    rng, cmd = np.random.default_rng(20), vk.Command(dev)
+    c = Cache(rng, [30000], 2, 128, 16, vk.FP16)
+    with cmd:
+        k, v, table, lens = c.up(cmd, dev)
+        q, op = tensor(cmd, dev, draw(rng, (1, 256), vk.FP16), vk.FP16), vk.PagedAttention(dev, cmd, 2, 2, 128, 16).init()
+        op(q, k, v, table, lens)
+    cmd.begin()
+    op(q, k, v, table, lens)  # its end waits for this
+    cmd.end()
+    cmd.close()
+    assert 2 <= op.time() < 1000
+
+
 def test_a_shape_that_is_captured_first(dev):
     """Its workspace is zero for the first direct call too, which comes before any replay."""
     torch = pytest.importorskip("torch")

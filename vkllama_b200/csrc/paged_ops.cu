@@ -35,13 +35,15 @@ struct OwnStream {
 
 struct PagedOp : vkl_op {
   vkl_tensor *stamps = nullptr;  // of the last launch (paged.h), in the place of the other ops' events
-  uint64_t run_in = 0;           // the command's waits before the last launch
+  std::shared_ptr<std::atomic<uint64_t>> waits;  // the command's
+  uint64_t run_in = 0;                           // what they were at the last launch
   using vkl_op::vkl_op;
   ~PagedOp() override { vkl_tensor_release(stamps); }
   int paged_init() {
     if (!dev || !cmd) return fail(VKL_INVALID_ARGUMENT, "op: null device or command");
     VKL_OKAY(ensure_tensor(dev, &stamps, 1, 1, 4, VKL_UINT32));
     VKL_CUDA(cudaMemsetAsync(stamps->data(), 0, 16, cmd->stream));
+    waits = cmd->waits;
     uint32_t *word;
     VKL_OKAY(command_error_word(cmd, &word));  // allocated here, so that run() does not have to
     inited = true;
@@ -53,14 +55,14 @@ struct PagedOp : vkl_op {
   }
   unsigned long long *stamp() {
     timed = true;
-    run_in = cmd->waits;
+    run_in = *waits;
     return (unsigned long long *)stamps->data();
   }
   int elapsed(uint64_t *usec) override {
     *usec = 0;
     if (!timed) return VKL_OK;
     OnDevice here(dev->ordinal);
-    if (cmd->waits == run_in) {  // not waited for since: over where the stream has nothing left
+    if (*waits == run_in) {  // not waited for since (so the command is there): over where its stream has nothing left
       cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;  // a query would end a capture
       if (cudaStreamIsCapturing(cmd->stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone || cudaStreamQuery(cmd->stream) != cudaSuccess) {
         (void)cudaGetLastError();

@@ -376,6 +376,7 @@ int vkl_command_create(vkl_device *dev, vkl_command **out) {
 int vkl_command_destroy(vkl_command *cmd) {
   if (!cmd) return VKL_OK;
   cudaStreamSynchronize(cmd->stream);
+  ++*cmd->waits;
   for (auto &f : cmd->deferred) f();
   if (cmd->err_word) cmd->dev->release(cmd->err_word, 256);
   if (cmd->err_host) cudaFreeHost(cmd->err_host);
@@ -425,7 +426,7 @@ int vkl_command_wait(vkl_command *cmd) {
   cmd->deferred.clear();
   for (auto &f : tasks) f();
   if (e != cudaSuccess) return fail(VKL_INTERNAL, "command_wait: %s", cudaGetErrorString(e));
-  ++cmd->waits;
+  ++*cmd->waits;
   if (watched && *cmd->err_host) {
     cudaMemsetAsync(cmd->err_word, 0, 4, cmd->stream);
     switch (*cmd->err_host) {

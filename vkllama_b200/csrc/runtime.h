@@ -117,7 +117,8 @@ struct vkl_command {
   uint32_t *err_word = nullptr;  // device word raised by a kernel whose bounded wait ran out; read by wait()
   uint32_t *err_host = nullptr;  // pinned: where it is read to
   bool err_used = false;
-  uint64_t waits = 0;            // how often wait() has found everything over
+  // How often everything so far was found over, by wait() or at the end; ops ask it when the command may be gone.
+  std::shared_ptr<std::atomic<uint64_t>> waits = std::make_shared<std::atomic<uint64_t>>(0);
 };
 
 namespace vkl {
