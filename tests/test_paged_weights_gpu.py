@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import vkllama_b200 as vk
-from paged_weights import LONG_STEPS, Cache, Sink, draw, near, tensor, to_values
+from paged_weights import LONG_STEPS, Cache, Sink, draw, near, tensor, to_bits, to_values, tolerance
 
 pytestmark = pytest.mark.gpu
 GAPS = [14.0, 17.0, 18.0, 20.0]
@@ -73,3 +73,37 @@ def test_long_sequences_lack_no_tile(dev, dtype):
     for past, new, heads, dim, kernel in ((2999, 1, 3, 128, "tensor"), (2700, 300, 2, 128, "tensor"), (898, 2, 2, 200, "rows")):
         c = Cache(np.random.default_rng(dim), [past + new], 1, dim, 16, dtype)
         rows(dev, c, [past], [new], heads, kernel, 0.0, q=draw(np.random.default_rng(2), (new, heads * dim), dtype))
+
+
+@pytest.mark.parametrize("dtype", [vk.FP16, vk.BF16])
+@pytest.mark.parametrize("tokens,kv,dim,kernel,window", [(1 << 20, 160, 64, "tensor", 0), (1 << 21, 8, 64, "tensor", 0), (150000, 150, 128, "tensor", 0), (400000, 150, 80, "tensor", 300000), (1 << 20, 20, 136, "rows", 0)])
+def test_sums_over_many_positions(dev, dtype, tokens, kv, dim, kernel, window):
+    """Values of one sign, weights that grow along the way: what the matrix units cut off their sums adds up. Two pages, again and again; positions of a CTA
+    of its own, and in slices of many tiles."""
+    page, rows = 128, 3
+    rng, cmd = np.random.default_rng(dim), vk.Command(dev)
+    k, v = 0.3 * rng.standard_normal((2, kv, page, dim)), 1 + rng.random((2, kv, page, dim))
+    k[1, :, :, 0] += 4  # the second page's scores are higher
+    k, v = to_bits(k, dtype), to_bits(v, dtype)
+    q = 0.3 * rng.standard_normal((rows, kv, dim))
+    q[:, :, 0] = np.sqrt(dim)
+    q = to_bits(q, dtype)
+    width = -(-tokens // page)
+    table = np.repeat(np.array([0, 1], np.uint32), [width // 3, width - width // 3])
+    with cmd:
+        op = vk.PagedAttention(dev, cmd, kv, kv, dim, page, 0.0, window, dtype).init()
+        args = [tensor(cmd, dev, a.reshape(2, kv * page, dim), dtype) for a in (k, v)]
+        args += [tensor(cmd, dev, a.astype(np.uint32)) for a in (table[None], np.array([tokens]), np.array([0, rows]))]
+        got = to_values(cmd.download(op(tensor(cmd, dev, q.reshape(rows, -1), dtype), *args)), dtype).reshape(rows, kv, dim)
+    k, v, q = (to_values(a, dtype) for a in (k, v, q))
+    for r in range(rows):
+        last = tokens - rows + r
+        j = np.arange(max(0, last + 1 - window) if window else 0, last + 1)
+        times = np.bincount(table[j // page].astype(int) * page + j % page, minlength=2 * page).reshape(2, 1, page)
+        s = np.einsum("pkjd,kd->pkj", k, q[r]) / np.sqrt(dim)
+        w = times * np.exp(s - s.max((0, 2), keepdims=True))
+        mass = np.einsum("pkj,pkjd->kd", w, v) / w.sum((0, 2))[:, None]  # all values are positive: also the output
+        size = (np.einsum("pkjd,kd->pkj", np.abs(k), np.abs(q[r])) / np.sqrt(dim)).max((0, 2))[:, None]
+        den = w.sum((0, 2))[:, None]
+        tol = tolerance(mass, mass, size, den, dtype, dim, tokens, 2.0, kernel, steps=2048 + tokens / 32768)
+        assert (np.abs(got[r] - mass) <= tol).all(), (r, np.abs((got[r] - mass) / tol).max(), ((got[r] - mass) / mass).mean())

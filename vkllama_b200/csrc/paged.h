@@ -104,6 +104,10 @@ struct PagedUpdate {
 };
 cudaError_t launch_paged_update(const PagedUpdate &p, cudaStream_t s);
 
+// The matrix units cut their fp32 sums off instead of rounding them: what they add up themselves comes out low, by 0.014 % over this many positions of equal
+// weight and values of one sign, by 0.65 % over a million. Where a prompt's rows see more, sums of fewer are added up by ordinary additions.
+constexpr uint32_t kManyPositions = 32768;
+
 struct PagedAttention {
   const void *q;                // [rows] of heads * dim values, q_ld apart
   const void *kcache, *vcache;
@@ -124,6 +128,7 @@ struct PagedAttention {
   bool bf, count;               // count (one token): the tables could hold more tiles than 31 bits count, so the lengths have to be added up first
   uint32_t splits;              // parts of a sequence's positions at most
   uint32_t part;                // of a prompt call's sequences, those that the launch takes: 0 all, 1 or 2 by paged_rows.cuh's rule
+  float *aside;                 // prompts, tables beyond kManyPositions: sums so far, paged_prompt_aside() bytes; else null
 };
 // One new token per sequence.
 cudaError_t launch_paged_token(const PagedAttention &p, uint32_t sms, cudaStream_t s);
@@ -135,6 +140,7 @@ cudaError_t launch_paged_prompt(const PagedAttention &p, uint32_t sms, cudaStrea
 cudaError_t setup_paged_prompt();
 // The same on tcgen05, heads up to 128 wide.
 uint32_t paged_prompt_splits(const PagedAttention &p, uint32_t sms);
+size_t paged_prompt_aside(uint32_t dim, uint32_t sms);
 cudaError_t launch_paged_prompt_tc(const PagedAttention &p, uint32_t sms, cudaStream_t s);
 cudaError_t launch_paged_prompt_join(const PagedAttention &p, cudaStream_t s);  // where splits > 1, behind it
 cudaError_t setup_paged_prompt_tc();

@@ -252,13 +252,13 @@ struct UpdatePagedOp : PagedOp {
 struct PagedAttentionOp : PagedOp {
   int heads, kv_heads, dim, page, window, dtype;
   float scale;
-  vkl_tensor *out = nullptr, *scratch = nullptr, *counters = nullptr, *part_o = nullptr, *part_ml = nullptr;
+  vkl_tensor *out = nullptr, *scratch = nullptr, *counters = nullptr, *part_o = nullptr, *part_ml = nullptr, *aside = nullptr;
   vkl_tensor *older[64];  // smaller part_o and part_ml, which captured calls go on using
   int n_older = 0;
   PagedAttentionOp(vkl_device *d, vkl_command *c, int h, int kv, int dm, int pg, float s, int w, int dt)
       : PagedOp(d, c), heads(h), kv_heads(kv), dim(dm), page(pg), window(w), dtype(dt), scale(s) {}
   ~PagedAttentionOp() override {
-    for (vkl_tensor *t : {out, scratch, counters, part_o, part_ml}) vkl_tensor_release(t);
+    for (vkl_tensor *t : {out, scratch, counters, part_o, part_ml, aside}) vkl_tensor_release(t);
     while (n_older) vkl_tensor_release(older[--n_older]);
   }
   int init() override {
@@ -342,6 +342,10 @@ struct PagedAttentionOp : PagedOp {
         VKL_OKAY(room(&part_o, parts * (dim <= 64 ? 64 : 128)));
         VKL_OKAY(room(&part_ml, parts * 2));
         p.part_o = (float *)part_o->data(), p.part_ml = (float2 *)part_ml->data();
+      }
+      if (starts && dim <= 128 && table->w * page > kManyPositions) {
+        VKL_OKAY(ensure_tensor(dev, &aside, 1, 1, paged_prompt_aside(dim, sms) / 4, VKL_FP32));
+        p.aside = (float *)aside->data();
       }
       VKL_LAUNCH(starts ? paged_prompt_launches(p) : 1, starts ? launch_paged_prompt(p, sms, cmd->stream) : launch_paged_token(p, sms, cmd->stream));
     }

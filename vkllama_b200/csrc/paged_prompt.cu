@@ -34,7 +34,9 @@ template <int DP> struct Cfg {
   static constexpr uint32_t kSmem = 2 * 2 * kKeys * DP * 2;
 };
 
-template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 3) paged_prompt_kernel(const PagedAttention p) {
+// MANY: tables that hold more than kManyPositions (paged_rows.cuh). The other widths have no more than 128 positions here, or the tcgen05 kernel takes them. (One
+// kernel for both: 4096 rows, 16 heads of 256, 574 us instead of 565.)
+template <bool BF, int DP, bool MANY = false> __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 3) paged_prompt_kernel(const PagedAttention p) {
   using C = Cfg<DP>;
   constexpr uint32_t CH = DP / 8, KT = C::kKeys;
   constexpr int KS = DP / 16, NT = DP / 8, SN = KT / 8;
@@ -175,16 +177,37 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256
         s[n][e] = exp2f(s[n][e] - from[e >> 1]);
         sum[e >> 1] += s[n][e];
       }
+    if (MANY && t1 - t0 > kManyPositions / KT) {
+      uint32_t a[KT / 16][4];
 #pragma unroll
-    for (int k = 0; k < (int)KT / 16; ++k) {
-      const uint32_t a0 = pack2<BF>(s[2 * k][0], s[2 * k][1]), a1 = pack2<BF>(s[2 * k][2], s[2 * k][3]);
-      const uint32_t a2 = pack2<BF>(s[2 * k + 1][0], s[2 * k + 1][1]), a3 = pack2<BF>(s[2 * k + 1][2], s[2 * k + 1][3]);
+      for (int k = 0; k < (int)KT / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[k][e] = pack2<BF>(s[2 * k + (e >> 1)][2 * (e & 1)], s[2 * k + (e >> 1)][2 * (e & 1) + 1]);
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
-        uint32_t b[4];
-        ldmatrix4_t(b, vt + ((k * 16 + lrow + (lsel & 1) * 8) * CH + ((n + (lsel >> 1)) ^ lrow)) * 16);
-        mma2<BF>(o[n], a0, a1, a2, a3, b[0], b[1]);
-        mma2<BF>(o[n + 1], a0, a1, a2, a3, b[2], b[3]);
+        float x[4] = {}, y[4] = {};
+#pragma unroll
+        for (int k = 0; k < (int)KT / 16; ++k) {
+          uint32_t b[4];
+          ldmatrix4_t(b, vt + ((k * 16 + lrow + (lsel & 1) * 8) * CH + ((n + (lsel >> 1)) ^ lrow)) * 16);
+          mma2<BF>(x, a[k][0], a[k][1], a[k][2], a[k][3], b[0], b[1]);
+          mma2<BF>(y, a[k][0], a[k][1], a[k][2], a[k][3], b[2], b[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] += x[e], o[n + 1][e] += y[e];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < (int)KT / 16; ++k) {
+        const uint32_t a0 = pack2<BF>(s[2 * k][0], s[2 * k][1]), a1 = pack2<BF>(s[2 * k][2], s[2 * k][3]);
+        const uint32_t a2 = pack2<BF>(s[2 * k + 1][0], s[2 * k + 1][1]), a3 = pack2<BF>(s[2 * k + 1][2], s[2 * k + 1][3]);
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t b[4];
+          ldmatrix4_t(b, vt + ((k * 16 + lrow + (lsel & 1) * 8) * CH + ((n + (lsel >> 1)) ^ lrow)) * 16);
+          mma2<BF>(o[n], a0, a1, a2, a3, b[0], b[1]);
+          mma2<BF>(o[n + 1], a0, a1, a2, a3, b[2], b[3]);
+        }
       }
     }
     __syncthreads();  // everyone is through with the tile
@@ -214,8 +237,8 @@ template <bool BF, int DP> __global__ void __launch_bounds__(kThreads, DP == 256
   stamp_end(p.stamps);
 }
 
-template <bool BF, int DP> cudaError_t setup_one() {
-  return cudaFuncSetAttribute(paged_prompt_kernel<BF, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);
+template <bool BF, int DP, bool MANY = false> cudaError_t setup_one() {
+  return cudaFuncSetAttribute(paged_prompt_kernel<BF, DP, MANY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<DP>::kSmem);
 }
 template <bool BF> cudaError_t pick(const PagedAttention &p, cudaStream_t s) {
   // tiles are counted on the device; every sequence has at most one that is not full
@@ -223,13 +246,14 @@ template <bool BF> cudaError_t pick(const PagedAttention &p, cudaStream_t s) {
   const dim3 grid((uint32_t)(tiles * p.kv_heads));  // all heads of a tile, then the next tile
   if (p.dim <= 64) return launch_following(paged_prompt_kernel<BF, 64>, grid, kThreads, Cfg<64>::kSmem, s, p);
   if (p.dim <= 128) return launch_following(paged_prompt_kernel<BF, 128>, grid, kThreads, Cfg<128>::kSmem, s, p);
-  return launch_following(paged_prompt_kernel<BF, 256>, grid, kThreads, Cfg<256>::kSmem, s, p);
+  return launch_following(p.width * p.page.d > kManyPositions ? paged_prompt_kernel<BF, 256, true> : paged_prompt_kernel<BF, 256>, grid, kThreads, Cfg<256>::kSmem, s, p);
 }
 
 }  // namespace
 
 cudaError_t setup_paged_prompt() {
-  for (cudaError_t e : {setup_one<false, 64>(), setup_one<false, 128>(), setup_one<false, 256>(), setup_one<true, 64>(), setup_one<true, 128>(), setup_one<true, 256>()})
+  for (cudaError_t e : {setup_one<false, 64>(), setup_one<false, 128>(), setup_one<false, 256>(), setup_one<false, 256, true>(), setup_one<true, 64>(), setup_one<true, 128>(),
+                        setup_one<true, 256>(), setup_one<true, 256, true>()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }

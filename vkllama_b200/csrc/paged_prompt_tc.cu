@@ -32,6 +32,8 @@ constexpr uint32_t kWaitCode = 9, kPolls = 1u << 20, kRounds = 64, kLongPolls = 
 // Where there are fewer items than SMs, an item's positions are split, into slices of at least kSliceTiles tiles; the sums of a row's slices meet
 // in a kernel of their own.
 constexpr uint32_t kSliceTiles = 4, kMostSplits = 32;
+constexpr uint32_t kAsideTiles = kManyPositions / kKeys;
+template <int DP> constexpr uint32_t kAsideRow = DP + 4;  // numbers of a row's sums put aside: outputs, their reference, the sum of probabilities
 // Octaves that a maximum grows by before the reference follows, and that probabilities are raised by: together 2^15, of 2^16 that fp16 has. (Of normally
 // distributed scores, 32 rows of 4096 positions, 0.1 % of the tiles let O be multiplied; with 2^3 2.4 %, and 4096 rows take 165 us instead of 163.)
 template <bool BF> constexpr float kGrown = BF ? 8.0f : 4.0f;
@@ -142,21 +144,56 @@ __device__ __forceinline__ void store32(void *to, const uint32_t *v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
-// Sixteen columns times c.
-__device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
-  uint32_t u[16];
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&u)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]),
                  "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
                : "r"(taddr)
                : "memory");
+}
+// Sixteen columns times c.
+__device__ __forceinline__ void rescale16(uint32_t taddr, float c) {
+  uint32_t u[16];
+  tmem_ld16(taddr, u);
 #pragma unroll
   for (int x = 0; x < 16; ++x) u[x] = __float_as_uint(__uint_as_float(u[x]) * c);
   tmem_st16(taddr, u);
 }
 
-// SPLIT: p.splits > 1. (One kernel for both costs 0.4 us an item.)
-template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThreads, 1)
+// A row's sums, relative to `ref`, out of the way: added to what is there (unless this is the first time), and 0 from here on. Or back, added to what came since.
+template <int DP, bool BACK> __device__ __forceinline__ void put_aside(float *there, bool first, uint32_t o_t, float ref, float &sum) {
+  if (!first) {  // it has long left the caches
+#pragma unroll
+    for (uint32_t d = 0; d < DP + 2; d += 32) asm volatile("prefetch.global.L1 [%0];" ::"l"(there + d));
+  }
+  const float2 ml = first ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2 *>(there + DP);  // reference, sum of probabilities
+  const float c = ml.y == 0.f ? 0.f : exp2_fast(ml.x - ref);  // nothing was seen until then, and the reference stands for nothing
+  sum += ml.y * c;
+#pragma unroll 2
+  for (uint32_t d = 0; d < DP; d += 16) {
+    uint32_t u[16];
+    tmem_ld16(o_t + d, u);
+#pragma unroll
+    for (int x = 0; x < 16; x += 4) {
+      float4 *at = reinterpret_cast<float4 *>(there + d + x), v = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+      v.x = v.x * c + __uint_as_float(u[x]), v.y = v.y * c + __uint_as_float(u[x + 1]);
+      v.z = v.z * c + __uint_as_float(u[x + 2]), v.w = v.w * c + __uint_as_float(u[x + 3]);
+      if (!BACK) *at = v;
+      u[x] = BACK ? __float_as_uint(v.x) : 0, u[x + 1] = BACK ? __float_as_uint(v.y) : 0;
+      u[x + 2] = BACK ? __float_as_uint(v.z) : 0, u[x + 3] = BACK ? __float_as_uint(v.w) : 0;
+    }
+    tmem_st16(o_t + d, u);
+  }
+  tmem_stored();
+  if (!BACK) {
+    *reinterpret_cast<float2 *>(there + DP) = make_float2(ref, sum);
+    sum = 0.f;
+  }
+}
+
+// SPLIT: p.splits > 1. (One kernel for both costs 0.4 us an item.) MANY: p.aside, every kAsideTiles tiles a row's sums are added to what
+// lies there, in 32 bits as everywhere but rounded (bf16, 1024 rows behind 100,000 positions, 32 heads of 128 over 8: 1.5 % more on a cool GPU).
+template <bool BF, int DP, bool SPLIT, bool MANY> __global__ void __launch_bounds__(kThreads, 1)
     paged_prompt_tc_kernel(const PagedAttention p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const __grid_constant__ CUtensorMap map_q, const uint32_t box, const bool q_box) {
   using C = Cfg<DP>;
@@ -270,7 +307,9 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
             ref = m == -INFINITY ? 0.f : m * scale;
           } else {
             const bool grown = m * scale - ref > kGrown<BF> || (top == -INFINITY && m != -INFINITY);
-            if (__any_sync(0xffffffffu, grown)) {
+            const bool due = MANY && (t - bi) % kAsideTiles == 0;
+            if (__any_sync(0xffffffffu, grown || due)) {
+              if (due) put_aside<DP, false>(p.aside + ((size_t)blockIdx.x * kSoftmaxWarps * 32 + tid) * kAsideRow<DP>, t - bi == kAsideTiles, o_t, ref, sum);
               float c = 1.0f;
               if (grown) {
                 c = exp2_fast((top - m) * scale);
@@ -322,6 +361,8 @@ template <bool BF, int DP, bool SPLIT> __global__ void __launch_bounds__(kThread
         output ^= 1;
         if (ok) {
           tc_after();
+          if (MANY && bi + kAsideTiles < ei)
+            put_aside<DP, true>(p.aside + ((size_t)blockIdx.x * kSoftmaxWarps * 32 + tid) * kAsideRow<DP>, false, o_t, ref, sum);
           const float inv = 1.0f / sum;
           const uint32_t row = min(r, packed - 1), rt = quotient(row, p.group);
           const size_t to = (size_t)(at.row0 + rt) * p.heads + kvh * per + row - rt * per;
@@ -713,11 +754,13 @@ template <bool BF, int DP> cudaError_t run(const PagedAttention &p, uint32_t sms
     box = 0;
   const bool q_box = kRows % per == 0 && make_q_map<BF>(&map_q, p, (uint32_t)per);
   const dim3 grid((uint32_t)std::min<uint64_t>(sms, most_items(p) * p.splits));
-  return launch_following(p.splits > 1 ? paged_prompt_tc_kernel<BF, DP, true> : paged_prompt_tc_kernel<BF, DP, false>, grid, kThreads, Cfg<DP>::kSmem, s, p, map_k,
-                          map_v, map_q, box, q_box);
+  auto kernel = p.splits > 1 ? (p.aside ? paged_prompt_tc_kernel<BF, DP, true, true> : paged_prompt_tc_kernel<BF, DP, true, false>)
+                             : (p.aside ? paged_prompt_tc_kernel<BF, DP, false, true> : paged_prompt_tc_kernel<BF, DP, false, false>);
+  return launch_following(kernel, grid, kThreads, Cfg<DP>::kSmem, s, p, map_k, map_v, map_q, box, q_box);
 }
 template <bool BF, int DP> cudaError_t setup_one() {
-  for (auto kernel : {paged_prompt_tc_kernel<BF, DP, false>, paged_prompt_tc_kernel<BF, DP, true>}) {
+  for (auto kernel : {paged_prompt_tc_kernel<BF, DP, false, false>, paged_prompt_tc_kernel<BF, DP, true, false>, paged_prompt_tc_kernel<BF, DP, false, true>,
+                      paged_prompt_tc_kernel<BF, DP, true, true>}) {
     cudaFuncAttributes a;
     cudaError_t e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return e;
@@ -748,6 +791,7 @@ uint32_t paged_prompt_splits(const PagedAttention &p, uint32_t sms) {
     if (6 * waves(n) * best < 5 * waves(best) * n) best = n;
   return best;
 }
+size_t paged_prompt_aside(uint32_t dim, uint32_t sms) { return (size_t)sms * kSoftmaxWarps * 32 * (dim <= 64 ? kAsideRow<64> : kAsideRow<128>) * 4; }
 cudaError_t launch_paged_prompt_join(const PagedAttention &p, cudaStream_t s) {
   const dim3 grid((uint32_t)(((uint64_t)p.rows * p.heads + 7) / 8));
   if (p.dim <= 64) return launch_following(p.bf ? paged_prompt_join_kernel<true, 64> : paged_prompt_join_kernel<false, 64>, grid, 256, 0, s, p);
