@@ -240,9 +240,9 @@ int vkl_update_paged_kvcache_run(vkl_op *op, vkl_tensor *kcache, vkl_tensor *vca
  * kv_heads, query head h reads key head h / (heads / kv_heads). scale 0: 1 / sqrt(dim). window > 0: a token sees the last `window`
  * positions up to its own. fp32 sums and softmax, one rounding of the output. Probabilities are multiplied with the values as 16-bit numbers: with
  * `starts` one of dtype, off by up to 2^-8 (bf16) or 2^-11 (fp16) of itself; without, two that add up, 2^-16 or 2^-22. In fp16 each is also off by up to
- * 2^-36 (without `starts` 2^-39) of its row's largest. The matrix units cut sums of products off at 32 bits, every 16 positions; no more than
- * 32,768 positions are added up that way with `starts` (output at most 0.014 % low, where all have one weight and values of one sign), without what one warp of all
- * has of a sequence (0.06 % where a million positions and 160 key heads are a call).
+ * 2^-36 (without `starts` 2^-39) of its row's largest. The matrix units cut sums of products off at 32 bits, every 16 positions; with
+ * `starts` that is no more than 32,768 positions (the output at most 0.014 % low, where all have one weight and values of one sign), without `starts` the part
+ * of a sequence that one of the GPU's 1,184 warps has (0.06 % low in a call of a million positions and 160 key heads).
  *   starts NULL: one new token per sequence, q [1, n, heads * dim], row i the last token of sequence i (position lengths[i] - 1); a sequence
  *   of no tokens gives zeros. Up to 2^35 tokens of all sequences times key heads (times eights of query heads, where one has more than eight); the
  *   device refuses a call of more than it can count (OUT_OF_RANGE), by lengths, not by what the table could hold.

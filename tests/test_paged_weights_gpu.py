@@ -107,3 +107,24 @@ def test_sums_over_many_positions(dev, dtype, tokens, kv, dim, kernel, window):
         den = w.sum((0, 2))[:, None]
         tol = tolerance(mass, mass, size, den, dtype, dim, tokens, 2.0, kernel, steps=2048 + tokens / 32768)
         assert (np.abs(got[r] - mass) <= tol).all(), (r, np.abs((got[r] - mass) / tol).max(), ((got[r] - mass) / mass).mean())
+
+
+@pytest.mark.parametrize("dtype", [vk.FP16, vk.BF16])
+@pytest.mark.parametrize("dim,kv", [(64, 150), (128, 4), (136, 4)])
+def test_infinite_and_missing_numbers_behind_many_positions(dev, dtype, dim, kv):
+    """Before sums are put aside and behind; by rows that see them and by ones that do not."""
+    page, width, rows = 128, 1200, 2  # a page of ordinary values again and again, one with an infinity, a last one that ends with NaN
+    rng, cmd = np.random.default_rng(27), vk.Command(dev)
+    k, v = (draw(rng, (3, kv, page, dim), dtype) for _ in range(2))
+    inf, nan = (0x7c00, 0x7e00) if dtype == vk.FP16 else (0x7f80, 0x7fc0)
+    v[1, :, 5, 3], v[2, :, page - 1, 7] = inf, nan
+    table = np.zeros((1, width), np.uint32)
+    table[0, 1], table[0, -1] = 1, 2
+    q = draw(rng, (rows, kv * dim), dtype)
+    with cmd:
+        args = [tensor(cmd, dev, a.reshape(3, kv * page, dim), dtype) for a in (k, v)]
+        args += [tensor(cmd, dev, np.array(a, np.uint32)) for a in (table, [width * page], [0, rows])]
+        got = cmd.download(vk.PagedAttention(dev, cmd, kv, kv, dim, page, dtype=dtype).init()(tensor(cmd, dev, q, dtype), *args))
+    got = to_values(got, dtype).reshape(rows, kv, dim)
+    assert np.isposinf(got[:, :, 3]).all() and np.isfinite(got[0, :, 7]).all() and np.isnan(got[1, :, 7]).all()
+    assert np.isfinite(np.delete(got, [3, 7], 2)).all() and np.abs(np.delete(got, [3, 7], 2)).max() < 5
